@@ -13,6 +13,7 @@
 #include "common/logging.h"
 #include "common/runtime.h"
 #include "common/windows.h"
+#include "cuda/attn_tcgen05.h"
 #include "cuda/bn_kernels.h"
 #include "cuda/bucket.h"
 #include "cuda/combine_noalloc.h"
@@ -165,6 +166,56 @@ at::Tensor& GemmStatusWord(const at::Tensor& like) {
   static at::Tensor status;
   if (!status.defined()) status = at::zeros({1}, like.options().dtype(at::kInt));
   return status;
+}
+
+// The same for the attention kernels, one word per device (bits: AttnStatus).
+unsigned int* AttnStatusWord(int device) {
+  static std::mutex mu;
+  static std::map<int, at::Tensor> words;
+  std::lock_guard<std::mutex> lock(mu);
+  at::Tensor& w = words[device];
+  if (!w.defined()) w = at::zeros({1}, at::TensorOptions().device(at::kCUDA, device).dtype(at::kInt));
+  return reinterpret_cast<unsigned int*>(w.data_ptr<int>());
+}
+
+// Strides of a bf16 [tokens, heads, D] or [batch, tokens, heads, D] operand; extents of one have no stride of their own.
+AttnTensor ToAttn(const at::Tensor& t, const char* what) {
+  TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kBFloat16 && (t.dim() == 3 || t.dim() == 4) && t.numel() > 0,
+              what, " has to be a bf16 CUDA tensor [tokens, heads, D] or [batch, tokens, heads, D]");
+  const int64_t n = t.dim();
+  AttnTensor a;
+  a.ptr = t.data_ptr();
+  a.head_stride = t.size(n - 2) > 1 ? t.stride(n - 2) : (t.size(n - 1) + 7) / 8 * 8;
+  const bool one_token = t.size(n - 3) == 1 && (n == 3 || t.size(0) == 1);
+  a.token_stride = one_token ? t.size(n - 2) * a.head_stride : (t.size(n - 3) > 1 ? t.stride(n - 3) : t.stride(0));
+  TORCH_CHECK(t.stride(n - 1) == 1 && a.head_stride >= t.size(n - 1) && a.token_stride >= t.size(n - 2) * a.head_stride &&
+              a.head_stride % 8 == 0 && a.token_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(a.ptr) & 15) == 0 &&
+              (n == 3 || t.size(0) == 1 || t.size(1) == 1 || t.stride(0) == t.size(1) * a.token_stride),
+              what, ": rows have to be contiguous, 16-byte aligned and evenly spaced");
+  return a;
+}
+
+AttnShape ToAttnShape(const at::Tensor& q, const at::Tensor& k, const c10::optional<at::Tensor>& cu, double scale) {
+  const int64_t n = q.dim();
+  TORCH_CHECK(k.dim() == n && k.size(n - 1) == q.size(n - 1) && k.size(0) == q.size(0) && (n == 3 || k.size(1) == q.size(1)) &&
+              q.size(n - 2) % k.size(n - 2) == 0, "attention: q and k do not match");
+  AttnShape s;
+  if (cu.has_value() && cu->defined()) {
+    TORCH_CHECK(cu->is_cuda() && cu->get_device() == q.get_device() && cu->scalar_type() == at::kInt && cu->dim() == 1 &&
+                cu->numel() >= 2 && cu->is_contiguous(), "attention: cu_seqlens has to be contiguous int32 on the device of q");
+    s.cu = cu->data_ptr<int>();
+    s.batch = static_cast<int>(cu->numel() - 1);
+    s.seq = q.numel() / (q.size(n - 1) * q.size(n - 2));
+  } else {
+    s.batch = n == 4 ? static_cast<int>(q.size(0)) : 1;
+    s.seq = q.size(n - 3);
+  }
+  s.heads = static_cast<int>(q.size(n - 2));
+  s.kv_heads = static_cast<int>(k.size(n - 2));
+  s.dim = static_cast<int>(q.size(n - 1));
+  s.scale = static_cast<float>(scale);
+  TORCH_CHECK(AttnSupported(s), "attention: unsupported shape");
+  return s;
 }
 
 // ---- single-process world of windows: every "rank" is a block [WinHeader | self | one slot per source rank] on
@@ -1081,6 +1132,52 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     TORCH_CHECK(e == cudaSuccess, "gemm_bf16_tn launch failed: ", cudaGetErrorString(e));
     return out;
   }, py::arg("a"), py::arg("b"));
+
+  // ---- causal attention over packed sequences ----------------------------------------------------
+  // q [.., heads, D], k and v [.., kv_heads, D]; returns (out, stats); stats only where they are wanted (backward pass)
+  m.def("attn_forward", [](at::Tensor q, at::Tensor k, at::Tensor v, c10::optional<at::Tensor> cu, double scale, bool want_stats) {
+    TORCH_CHECK(v.sizes() == k.sizes() && q.is_cuda() && k.is_cuda() && v.is_cuda() && k.get_device() == q.get_device() &&
+                v.get_device() == q.get_device(), "attn_forward: q, k and v do not match");
+    c10::cuda::CUDAGuard g(q.get_device());
+    const AttnTensor tq = ToAttn(q, "q"), tk = ToAttn(k, "k"), tv = ToAttn(v, "v");
+    const AttnShape s = ToAttnShape(q, k, cu, scale);
+    at::Tensor out = at::empty(q.sizes(), q.options());
+    at::Tensor stats;
+    if (want_stats) stats = at::empty({s.heads, AttnTiles(s), 128}, q.options().dtype(at::kFloat));
+    cudaError_t e = LaunchAttnForward(s, tq, tk, tv, ToAttn(out, "out"), want_stats ? stats.data_ptr<float>() : nullptr,
+                                      AttnStatusWord(q.get_device()), CurrentStream(q.get_device()));
+    TORCH_CHECK(e == cudaSuccess, "attn_forward launch failed: ", cudaGetErrorString(e));
+    return std::make_tuple(out, stats);
+  });
+  // writes dq, dk and dv (any strides that attn_forward would take)
+  m.def("attn_backward", [](at::Tensor dout, at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor out, at::Tensor stats,
+                            c10::optional<at::Tensor> cu, double scale, at::Tensor dq, at::Tensor dk, at::Tensor dv) {
+    c10::cuda::CUDAGuard g(q.get_device());
+    TORCH_CHECK(v.sizes() == k.sizes() && dout.sizes() == q.sizes() && out.sizes() == q.sizes() && dq.sizes() == q.sizes() &&
+                dk.sizes() == k.sizes() && dv.sizes() == k.sizes(), "attn_backward: shapes do not match");
+    for (const at::Tensor& t : {dout, k, v, out, stats, dq, dk, dv})
+      TORCH_CHECK(t.is_cuda() && t.get_device() == q.get_device(), "attn_backward: tensors on different devices");
+    const AttnShape s = ToAttnShape(q, k, cu, scale);
+    TORCH_CHECK(stats.scalar_type() == at::kFloat && stats.is_contiguous() && stats.numel() == s.heads * AttnTiles(s) * 128,
+                "attn_backward: statistics do not match q");
+    at::Tensor delta = at::empty_like(stats);
+    cudaError_t e = LaunchAttnBackward(s, ToAttn(q, "q"), ToAttn(k, "k"), ToAttn(v, "v"), ToAttn(out, "out"), ToAttn(dout, "dout"),
+                                       stats.data_ptr<float>(), delta.data_ptr<float>(), ToAttn(dq, "dq"), ToAttn(dk, "dk"),
+                                       ToAttn(dv, "dv"), AttnStatusWord(q.get_device()), CurrentStream(q.get_device()));
+    TORCH_CHECK(e == cudaSuccess, "attn_backward launch failed: ", cudaGetErrorString(e));
+  });
+  // reads and clears the status word of the attention kernels (synchronises with the device)
+  m.def("attn_status", [](int device) {
+    c10::cuda::CUDAGuard g(device);
+    cudaStream_t stream = CurrentStream(device);
+    unsigned int* word = AttnStatusWord(device);
+    unsigned int value = 0;
+    cudaError_t e = cudaMemcpyAsync(&value, word, sizeof(value), cudaMemcpyDeviceToHost, stream);
+    if (e == cudaSuccess) e = cudaMemsetAsync(word, 0, sizeof(value), stream);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
+    TORCH_CHECK(e == cudaSuccess, "attn_status failed: ", cudaGetErrorString(e));
+    return value;
+  });
 
   m.def("gemm_status", [] {
     at::Tensor probe = at::empty({0}, at::TensorOptions().device(at::kCUDA));
