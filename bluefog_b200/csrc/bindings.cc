@@ -19,6 +19,7 @@
 #include "cuda/combine_noalloc.h"
 #include "cuda/ce_kernels.h"
 #include "cuda/conv_tcgen05.h"
+#include "cuda/dropout_kernels.h"
 #include "cuda/embed_kernels.h"
 #include "cuda/gemm_tcgen05.h"
 #include "cuda/gpu_channel.h"
@@ -1119,6 +1120,41 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     return out;
   });
 
+  // gated feed-forward block: h = act(a Wg^T) * (a Wu^T) with w = [Wg; Wu]; act 2 = GELU (tanh), 3 = SiLU.  Returns (h, [G U]),
+  // the second only where it is wanted (backward pass)
+  m.def("gemm_bf16_gated", [](at::Tensor a, at::Tensor w, int act, bool want_preact) {
+    TORCH_CHECK(a.is_cuda() && w.is_cuda() && w.get_device() == a.get_device() && a.dim() == 2 && w.dim() == 2 &&
+                a.scalar_type() == at::kBFloat16 && w.scalar_type() == at::kBFloat16 && a.is_contiguous() && w.is_contiguous() &&
+                a.size(1) == w.size(1) && a.size(1) % 8 == 0 && w.size(0) % 16 == 0 && a.numel() > 0 && w.numel() > 0 &&
+                a.size(0) < (1ll << 31) - 256, "gemm_bf16_gated expects contiguous bf16 [M,K], [2F,K] with K, F % 8 == 0");
+    c10::cuda::CUDAGuard g(a.get_device());
+    at::Tensor& status = GemmStatusWord(a);
+    const int64_t f = w.size(0) / 2;
+    at::Tensor h = at::empty({a.size(0), f}, a.options()), pre;
+    if (want_preact) pre = at::empty({a.size(0), 2 * f}, a.options());
+    cudaError_t e = LaunchGemmBf16Gated(a.data_ptr(), w.data_ptr(), h.data_ptr(), want_preact ? pre.data_ptr() : nullptr,
+                                        static_cast<int>(a.size(0)), static_cast<int>(f), static_cast<int>(a.size(1)), act,
+                                        reinterpret_cast<unsigned int*>(status.data_ptr()), CurrentStream(a.get_device()));
+    TORCH_CHECK(e == cudaSuccess, "gemm_bf16_gated launch failed: ", cudaGetErrorString(e));
+    return std::make_tuple(h, pre);
+  });
+  // [dG dU] from dH = a b and the kept [G U]
+  m.def("gemm_bf16_nn_gated_grad", [](at::Tensor a, at::Tensor b, at::Tensor preact, int act) {
+    TORCH_CHECK(a.is_cuda() && b.is_cuda() && preact.is_cuda() && a.dim() == 2 && b.dim() == 2 && preact.dim() == 2 &&
+                a.scalar_type() == at::kBFloat16 && b.scalar_type() == at::kBFloat16 && preact.scalar_type() == at::kBFloat16 &&
+                a.is_contiguous() && b.is_contiguous() && preact.is_contiguous() && a.size(1) == b.size(0) &&
+                preact.size(0) == a.size(0) && preact.size(1) == 2 * b.size(1) && b.get_device() == a.get_device() &&
+                preact.get_device() == a.get_device(), "gemm_bf16_nn_gated_grad expects contiguous bf16 [M,K], [K,F], [M,2F]");
+    c10::cuda::CUDAGuard g(a.get_device());
+    at::Tensor& status = GemmStatusWord(a);
+    at::Tensor out = at::empty(preact.sizes(), preact.options());
+    cudaError_t e = LaunchGemmBf16NNGatedGrad(a.data_ptr(), b.data_ptr(), preact.data_ptr(), out.data_ptr(), static_cast<int>(a.size(0)),
+                                              static_cast<int>(b.size(1)), static_cast<int>(a.size(1)), act,
+                                              reinterpret_cast<unsigned int*>(status.data_ptr()), CurrentStream(a.get_device()));
+    TORCH_CHECK(e == cudaSuccess, "gemm_bf16_nn_gated_grad launch failed: ", cudaGetErrorString(e));
+    return out;
+  });
+
   m.def("gemm_bf16_tn", [](at::Tensor a, at::Tensor b) {
     TORCH_CHECK(a.is_cuda() && b.is_cuda() && a.dim() == 2 && b.dim() == 2 && a.scalar_type() == at::kBFloat16 &&
                 b.scalar_type() == at::kBFloat16 && a.is_contiguous() && b.is_contiguous() && a.size(0) == b.size(0),
@@ -1177,6 +1213,28 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
     TORCH_CHECK(e == cudaSuccess, "attn_status failed: ", cudaGetErrorString(e));
     return value;
+  });
+
+  // ---- dropout joined with the residual stream ---------------------------------------------------
+  // threshold: of 65536 (dropped share); key: int64 [2] = (seed, step) on the device of x
+  m.def("dropout_add", [](at::Tensor x, c10::optional<at::Tensor> residual, int64_t threshold, double factor, at::Tensor key, int64_t site) {
+    TORCH_CHECK(x.is_cuda() && x.is_contiguous() && x.numel() > 0, "dropout_add expects a contiguous CUDA tensor");
+    TORCH_CHECK(key.is_cuda() && key.get_device() == x.get_device() && key.scalar_type() == at::kLong && key.numel() == 2 &&
+                key.is_contiguous(), "dropout_add: key has to be int64 [2] on the device of x");
+    TORCH_CHECK(threshold >= 0 && threshold <= 65536 && site >= 0 && site <= 65535, "dropout_add: threshold or site out of range");
+    const int type = x.scalar_type() == at::kFloat ? kDropF32 : x.scalar_type() == at::kHalf ? kDropF16 : kDropBF16;
+    TORCH_CHECK(type != kDropBF16 || x.scalar_type() == at::kBFloat16, "dropout_add: fp32, fp16 or bf16");
+    const void* res = PtrOrNull(residual);
+    if (res != nullptr)
+      TORCH_CHECK(residual->is_cuda() && residual->get_device() == x.get_device() && residual->sizes() == x.sizes() &&
+                  residual->scalar_type() == x.scalar_type() && residual->is_contiguous(), "dropout_add: residual does not match x");
+    c10::cuda::CUDAGuard g(x.get_device());
+    at::Tensor out = at::empty(x.sizes(), x.options());
+    cudaError_t e = LaunchDropoutAdd(x.data_ptr(), res, out.data_ptr(), x.numel(), type, static_cast<unsigned int>(threshold),
+                                     static_cast<float>(factor), reinterpret_cast<const long long*>(key.data_ptr<int64_t>()),
+                                     static_cast<unsigned int>(site), CurrentStream(x.get_device()));
+    TORCH_CHECK(e == cudaSuccess, "dropout_add launch failed: ", cudaGetErrorString(e));
+    return out;
   });
 
   m.def("gemm_status", [] {

@@ -1,0 +1,135 @@
+// Dropout joined with the residual stream:  out = residual + keep * x / (1 - p),  and its backward pass  dx = keep * dy / (1 - p).
+//
+// The mask is never stored: keep(i) is a function of (seed, step, site, i), computed where it is needed by Philox4x32-10
+// (J. K. Salmon, M. A. Moraes, R. O. Dror, D. E. Shaw, "Parallel random numbers: as easy as 1, 2, 3", SC 2011).  One block
+// of 128 bits serves eight elements, sixteen bits each: p is a multiple of 2^-16, and the factor is the inverse of the
+// probability that is really used, so the expectation is exact.  A dropped element contributes zero whatever x holds.
+//
+// Bound by memory: x and residual are read and out is written once (6 bytes per bf16 element forward, 4 backward); a block
+// of Philox costs about 60 instructions, 8 per element, half of what the memory leaves time for.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "comm_kernels.h"
+#include "dropout_kernels.h"
+
+namespace bfb {
+namespace {
+
+constexpr int kThreads = 256;
+
+__device__ __forceinline__ uint4 philox(uint4 c, uint32_t k0, uint32_t k1) {
+#pragma unroll
+  for (int r = 0; r < 10; ++r) {
+    const uint64_t a = uint64_t(c.x) * 0xD2511F53u, b = uint64_t(c.z) * 0xCD9E8D57u;
+    c = make_uint4(uint32_t(b >> 32) ^ c.y ^ k0, uint32_t(b), uint32_t(a >> 32) ^ c.w ^ k1, uint32_t(a));
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+  return c;
+}
+
+template <typename T> __device__ __forceinline__ float to_f(T v);
+template <> __device__ __forceinline__ float to_f<float>(float v) { return v; }
+template <> __device__ __forceinline__ float to_f<__half>(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from_f(float v);
+template <> __device__ __forceinline__ float from_f<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// eight elements, the unit of a Philox block
+template <typename T>
+struct alignas(16) Eight {
+  T v[8];
+};
+template <typename T>
+__device__ __forceinline__ Eight<T> load8(const T* p) {
+  Eight<T> e;
+  const uint4* s = reinterpret_cast<const uint4*>(p);
+#pragma unroll
+  for (int i = 0; i < int(sizeof(Eight<T>) / 16); ++i) reinterpret_cast<uint4*>(&e)[i] = s[i];
+  return e;
+}
+
+template <typename T, bool RES>
+__device__ __forceinline__ void apply(Eight<T>& x, const Eight<T>& res, const uint4 bits, uint32_t threshold, float factor) {
+  const uint32_t w[4] = {bits.x, bits.y, bits.z, bits.w};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t u = (i & 1) ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu;
+    float y = u >= threshold ? to_f(x.v[i]) * factor : 0.f;
+    if (RES) y += to_f(res.v[i]);
+    x.v[i] = from_f<T>(y);
+  }
+}
+
+template <typename T, bool RES>
+__global__ void __launch_bounds__(kThreads)
+dropout_add_kernel(const T* x, const T* residual, T* out, const long long n, const uint32_t threshold, const float factor,
+                   const long long* __restrict__ key, const uint32_t site) {
+  const unsigned long long seed = key[0], step = key[1];
+  const long long groups = n / 8;
+  const long long stride = (long long)gridDim.x * kThreads;
+  for (long long g = (long long)blockIdx.x * kThreads + threadIdx.x; g <= groups; g += stride) {
+    const uint4 c = make_uint4(uint32_t(g), uint32_t(g >> 32) | site << 16, uint32_t(step), uint32_t(step >> 32));
+    if (g < groups) {
+      Eight<T> a = load8(x + g * 8), r = a;
+      if (RES) r = load8(residual + g * 8);
+      apply<T, RES>(a, r, philox(c, uint32_t(seed), uint32_t(seed >> 32)), threshold, factor);
+#pragma unroll
+      for (int i = 0; i < int(sizeof(Eight<T>) / 16); ++i)
+        reinterpret_cast<uint4*>(out + g * 8)[i] = reinterpret_cast<const uint4*>(&a)[i];
+    } else if (groups * 8 < n) {                        // up to seven elements at the end
+      const int rest = int(n - groups * 8);
+      Eight<T> a = {}, r = {};
+      for (int i = 0; i < 7; ++i)
+        if (i < rest) {
+          a.v[i] = x[groups * 8 + i];
+          if (RES) r.v[i] = residual[groups * 8 + i];
+        }
+      apply<T, RES>(a, r, philox(c, uint32_t(seed), uint32_t(seed >> 32)), threshold, factor);
+      for (int i = 0; i < 7; ++i)
+        if (i < rest) out[groups * 8 + i] = a.v[i];
+    }
+  }
+}
+
+template <typename T>
+cudaError_t Launch(const void* x, const void* residual, void* out, long long n, unsigned int threshold, float factor,
+                   const long long* key, unsigned int site, cudaStream_t stream) {
+  int dev = 0, sms = 148;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e != cudaSuccess) return e;
+  const long long blocks = (n / 8 + 1 + kThreads - 1) / kThreads;
+  const unsigned grid = static_cast<unsigned>(blocks < (long long)sms * 8 ? blocks : (long long)sms * 8);
+  const T* a = static_cast<const T*>(x);
+  const T* r = static_cast<const T*>(residual);
+  T* o = static_cast<T*>(out);
+  if (r != nullptr) dropout_add_kernel<T, true><<<grid, kThreads, 0, stream>>>(a, r, o, n, threshold, factor, key, site);
+  else dropout_add_kernel<T, false><<<grid, kThreads, 0, stream>>>(a, r, o, n, threshold, factor, key, site);
+  CountKernelLaunch();
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t LaunchDropoutAdd(const void* x, const void* residual, void* out, long long n, int type, unsigned int threshold,
+                             float factor, const long long* key, unsigned int site, cudaStream_t stream) {
+  (void)cudaGetLastError();   // the value returned below must be this launch's own, not an older error of the calling thread
+  const uintptr_t all = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(residual) | reinterpret_cast<uintptr_t>(out);
+  if (n <= 0 || (n >> 51) != 0 || x == nullptr || out == nullptr || key == nullptr || (all & 15) != 0 || threshold > 65536u ||
+      site > 65535u)
+    return cudaErrorInvalidValue;
+  switch (type) {
+    case kDropF32: return Launch<float>(x, residual, out, n, threshold, factor, key, site, stream);
+    case kDropF16: return Launch<__half>(x, residual, out, n, threshold, factor, key, site, stream);
+    case kDropBF16: return Launch<__nv_bfloat16>(x, residual, out, n, threshold, factor, key, site, stream);
+    default: return cudaErrorInvalidValue;
+  }
+}
+
+}  // namespace bfb

@@ -106,6 +106,30 @@ __device__ __forceinline__ float gelu_tanh_grad(float x) {
   return 0.5f * (1.f + t) + 0.5f * x * (1.f - t * t) * c * (1.f + 3.f * 0.044715f * x * x);
 }
 
+// Gates of a gated feed-forward block, act(x) = x * sigmoid(w(x)): w = x (kActSilu), or w = 2 sqrt(2/pi) (x + 0.044715 x^3)
+// (kActGeluTanh: (1 + tanh z) / 2 = sigmoid(2 z), which keeps its relative accuracy where tanh is near -1).
+// Returns act(x); grad receives act'(x) = s + x s (1 - s) w'(x).
+__device__ __forceinline__ float gate_fn(float x, int act, float* grad) {
+  float w = x, dw = 1.f;
+  if (act == kActGeluTanh) {
+    const float c = 1.5957691216057308f;
+    w = c * (x + 0.044715f * x * x * x);
+    dw = c * (1.f + 0.134145f * x * x);
+  }
+  const float s = __fdividef(1.f, 1.f + __expf(-w));
+  const float y = x * s;
+  if (grad != nullptr) *grad = s + y * (1.f - s) * dw;
+  return y;
+}
+// eight floats as bf16, 16 bytes
+__device__ __forceinline__ uint4 pack8(const float* v) {
+  uint4 pk;
+  __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&pk);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+  return pk;
+}
+
 __global__ void __launch_bounds__(kThreads, 1)
 gemm_bf16_nt_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                     __nv_bfloat16* __restrict__ out, const __nv_bfloat16* __restrict__ bias, int M, int N, int K,
@@ -291,6 +315,9 @@ struct PersistentCfg {
   // per epilogue warp: BN_ column sums and BN_ sums of squares
   static constexpr uint32_t kStatBytes = EPI == kEpiColumnStats ? kEpiWarps * 2 * BN_ * 4 : 0;
   static constexpr int kRowsB = PAIR ? BN_ / 2 : BN_;          // rows (output columns) of B one CTA loads
+  // kEpiGated: the accumulator holds BN_ / 2 columns of the gate product and the same columns of the up product beside
+  // them, and BN_ / 2 output columns leave
+  static constexpr int kTileN = EPI == kEpiGated ? BN_ / 2 : BN_;
   static constexpr int kTileM = PAIR ? 2 * BM : BM;
   static constexpr uint32_t kBytesA = BM * BK * 2;
   static constexpr uint32_t kBytesB = kRowsB * BK * 2;
@@ -320,7 +347,8 @@ gemm_bf16_nt_persistent_kernel(const __grid_constant__ CUtensorMap map_a, const 
                                const __grid_constant__ CUtensorMap map_c, __nv_bfloat16* __restrict__ out,
                                const __nv_bfloat16* __restrict__ bias, int M, int N, int K, int act, int tma_out,
                                unsigned int* __restrict__ status, const __grid_constant__ CUtensorMap map_aux,
-                               const __nv_bfloat16* __restrict__ aux_in, float* __restrict__ col_stats) {
+                               const __nv_bfloat16* __restrict__ aux_in, float* __restrict__ col_stats,
+                               const __grid_constant__ CUtensorMap map_b2, const __grid_constant__ CUtensorMap map_aux2) {
   using Cfg = PersistentCfg<BN_, EPI, PAIR>;
   constexpr int S = Cfg::kStagesP;
   extern __shared__ unsigned char smem_raw[];
@@ -338,7 +366,7 @@ gemm_bf16_nt_persistent_kernel(const __grid_constant__ CUtensorMap map_a, const 
   const int lane = threadIdx.x & 31;
   const uint32_t rank = PAIR ? cluster_ctarank() : 0u;
   const bool leader = rank == 0;
-  const int tiles_n = (N + BN_ - 1) / BN_;
+  const int tiles_n = (N + Cfg::kTileN - 1) / Cfg::kTileN;
   const int tiles_m = (M + Cfg::kTileM - 1) / Cfg::kTileM;
   const int num_tiles = tiles_m * tiles_n;
   const int num_kb = (K + BK - 1) / BK;
@@ -386,7 +414,8 @@ gemm_bf16_nt_persistent_kernel(const __grid_constant__ CUtensorMap map_a, const 
         int tm, tn;
         tile_coords(tile, tiles_m, tiles_n, tm, tn);
         const int m0 = tm * Cfg::kTileM + int(rank) * BM;
-        const int n0 = tn * BN_ + int(rank) * Cfg::kRowsB;          // PAIR: this CTA's half of the tile's columns
+        // PAIR: this CTA's half of the tile's columns; with two B matrices the leader loads the gate's, the other the up's
+        const int n0 = tn * Cfg::kTileN + (EPI == kEpiGated ? 0 : int(rank) * Cfg::kRowsB);
         for (int kb = 0; kb < num_kb; ++kb, ++it) {
           const int s = it % S;
           if (!mbar_wait(smem_u32(&bars[S + s]), ((it / S) & 1) ^ 1, failed)) { ok = false; break; }
@@ -404,7 +433,15 @@ gemm_bf16_nt_persistent_kernel(const __grid_constant__ CUtensorMap map_a, const 
             for (int j = 0; j < BM / 64; ++j)
               load(smem_u32(stage_a + size_t(s) * Cfg::kBytesA + size_t(j) * 8192), &map_a, m0 + j * 64, kb * BK);
           }
-          if (BMODE == 0) {
+          if (EPI == kEpiGated) {
+            const uint32_t dst = smem_u32(stage_b + size_t(s) * Cfg::kBytesB);
+            if (PAIR) {
+              load(dst, leader ? &map_b : &map_b2, kb * BK, n0);
+            } else {
+              load(dst, &map_b, kb * BK, n0);
+              load(dst + (BN_ / 2) * BK * 2, &map_b2, kb * BK, n0);
+            }
+          } else if (BMODE == 0) {
             load(smem_u32(stage_b + size_t(s) * Cfg::kBytesB), &map_b, kb * BK, n0);
           } else {
 #pragma unroll
@@ -472,7 +509,7 @@ gemm_bf16_nt_persistent_kernel(const __grid_constant__ CUtensorMap map_a, const 
     const int q = warp & 3;                // the quarter of tensor memory (32 lanes = 32 rows) this warp can read
     const int ew = warp - 2;               // epilogue warp index
     // eight warps: warps 2-5 take the first half of the columns, warps 6-9 the second
-    constexpr int kChunks = BN_ / 64;
+    constexpr int kChunks = Cfg::kTileN / 64;
     constexpr int kChunksW = Cfg::kEpiWarps == 8 ? kChunks / 2 : kChunks;
     const int c_first = Cfg::kEpiWarps == 8 ? (ew >> 2) * kChunksW : 0;
     const bool vec_ok = (N % 8) == 0;
@@ -512,7 +549,7 @@ gemm_bf16_nt_persistent_kernel(const __grid_constant__ CUtensorMap map_a, const 
       int tm, tn;
       tile_coords(tile, tiles_m, tiles_n, tm, tn);
       const int m0 = tm * Cfg::kTileM + int(rank) * BM;         // this CTA's 128 rows, all BN_ columns
-      const int n0 = tn * BN_;
+      const int n0 = tn * Cfg::kTileN;
       if (!mbar_wait(smem_u32(&bars[2 * S + acc]), (local >> 1) & 1, failed)) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const int m = m0 + q * 32 + lane;
@@ -522,7 +559,50 @@ gemm_bf16_nt_persistent_kernel(const __grid_constant__ CUtensorMap map_a, const 
           stat_n0 = n0;
         }
       }
-      if (tma_out) {
+      if constexpr (EPI == kEpiGated) {
+        // h = act(g) u from the fp32 accumulators; g and u leave too (rounded, for the backward pass) when tma_out is 2.
+        // Their boxes take turns in the warp's two staging buffers.
+#pragma unroll 1
+        for (int c = c_first; c < c_first + kChunksW; ++c) {
+          const int nbase = n0 + c * 64;
+          if (nbase >= N || m0 + q * 32 >= M) break;           // warp-uniform
+          const uint32_t taddr = tmem_base + (uint32_t(q * 32) << 16) + uint32_t(acc * BN_ + c * 64);
+          uint32_t g[64], u[64];
+          tmem_ld32(taddr, g);
+          tmem_ld32(taddr + 32, g + 32);
+          tmem_ld32(taddr + BN_ / 2, u);
+          tmem_ld32(taddr + BN_ / 2 + 32, u + 32);
+          tmem_wait_ld();
+          tie32(g);
+          tie32(g + 32);
+          tie32(u);
+          tie32(u + 32);
+          auto leave = [&](const CUtensorMap* map, auto&& value) {
+            if (lane == 0) tma_store_wait_read<1>();           // the box written two stores ago has been read
+            __syncwarp();
+            unsigned char* box = my_out + size_t(boxes & 1) * Cfg::kBytesOutBox;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              float v[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) v[i] = value(j * 8 + i);
+              *reinterpret_cast<uint4*>(box + lane * 128 + ((j ^ (lane & 7)) << 4)) = pack8(v);      // 128-byte swizzle
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_2d(map, smem_u32(box), nbase, m0 + q * 32);
+              tma_store_commit();
+            }
+            ++boxes;
+          };
+          if (tma_out == 2) {
+            leave(&map_aux, [&](int i) { return __uint_as_float(g[i]); });
+            leave(&map_aux2, [&](int i) { return __uint_as_float(u[i]); });
+          }
+          leave(&map_c, [&](int i) { return gate_fn(__uint_as_float(g[i]), act, nullptr) * __uint_as_float(u[i]); });
+        }
+      } else if (tma_out) {
 #pragma unroll 1
         for (int c = c_first; c < c_first + kChunksW; ++c) {
           const int nbase = n0 + c * 64;
@@ -645,6 +725,42 @@ gemm_bf16_nt_persistent_kernel(const __grid_constant__ CUtensorMap map_a, const 
               tma_store_commit();
             }
             ++boxes;
+          } else if constexpr (EPI == kEpiGatedGrad) {
+            // accumulator = dH; with the kept g (aux_in) and u (N values behind it in the same row of 2 N):
+            // dG = dH u act'(g) through map_c, dU = dH act(g) through map_aux
+            if (lane == 0) tma_store_wait_read<0>();
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              uint4 gv = make_uint4(0u, 0u, 0u, 0u), uv = gv;
+              if (m < M && nbase + j * 8 < N) {
+                const __nv_bfloat16* src = aux_in + size_t(m) * (2 * size_t(N)) + nbase + j * 8;
+                gv = __ldg(reinterpret_cast<const uint4*>(src));
+                uv = __ldg(reinterpret_cast<const uint4*>(src + N));
+              }
+              const __nv_bfloat162* gh = reinterpret_cast<const __nv_bfloat162*>(&gv);
+              const __nv_bfloat162* uh = reinterpret_cast<const __nv_bfloat162*>(&uv);
+              float dg[8], du[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const float2 g2 = __bfloat1622float2(gh[i >> 1]), u2 = __bfloat1622float2(uh[i >> 1]);
+                const float dh = __uint_as_float(r[j * 8 + i]);
+                float slope;
+                du[i] = dh * gate_fn((i & 1) ? g2.y : g2.x, act, &slope);
+                dg[i] = dh * ((i & 1) ? u2.y : u2.x) * slope;
+              }
+              const int off = (j ^ (lane & 7)) << 4;                                // 128-byte swizzle
+              *reinterpret_cast<uint4*>(my_out + lane * 128 + off) = pack8(dg);
+              *reinterpret_cast<uint4*>(my_out + Cfg::kBytesOutBox + lane * 128 + off) = pack8(du);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_2d(&map_c, smem_u32(my_out), nbase, m0 + q * 32);
+              tma_store_2d(&map_aux, smem_u32(my_out + Cfg::kBytesOutBox), nbase, m0 + q * 32);
+              tma_store_commit();
+            }
+            boxes += 2;
           } else {
             // kEpiStorePreact: two boxes leave per chunk, x = accumulator + bias through map_aux and act(x)
             // through map_c; both staging boxes are in use, so every earlier store must have been read
@@ -755,9 +871,10 @@ gemm_bf16_nt_persistent_kernel(const __grid_constant__ CUtensorMap map_a, const 
   if (threadIdx.x == 0 && failed_s && status != nullptr) atomicExch(status, 1u);
 }
 
-bool MakeMap(CUtensorMap* map, const void* base, int rows, int cols /*K*/, int box_rows) {
+// pitch: elements from row to row (0: the rows follow one another)
+bool MakeMap(CUtensorMap* map, const void* base, int rows, int cols /*K*/, int box_rows, long long pitch = 0) {
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
-  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(cols) * 2};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch != 0 ? pitch : cols) * 2};
   const cuuint32_t box[2] = {static_cast<cuuint32_t>(BK), static_cast<cuuint32_t>(box_rows)};
   return EncodeTiled(map, 2, base, dims, strides, box);
 }
@@ -768,19 +885,27 @@ template <int BN_, int BMODE, int AMODE, int EPI, int PAIR = 0>
 cudaError_t LaunchPersistent(const CUtensorMap& map_a, const CUtensorMap& map_b, const CUtensorMap& map_c,
                              const CUtensorMap& map_aux, __nv_bfloat16* out, const __nv_bfloat16* bias,
                              const __nv_bfloat16* aux_in, int M, int N, int K, int act, int tma_out, int sm_count,
-                             unsigned int* status, cudaStream_t stream, float* col_stats = nullptr) {
+                             unsigned int* status, cudaStream_t stream, float* col_stats = nullptr,
+                             const CUtensorMap* map_b2 = nullptr, const CUtensorMap* map_aux2 = nullptr) {
   using Cfg = PersistentCfg<BN_, EPI, PAIR>;
   auto kernel = gemm_bf16_nt_persistent_kernel<BN_, BMODE, AMODE, EPI, PAIR>;
-  static bool attr_set = false;
-  if (!attr_set) {
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Cfg::kSmem));
+  // the permission for this much shared memory belongs to a device
+  constexpr int kMaxDevices = 64;
+  static bool attr_set[kMaxDevices] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev >= kMaxDevices || !attr_set[dev]) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Cfg::kSmem));
     if (e != cudaSuccess) return e;
-    attr_set = true;
+    if (dev < kMaxDevices) attr_set[dev] = true;
   }
-  const int tiles = ((M + Cfg::kTileM - 1) / Cfg::kTileM) * ((N + BN_ - 1) / BN_);
+  const int tiles = ((M + Cfg::kTileM - 1) / Cfg::kTileM) * ((N + Cfg::kTileN - 1) / Cfg::kTileN);
+  const CUtensorMap& b2 = map_b2 != nullptr ? *map_b2 : map_b;
+  const CUtensorMap& aux2 = map_aux2 != nullptr ? *map_aux2 : map_aux;
   if (!PAIR) {
     kernel<<<tiles < sm_count ? tiles : sm_count, Cfg::kThreadsP, Cfg::kSmem, stream>>>(map_a, map_b, map_c, out, bias, M, N, K, act,
-                                                                               tma_out, status, map_aux, aux_in, col_stats);
+                                                                               tma_out, status, map_aux, aux_in, col_stats, b2, aux2);
     return cudaSuccess;
   }
   const int pairs = tiles < sm_count / 2 ? tiles : sm_count / 2;
@@ -796,7 +921,8 @@ cudaError_t LaunchPersistent(const CUtensorMap& map_a, const CUtensorMap& map_b,
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, map_a, map_b, map_c, out, bias, M, N, K, act, tma_out, status, map_aux, aux_in, col_stats);
+  return cudaLaunchKernelEx(&cfg, kernel, map_a, map_b, map_c, out, bias, M, N, K, act, tma_out, status, map_aux, aux_in, col_stats, b2,
+                            aux2);
 }
 
 // Whether a plain product goes to the two-SM kernel: TMA-storable output, at least one full pair tile in each
@@ -964,6 +1090,65 @@ cudaError_t LaunchGemmBf16NN(const void* a, const void* b, void* out, int M, int
                        : LaunchPersistent<128, 1, 0, kEpiNone>(map_a, map_b, map_c, map_c, o, nullptr, nullptr, M, N, K, 0, 1,
                                                                sm_count, status, stream);
   }
+  if (e != cudaSuccess) return e;
+  CountKernelLaunch();
+  return cudaGetLastError();
+}
+
+// h[M,F] = act(a Wg^T) * (a Wu^T) with [Wg; Wu] = w [2F, K]: one tile of the accumulator holds the same columns of both
+// products, so the activation and the product with the gate are part of the epilogue.
+cudaError_t LaunchGemmBf16Gated(const void* a, const void* w, void* h, void* preact, int M, int F, int K, int act,
+                                unsigned int* status, cudaStream_t stream) {
+  (void)cudaGetLastError();   // the value returned below must be this launch's own, not an older error of the calling thread
+  if (M <= 0 || F <= 0 || K <= 0 || (K % 8) != 0 || (F % 8) != 0 || (act != kActSilu && act != kActGeluTanh)) return cudaErrorInvalidValue;
+  if ((reinterpret_cast<uintptr_t>(a) & 15) || (reinterpret_cast<uintptr_t>(w) & 15) || (reinterpret_cast<uintptr_t>(h) & 15) ||
+      (reinterpret_cast<uintptr_t>(preact) & 15))
+    return cudaErrorInvalidValue;
+  const int sm_count = SmCount();
+  const __nv_bfloat16* wu = static_cast<const __nv_bfloat16*>(w) + size_t(F) * K;
+  __nv_bfloat16* pre = static_cast<__nv_bfloat16*>(preact);
+  CUtensorMap map_a, map_g, map_u, map_h, map_pg, map_pu;
+  // the weights' boxes: half of the accumulator's columns each
+  const bool pair = UsePair(M, 2 * F, K, sm_count);
+  const int box_w = pair || F > 64 ? 128 : 64;
+  if (!MakeMap(&map_a, a, M, K, BM) || !MakeMap(&map_g, w, F, K, box_w) || !MakeMap(&map_u, wu, F, K, box_w) || !MakeMap(&map_h, h, M, F, 32))
+    return cudaErrorInvalidValue;
+  map_pg = map_pu = map_h;
+  if (pre != nullptr && (!MakeMap(&map_pg, pre, M, F, 32, 2ll * F) || !MakeMap(&map_pu, pre + F, M, F, 32, 2ll * F))) return cudaErrorInvalidValue;
+  __nv_bfloat16* o = static_cast<__nv_bfloat16*>(h);
+  const int mode = pre != nullptr ? 2 : 1;
+  const cudaError_t e =
+      pair      ? LaunchPersistent<256, 0, 0, kEpiGated, 1>(map_a, map_g, map_h, map_pg, o, nullptr, nullptr, M, F, K, act, mode, sm_count,
+                                                            status, stream, nullptr, &map_u, &map_pu)
+      : F > 64 ? LaunchPersistent<256, 0, 0, kEpiGated>(map_a, map_g, map_h, map_pg, o, nullptr, nullptr, M, F, K, act, mode, sm_count, status,
+                                                        stream, nullptr, &map_u, &map_pu)
+               : LaunchPersistent<128, 0, 0, kEpiGated>(map_a, map_g, map_h, map_pg, o, nullptr, nullptr, M, F, K, act, mode, sm_count, status,
+                                                        stream, nullptr, &map_u, &map_pu);
+  if (e != cudaSuccess) return e;
+  CountKernelLaunch();
+  return cudaGetLastError();
+}
+
+// dpre[M,2F] = [dG dU] from dH = a[M,K] * b[K,F] and the kept preact[M,2F] = [G U].
+cudaError_t LaunchGemmBf16NNGatedGrad(const void* a, const void* b, const void* preact, void* dpre, int M, int F, int K, int act,
+                                      unsigned int* status, cudaStream_t stream) {
+  (void)cudaGetLastError();
+  if (M <= 0 || F <= 0 || K <= 0 || (K % 8) != 0 || (F % 8) != 0 || (act != kActSilu && act != kActGeluTanh)) return cudaErrorInvalidValue;
+  if ((reinterpret_cast<uintptr_t>(a) & 15) || (reinterpret_cast<uintptr_t>(b) & 15) || (reinterpret_cast<uintptr_t>(preact) & 15) ||
+      (reinterpret_cast<uintptr_t>(dpre) & 15))
+    return cudaErrorInvalidValue;
+  const int sm_count = SmCount();
+  __nv_bfloat16* o = static_cast<__nv_bfloat16*>(dpre);
+  const __nv_bfloat16* pre = static_cast<const __nv_bfloat16*>(preact);
+  CUtensorMap map_a, map_b, map_g, map_u;
+  if (!MakeMap(&map_a, a, M, K, BM) || !MakeMap(&map_b, b, K, F, 64) || !MakeMap(&map_g, o, M, F, 32, 2ll * F) ||
+      !MakeMap(&map_u, o + F, M, F, 32, 2ll * F))
+    return cudaErrorInvalidValue;
+  const cudaError_t e =
+      UsePair(M, F, K, sm_count) ? LaunchPersistent<256, 1, 0, kEpiGatedGrad, 1>(map_a, map_b, map_g, map_u, o, nullptr, pre, M, F, K, act, 1,
+                                                                                 sm_count, status, stream)
+      : F > 128 ? LaunchPersistent<256, 1, 0, kEpiGatedGrad>(map_a, map_b, map_g, map_u, o, nullptr, pre, M, F, K, act, 1, sm_count, status, stream)
+                : LaunchPersistent<128, 1, 0, kEpiGatedGrad>(map_a, map_b, map_g, map_u, o, nullptr, pre, M, F, K, act, 1, sm_count, status, stream);
   if (e != cudaSuccess) return e;
   CountKernelLaunch();
   return cudaGetLastError();

@@ -4,11 +4,13 @@
 
 namespace bfb {
 
-enum GemmAct : int { kActNone = 0, kActRelu = 1, kActGeluTanh = 2 };
+enum GemmAct : int { kActNone = 0, kActRelu = 1, kActGeluTanh = 2, kActSilu = 3 };
 // Extra work of the epilogue: store the pre-activation value (accumulator + bias) to a second matrix besides
 // act(...) of it; or multiply the result by GELU'(aux[m, n]) (the input gradient through a GELU whose
-// pre-activation was kept).
-enum GemmEpi : int { kEpiNone = 0, kEpiStorePreact = 1, kEpiMulGeluGrad = 2, kEpiColumnStats = 3, kEpiAddAux = 4 };
+// pre-activation was kept); or one half of a gated feed-forward block (two products in one accumulator, their gated
+// product or its gradients out).
+enum GemmEpi : int { kEpiNone = 0, kEpiStorePreact = 1, kEpiMulGeluGrad = 2, kEpiColumnStats = 3, kEpiAddAux = 4, kEpiGated = 5,
+                     kEpiGatedGrad = 6 };
 
 // True when the driver exposes cuTensorMapEncodeTiled (needed to build TMA descriptors).
 bool GemmSupported();
@@ -36,5 +38,13 @@ cudaError_t LaunchGemmBf16NN(const void* a, const void* b, void* out, int M, int
 // out[M,N] = a[K,M]^T * b[K,N], a and b row-major (both consumed MN-major); M % 8 == 0, N % 8 == 0.
 cudaError_t LaunchGemmBf16TN(const void* a, const void* b, void* out, int M, int N, int K, unsigned int* status,
                              cudaStream_t stream);
+
+// h[M,F] = act(a[M,K] * w[0:F,K]^T) * (a * w[F:2F,K]^T), act kActSilu or kActGeluTanh; K % 8 == 0, F % 8 == 0.  preact
+// (optional, [M,2F]): receives both products before the activation.
+cudaError_t LaunchGemmBf16Gated(const void* a, const void* w, void* h, void* preact, int M, int F, int K, int act,
+                                unsigned int* status, cudaStream_t stream);
+// Its gradient: with dH[M,F] = a[M,K] * b[K,F] and preact = [G U], dpre[M,2F] = [dH U act'(G), dH act(G)].
+cudaError_t LaunchGemmBf16NNGatedGrad(const void* a, const void* b, const void* preact, void* dpre, int M, int F, int K, int act,
+                                      unsigned int* status, cudaStream_t stream);
 
 }  // namespace bfb

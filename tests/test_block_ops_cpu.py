@@ -69,3 +69,63 @@ def test_side_by_side_projection_refuses(shape, h, hkv):
     from bluefog_b200.ops import fused_attention as fa
     with pytest.raises(ValueError):
         fa.causal_self_attention(torch.zeros(shape), h, hkv)
+
+
+def test_philox_reference_vectors():
+    """The generator against the three test vectors published with it."""
+    from test_gpu_dropout import philox
+    ones = 0xFFFFFFFF
+    assert philox((0, 0, 0, 0), (0, 0)) == [0x6627E8D5, 0xE169C58D, 0xBC57AC4C, 0x9B00DBD8]
+    assert philox((ones,) * 4, (ones,) * 2) == [0x408F276D, 0x41C83B0E, 0xA20BC7C6, 0x6D5451FD]
+    assert philox((0x243F6A88, 0x85A308D3, 0x13198A2E, 0x03707344), (0xA4093822, 0x299F31D0)) == \
+        [0xD16CFE09, 0x94FDCCEB, 0x5001E420, 0x24126EA1]
+
+
+@pytest.mark.parametrize("count,p,seed,step,site", [(1, 0.5, 0, 0, 0), (41, 0.1, -5, 2 ** 33 + 1, 7), (64, 1.0, 1, 1, 1), (64, 0.0, 1, 1, 1)])
+def test_dropout_on_the_cpu(count, p, seed, step, site):
+    from bluefog_b200.ops import fused_dropout
+    from test_gpu_dropout import kept
+    x = torch.randn(count, dtype=torch.float64, requires_grad=True)
+    r = torch.randn(count, dtype=torch.float64)
+    keep = kept(count, p, seed, step, site)
+    y = fused_dropout.dropout_add(x, r, p, torch.tensor([seed, step]), site)
+    q = round(65536 * p) / 65536
+    factor = keep.double() / (1 - q) if q < 1 else torch.zeros(count, dtype=torch.float64)
+    torch.testing.assert_close(y, r + x * factor)
+    (g,) = torch.autograd.grad(y.sum(), x)
+    torch.testing.assert_close(g, factor)
+
+
+@pytest.mark.parametrize("change", [
+    dict(p=-0.1), dict(p=1.1), dict(p=math.nan), dict(x=torch.zeros(4, 4, dtype=torch.int64)), dict(residual=torch.zeros(4)),
+    dict(residual=torch.zeros(4, 4, dtype=torch.float64)), dict(key=torch.zeros(2)), dict(key=torch.zeros(3, dtype=torch.int64)),
+    dict(site=-1), dict(site=65536)])
+def test_dropout_refuses(change):
+    from bluefog_b200.ops import fused_dropout
+    args = dict(x=torch.zeros(4, 4), residual=None, p=0.1, key=fused_dropout.new_key(0))
+    args.update(change)
+    with pytest.raises(ValueError):
+        fused_dropout.dropout_add(**args)
+
+
+def test_gated_mlp_on_the_cpu():
+    import torch.nn.functional as F
+    from bluefog_b200.ops import gemm
+    torch.manual_seed(0)
+    a, wgu, wd, r = (torch.randn(*s, dtype=torch.float64, requires_grad=True) for s in ((3, 5, 6), (14, 6), (4, 7), (3, 5, 4)))
+    g, u = F.linear(a, wgu[:7]), F.linear(a, wgu[7:])
+    torch.testing.assert_close(gemm.gated_mlp(a, wgu, wd, residual=r), F.linear(F.silu(g) * u, wd) + r)
+    torch.testing.assert_close(gemm.gated_mlp(a, wgu, wd, act="gelu"), F.linear(F.gelu(g, approximate="tanh") * u, wd))
+    assert torch.autograd.gradcheck(lambda *t: gemm.gated_mlp(*t), (a, wgu, wd))
+
+
+@pytest.mark.parametrize("change", [
+    dict(act="relu"), dict(a=torch.zeros(3, 5)), dict(w_gate_up=torch.zeros(13, 6)), dict(w_down=torch.zeros(4, 6)),
+    dict(w_down=torch.zeros(7)), dict(residual=torch.zeros(4)), dict(residual=torch.zeros(3, 6)),
+    dict(residual=torch.zeros(3, 4, dtype=torch.float64)), dict(a=torch.zeros(3, 6, dtype=torch.float64))])
+def test_gated_mlp_refuses(change):
+    from bluefog_b200.ops import gemm
+    args = dict(a=torch.zeros(3, 6), w_gate_up=torch.zeros(14, 6), w_down=torch.zeros(4, 7))
+    args.update(change)
+    with pytest.raises(ValueError):
+        gemm.gated_mlp(**args)
