@@ -10,16 +10,15 @@
 #include <map>
 #include <mutex>
 
+#include "block_ops.h"
 #include "common/logging.h"
 #include "common/runtime.h"
 #include "common/windows.h"
-#include "cuda/attn_tcgen05.h"
 #include "cuda/bn_kernels.h"
 #include "cuda/bucket.h"
 #include "cuda/combine_noalloc.h"
 #include "cuda/ce_kernels.h"
 #include "cuda/conv_tcgen05.h"
-#include "cuda/dropout_kernels.h"
 #include "cuda/embed_kernels.h"
 #include "cuda/gemm_tcgen05.h"
 #include "cuda/gpu_channel.h"
@@ -31,6 +30,13 @@
 
 namespace py = pybind11;
 using namespace bfb;
+
+// One device word per process that the GEMM kernel sets when a bounded wait expired.
+at::Tensor& bfb::GemmStatusWord(const at::Tensor& like) {
+  static at::Tensor status;
+  if (!status.defined()) status = at::zeros({1}, like.options().dtype(at::kInt));
+  return status;
+}
 
 namespace {
 
@@ -160,63 +166,6 @@ int PubElem(const std::string& dtype) {
   if (dtype == "float32") return kF32;
   if (dtype == "bfloat16") return kBF16;
   throw std::invalid_argument("published dtype must be float32 or bfloat16");
-}
-
-// One device word per process that the GEMM kernel sets when a bounded wait expired.
-at::Tensor& GemmStatusWord(const at::Tensor& like) {
-  static at::Tensor status;
-  if (!status.defined()) status = at::zeros({1}, like.options().dtype(at::kInt));
-  return status;
-}
-
-// The same for the attention kernels, one word per device (bits: AttnStatus).
-unsigned int* AttnStatusWord(int device) {
-  static std::mutex mu;
-  static std::map<int, at::Tensor> words;
-  std::lock_guard<std::mutex> lock(mu);
-  at::Tensor& w = words[device];
-  if (!w.defined()) w = at::zeros({1}, at::TensorOptions().device(at::kCUDA, device).dtype(at::kInt));
-  return reinterpret_cast<unsigned int*>(w.data_ptr<int>());
-}
-
-// Strides of a bf16 [tokens, heads, D] or [batch, tokens, heads, D] operand; extents of one have no stride of their own.
-AttnTensor ToAttn(const at::Tensor& t, const char* what) {
-  TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kBFloat16 && (t.dim() == 3 || t.dim() == 4) && t.numel() > 0,
-              what, " has to be a bf16 CUDA tensor [tokens, heads, D] or [batch, tokens, heads, D]");
-  const int64_t n = t.dim();
-  AttnTensor a;
-  a.ptr = t.data_ptr();
-  a.head_stride = t.size(n - 2) > 1 ? t.stride(n - 2) : (t.size(n - 1) + 7) / 8 * 8;
-  const bool one_token = t.size(n - 3) == 1 && (n == 3 || t.size(0) == 1);
-  a.token_stride = one_token ? t.size(n - 2) * a.head_stride : (t.size(n - 3) > 1 ? t.stride(n - 3) : t.stride(0));
-  TORCH_CHECK(t.stride(n - 1) == 1 && a.head_stride >= t.size(n - 1) && a.token_stride >= t.size(n - 2) * a.head_stride &&
-              a.head_stride % 8 == 0 && a.token_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(a.ptr) & 15) == 0 &&
-              (n == 3 || t.size(0) == 1 || t.size(1) == 1 || t.stride(0) == t.size(1) * a.token_stride),
-              what, ": rows have to be contiguous, 16-byte aligned and evenly spaced");
-  return a;
-}
-
-AttnShape ToAttnShape(const at::Tensor& q, const at::Tensor& k, const c10::optional<at::Tensor>& cu, double scale) {
-  const int64_t n = q.dim();
-  TORCH_CHECK(k.dim() == n && k.size(n - 1) == q.size(n - 1) && k.size(0) == q.size(0) && (n == 3 || k.size(1) == q.size(1)) &&
-              q.size(n - 2) % k.size(n - 2) == 0, "attention: q and k do not match");
-  AttnShape s;
-  if (cu.has_value() && cu->defined()) {
-    TORCH_CHECK(cu->is_cuda() && cu->get_device() == q.get_device() && cu->scalar_type() == at::kInt && cu->dim() == 1 &&
-                cu->numel() >= 2 && cu->is_contiguous(), "attention: cu_seqlens has to be contiguous int32 on the device of q");
-    s.cu = cu->data_ptr<int>();
-    s.batch = static_cast<int>(cu->numel() - 1);
-    s.seq = q.numel() / (q.size(n - 1) * q.size(n - 2));
-  } else {
-    s.batch = n == 4 ? static_cast<int>(q.size(0)) : 1;
-    s.seq = q.size(n - 3);
-  }
-  s.heads = static_cast<int>(q.size(n - 2));
-  s.kv_heads = static_cast<int>(k.size(n - 2));
-  s.dim = static_cast<int>(q.size(n - 1));
-  s.scale = static_cast<float>(scale);
-  TORCH_CHECK(AttnSupported(s), "attention: unsupported shape");
-  return s;
 }
 
 // ---- single-process world of windows: every "rank" is a block [WinHeader | self | one slot per source rank] on
@@ -1120,41 +1069,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     return out;
   });
 
-  // gated feed-forward block: h = act(a Wg^T) * (a Wu^T) with w = [Wg; Wu]; act 2 = GELU (tanh), 3 = SiLU.  Returns (h, [G U]),
-  // the second only where it is wanted (backward pass)
-  m.def("gemm_bf16_gated", [](at::Tensor a, at::Tensor w, int act, bool want_preact) {
-    TORCH_CHECK(a.is_cuda() && w.is_cuda() && w.get_device() == a.get_device() && a.dim() == 2 && w.dim() == 2 &&
-                a.scalar_type() == at::kBFloat16 && w.scalar_type() == at::kBFloat16 && a.is_contiguous() && w.is_contiguous() &&
-                a.size(1) == w.size(1) && a.size(1) % 8 == 0 && w.size(0) % 16 == 0 && a.numel() > 0 && w.numel() > 0 &&
-                a.size(0) < (1ll << 31) - 256, "gemm_bf16_gated expects contiguous bf16 [M,K], [2F,K] with K, F % 8 == 0");
-    c10::cuda::CUDAGuard g(a.get_device());
-    at::Tensor& status = GemmStatusWord(a);
-    const int64_t f = w.size(0) / 2;
-    at::Tensor h = at::empty({a.size(0), f}, a.options()), pre;
-    if (want_preact) pre = at::empty({a.size(0), 2 * f}, a.options());
-    cudaError_t e = LaunchGemmBf16Gated(a.data_ptr(), w.data_ptr(), h.data_ptr(), want_preact ? pre.data_ptr() : nullptr,
-                                        static_cast<int>(a.size(0)), static_cast<int>(f), static_cast<int>(a.size(1)), act,
-                                        reinterpret_cast<unsigned int*>(status.data_ptr()), CurrentStream(a.get_device()));
-    TORCH_CHECK(e == cudaSuccess, "gemm_bf16_gated launch failed: ", cudaGetErrorString(e));
-    return std::make_tuple(h, pre);
-  });
-  // [dG dU] from dH = a b and the kept [G U]
-  m.def("gemm_bf16_nn_gated_grad", [](at::Tensor a, at::Tensor b, at::Tensor preact, int act) {
-    TORCH_CHECK(a.is_cuda() && b.is_cuda() && preact.is_cuda() && a.dim() == 2 && b.dim() == 2 && preact.dim() == 2 &&
-                a.scalar_type() == at::kBFloat16 && b.scalar_type() == at::kBFloat16 && preact.scalar_type() == at::kBFloat16 &&
-                a.is_contiguous() && b.is_contiguous() && preact.is_contiguous() && a.size(1) == b.size(0) &&
-                preact.size(0) == a.size(0) && preact.size(1) == 2 * b.size(1) && b.get_device() == a.get_device() &&
-                preact.get_device() == a.get_device(), "gemm_bf16_nn_gated_grad expects contiguous bf16 [M,K], [K,F], [M,2F]");
-    c10::cuda::CUDAGuard g(a.get_device());
-    at::Tensor& status = GemmStatusWord(a);
-    at::Tensor out = at::empty(preact.sizes(), preact.options());
-    cudaError_t e = LaunchGemmBf16NNGatedGrad(a.data_ptr(), b.data_ptr(), preact.data_ptr(), out.data_ptr(), static_cast<int>(a.size(0)),
-                                              static_cast<int>(b.size(1)), static_cast<int>(a.size(1)), act,
-                                              reinterpret_cast<unsigned int*>(status.data_ptr()), CurrentStream(a.get_device()));
-    TORCH_CHECK(e == cudaSuccess, "gemm_bf16_nn_gated_grad launch failed: ", cudaGetErrorString(e));
-    return out;
-  });
-
   m.def("gemm_bf16_tn", [](at::Tensor a, at::Tensor b) {
     TORCH_CHECK(a.is_cuda() && b.is_cuda() && a.dim() == 2 && b.dim() == 2 && a.scalar_type() == at::kBFloat16 &&
                 b.scalar_type() == at::kBFloat16 && a.is_contiguous() && b.is_contiguous() && a.size(0) == b.size(0),
@@ -1169,39 +1083,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     return out;
   }, py::arg("a"), py::arg("b"));
 
-  // ---- causal attention over packed sequences ----------------------------------------------------
-  // q [.., heads, D], k and v [.., kv_heads, D]; returns (out, stats); stats only where they are wanted (backward pass)
-  m.def("attn_forward", [](at::Tensor q, at::Tensor k, at::Tensor v, c10::optional<at::Tensor> cu, double scale, bool want_stats) {
-    TORCH_CHECK(v.sizes() == k.sizes() && q.is_cuda() && k.is_cuda() && v.is_cuda() && k.get_device() == q.get_device() &&
-                v.get_device() == q.get_device(), "attn_forward: q, k and v do not match");
-    c10::cuda::CUDAGuard g(q.get_device());
-    const AttnTensor tq = ToAttn(q, "q"), tk = ToAttn(k, "k"), tv = ToAttn(v, "v");
-    const AttnShape s = ToAttnShape(q, k, cu, scale);
-    at::Tensor out = at::empty(q.sizes(), q.options());
-    at::Tensor stats;
-    if (want_stats) stats = at::empty({s.heads, AttnTiles(s), 128}, q.options().dtype(at::kFloat));
-    cudaError_t e = LaunchAttnForward(s, tq, tk, tv, ToAttn(out, "out"), want_stats ? stats.data_ptr<float>() : nullptr,
-                                      AttnStatusWord(q.get_device()), CurrentStream(q.get_device()));
-    TORCH_CHECK(e == cudaSuccess, "attn_forward launch failed: ", cudaGetErrorString(e));
-    return std::make_tuple(out, stats);
-  });
-  // writes dq, dk and dv (any strides that attn_forward would take)
-  m.def("attn_backward", [](at::Tensor dout, at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor out, at::Tensor stats,
-                            c10::optional<at::Tensor> cu, double scale, at::Tensor dq, at::Tensor dk, at::Tensor dv) {
-    c10::cuda::CUDAGuard g(q.get_device());
-    TORCH_CHECK(v.sizes() == k.sizes() && dout.sizes() == q.sizes() && out.sizes() == q.sizes() && dq.sizes() == q.sizes() &&
-                dk.sizes() == k.sizes() && dv.sizes() == k.sizes(), "attn_backward: shapes do not match");
-    for (const at::Tensor& t : {dout, k, v, out, stats, dq, dk, dv})
-      TORCH_CHECK(t.is_cuda() && t.get_device() == q.get_device(), "attn_backward: tensors on different devices");
-    const AttnShape s = ToAttnShape(q, k, cu, scale);
-    TORCH_CHECK(stats.scalar_type() == at::kFloat && stats.is_contiguous() && stats.numel() == s.heads * AttnTiles(s) * 128,
-                "attn_backward: statistics do not match q");
-    at::Tensor delta = at::empty_like(stats);
-    cudaError_t e = LaunchAttnBackward(s, ToAttn(q, "q"), ToAttn(k, "k"), ToAttn(v, "v"), ToAttn(out, "out"), ToAttn(dout, "dout"),
-                                       stats.data_ptr<float>(), delta.data_ptr<float>(), ToAttn(dq, "dq"), ToAttn(dk, "dk"),
-                                       ToAttn(dv, "dv"), AttnStatusWord(q.get_device()), CurrentStream(q.get_device()));
-    TORCH_CHECK(e == cudaSuccess, "attn_backward launch failed: ", cudaGetErrorString(e));
-  });
+  // ---- transformer-block operators with their backward passes (block_ops.cc) --------------------
+  m.def("causal_attention", &CausalAttention);
+  m.def("causal_self_attention", &CausalSelfAttention);
+  m.def("dropout_add", &DropoutAdd);
+  m.def("gated_mlp", &GatedMlp);
   // reads and clears the status word of the attention kernels (synchronises with the device)
   m.def("attn_status", [](int device) {
     c10::cuda::CUDAGuard g(device);
@@ -1213,28 +1099,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
     TORCH_CHECK(e == cudaSuccess, "attn_status failed: ", cudaGetErrorString(e));
     return value;
-  });
-
-  // ---- dropout joined with the residual stream ---------------------------------------------------
-  // threshold: of 65536 (dropped share); key: int64 [2] = (seed, step) on the device of x
-  m.def("dropout_add", [](at::Tensor x, c10::optional<at::Tensor> residual, int64_t threshold, double factor, at::Tensor key, int64_t site) {
-    TORCH_CHECK(x.is_cuda() && x.is_contiguous() && x.numel() > 0, "dropout_add expects a contiguous CUDA tensor");
-    TORCH_CHECK(key.is_cuda() && key.get_device() == x.get_device() && key.scalar_type() == at::kLong && key.numel() == 2 &&
-                key.is_contiguous(), "dropout_add: key has to be int64 [2] on the device of x");
-    TORCH_CHECK(threshold >= 0 && threshold <= 65536 && site >= 0 && site <= 65535, "dropout_add: threshold or site out of range");
-    const int type = x.scalar_type() == at::kFloat ? kDropF32 : x.scalar_type() == at::kHalf ? kDropF16 : kDropBF16;
-    TORCH_CHECK(type != kDropBF16 || x.scalar_type() == at::kBFloat16, "dropout_add: fp32, fp16 or bf16");
-    const void* res = PtrOrNull(residual);
-    if (res != nullptr)
-      TORCH_CHECK(residual->is_cuda() && residual->get_device() == x.get_device() && residual->sizes() == x.sizes() &&
-                  residual->scalar_type() == x.scalar_type() && residual->is_contiguous(), "dropout_add: residual does not match x");
-    c10::cuda::CUDAGuard g(x.get_device());
-    at::Tensor out = at::empty(x.sizes(), x.options());
-    cudaError_t e = LaunchDropoutAdd(x.data_ptr(), res, out.data_ptr(), x.numel(), type, static_cast<unsigned int>(threshold),
-                                     static_cast<float>(factor), reinterpret_cast<const long long*>(key.data_ptr<int64_t>()),
-                                     static_cast<unsigned int>(site), CurrentStream(x.get_device()));
-    TORCH_CHECK(e == cudaSuccess, "dropout_add launch failed: ", cudaGetErrorString(e));
-    return out;
   });
 
   m.def("gemm_status", [] {

@@ -1,0 +1,384 @@
+// Autograd nodes of the transformer-block operators.  They are C++ nodes because a training step calls them once per layer
+// and direction: with Python functions around the same launches an operator of 10 us cost 70 us of host time.
+#include "block_ops.h"
+
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+
+#include <map>
+#include <mutex>
+
+#include "cuda/attn_tcgen05.h"
+#include "cuda/dropout_kernels.h"
+#include "cuda/gemm_tcgen05.h"
+
+namespace bfb {
+namespace {
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+cudaStream_t StreamOf(const at::Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
+
+void Check(cudaError_t e, const char* what) { TORCH_CHECK(e == cudaSuccess, what, " launch failed: ", cudaGetErrorString(e)); }
+
+bool Aligned(const at::Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0; }
+
+// t itself where its memory is dense and 16-byte aligned, else a copy
+at::Tensor Dense(const at::Tensor& t) {
+  return t.is_contiguous() && Aligned(t) ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+at::Tensor OrUndefined(const c10::optional<at::Tensor>& t) { return t.has_value() ? *t : at::Tensor(); }
+
+bool NeedsGrad(std::initializer_list<at::Tensor> tensors) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const at::Tensor& t : tensors)
+    if (t.defined() && t.requires_grad()) return true;
+  return false;
+}
+
+// Gradients of these operators are not differentiable; asking for theirs is an error, at the time they are asked for.
+variable_list Once(const char* what, variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  auto node = std::make_shared<torch::autograd::DelayedError>(std::string(what) + " can be differentiated only once",
+                                                             static_cast<int64_t>(grads.size()));
+  return (*node)(std::move(grads));
+}
+
+// ---- attention -----------------------------------------------------------------------------------------------------
+
+// Spacing of the rows of t [.., tokens, columns...] (`inner` trailing dimensions belong to a row); 0 when they are not evenly spaced.
+// Extents of one have no spacing of their own.
+int64_t RowStride(const at::Tensor& t, int64_t inner, int64_t row_size) {
+  const int64_t n = t.dim() - inner;
+  int64_t stride = 0, span = 0;
+  for (int64_t i = n - 1; i >= 0; --i) {
+    if (t.size(i) == 1) continue;
+    if (stride == 0) stride = t.stride(i);
+    else if (t.stride(i) != span) return 0;
+    span = t.stride(i) * t.size(i);
+  }
+  return stride == 0 ? (row_size + 7) / 8 * 8 : stride;
+}
+
+// A [.., tokens, heads, D] operand, or false where the kernels cannot address it.
+bool Describe(const at::Tensor& t, AttnTensor* a) {
+  const int64_t n = t.dim(), heads = t.size(n - 2), d = t.size(n - 1);
+  a->ptr = t.data_ptr();
+  a->head_stride = heads > 1 ? t.stride(n - 2) : (d + 7) / 8 * 8;
+  a->token_stride = RowStride(t, 2, heads * a->head_stride);
+  return t.stride(n - 1) == 1 && Aligned(t) && a->head_stride % 8 == 0 && a->head_stride >= d && a->token_stride % 8 == 0 &&
+         a->token_stride >= heads * a->head_stride;
+}
+at::Tensor Rows(const at::Tensor& t) {
+  AttnTensor a;
+  return Describe(t, &a) ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+AttnTensor Described(const at::Tensor& t) {
+  AttnTensor a;
+  TORCH_CHECK(Describe(t, &a), "attention: rows have to be contiguous, 16-byte aligned and evenly spaced");
+  return a;
+}
+// qkv with rows that the kernels can address
+at::Tensor QkvRows(const at::Tensor& t) {
+  const int64_t cols = t.size(-1), stride = RowStride(t, 1, cols);
+  return t.stride(-1) == 1 && Aligned(t) && stride % 8 == 0 && stride >= cols ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+// the columns of `heads` heads of width d that start with head `first`
+AttnTensor QkvPart(const at::Tensor& t, int64_t first, int64_t d) {
+  AttnTensor a;
+  a.ptr = static_cast<char*>(t.data_ptr()) + first * d * 2;
+  a.head_stride = d;
+  a.token_stride = RowStride(t, 1, t.size(-1));
+  return a;
+}
+
+// lead: the dimensions in front of (heads, D)
+AttnShape ShapeOf(at::IntArrayRef lead, int64_t heads, int64_t kv_heads, int64_t d, const at::Tensor& cu, double scale, const at::Tensor& like) {
+  TORCH_CHECK(like.is_cuda() && like.scalar_type() == at::kBFloat16, "attention expects bf16 CUDA tensors");
+  int64_t tokens = 1;
+  for (int64_t n : lead) tokens *= n;
+  AttnShape s;
+  if (cu.defined()) {
+    TORCH_CHECK(cu.is_cuda() && cu.get_device() == like.get_device() && cu.scalar_type() == at::kInt && cu.dim() == 1 &&
+                cu.numel() >= 2 && cu.is_contiguous(), "attention: cu_seqlens has to be contiguous int32 on the device of q");
+    s.cu = cu.data_ptr<int>();
+    s.batch = static_cast<int>(cu.numel() - 1);
+    s.seq = tokens;
+  } else {
+    s.seq = lead.back();
+    s.batch = static_cast<int>(tokens / s.seq);
+  }
+  s.heads = static_cast<int>(heads);
+  s.kv_heads = static_cast<int>(kv_heads);
+  s.dim = static_cast<int>(d);
+  s.scale = static_cast<float>(scale);
+  TORCH_CHECK(AttnSupported(s), "attention: unsupported shape");
+  return s;
+}
+AttnShape ShapeOf(const at::Tensor& q, const at::Tensor& k, const at::Tensor& cu, double scale) {
+  const int64_t n = q.dim();
+  TORCH_CHECK(n >= 3 && k.dim() == n && q.numel() > 0 && k.sizes().slice(0, n - 2) == q.sizes().slice(0, n - 2) && k.size(n - 1) == q.size(n - 1),
+              "attention: q and k do not match");
+  return ShapeOf(q.sizes().slice(0, n - 2), q.size(n - 2), k.size(n - 2), q.size(n - 1), cu, scale, q);
+}
+AttnShape QkvShape(const at::Tensor& qkv, int64_t heads, int64_t kv_heads, const at::Tensor& cu, double scale) {
+  TORCH_CHECK(qkv.dim() >= 2 && qkv.numel() > 0 && heads > 0 && kv_heads > 0 && qkv.size(-1) % (heads + 2 * kv_heads) == 0,
+              "attention: columns do not match the heads");
+  return ShapeOf(qkv.sizes().slice(0, qkv.dim() - 1), heads, kv_heads, qkv.size(-1) / (heads + 2 * kv_heads), cu, scale, qkv);
+}
+at::Tensor StatsFor(const AttnShape& s, const at::Tensor& like) {
+  return at::empty({s.heads, AttnTiles(s), 128}, like.options().dtype(at::kFloat));
+}
+float* StatsPtr(const at::Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
+
+at::Tensor SeparateForward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cu, double scale, at::Tensor* stats) {
+  TORCH_CHECK(v.sizes() == k.sizes() && k.get_device() == q.get_device() && v.get_device() == q.get_device() &&
+              k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(), "attention: q, k and v do not match");
+  const AttnShape s = ShapeOf(q, k, cu, scale);
+  at::Tensor out = at::empty(q.sizes(), q.options());
+  if (stats != nullptr) *stats = StatsFor(s, q);
+  Check(LaunchAttnForward(s, Described(q), Described(k), Described(v), Described(out), stats != nullptr ? StatsPtr(*stats) : nullptr,
+                          AttnStatusWord(q.get_device()), StreamOf(q)), "attention forward");
+  return out;
+}
+
+struct AttentionNode : public torch::autograd::Function<AttentionNode> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& q0, const at::Tensor& k0, const at::Tensor& v0,
+                            const c10::optional<at::Tensor>& boundaries, double scale) {
+    const at::Tensor cu = OrUndefined(boundaries);
+    const at::Tensor q = Rows(q0), k = Rows(k0), v = Rows(v0);
+    at::Tensor stats;
+    at::Tensor out = SeparateForward(q, k, v, cu, scale, &stats);
+    ctx->save_for_backward({q, k, v, cu, out, stats});
+    ctx->saved_data["scale"] = scale;
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    const at::Tensor &q = saved[0], &k = saved[1], &v = saved[2], &out = saved[4], &stats = saved[5];
+    const c10::cuda::CUDAGuard guard(q.get_device());
+    const AttnShape s = ShapeOf(q, k, saved[3], ctx->saved_data["scale"].toDouble());
+    const at::Tensor dout = Rows(grads[0]);
+    at::Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()), dv = at::empty(v.sizes(), v.options());
+    at::Tensor delta = at::empty_like(stats);
+    Check(LaunchAttnBackward(s, Described(q), Described(k), Described(v), Described(out), Described(dout), StatsPtr(stats), StatsPtr(delta),
+                             Described(dq), Described(dk), Described(dv), AttnStatusWord(q.get_device()), StreamOf(q)), "attention backward");
+    variable_list g = Once("attention", {dq, dk, dv});
+    return {g[0], g[1], g[2], at::Tensor(), at::Tensor()};
+  }
+};
+
+at::Tensor QkvForward(const at::Tensor& qkv, int64_t h, int64_t hkv, const at::Tensor& cu, double scale, at::Tensor* stats) {
+  const AttnShape s = QkvShape(qkv, h, hkv, cu, scale);
+  std::vector<int64_t> sizes(qkv.sizes().begin(), qkv.sizes().end() - 1);
+  sizes.push_back(h);
+  sizes.push_back(s.dim);
+  at::Tensor out = at::empty(sizes, qkv.options());
+  if (stats != nullptr) *stats = StatsFor(s, qkv);
+  Check(LaunchAttnForward(s, QkvPart(qkv, 0, s.dim), QkvPart(qkv, h, s.dim), QkvPart(qkv, h + hkv, s.dim), Described(out),
+                          stats != nullptr ? StatsPtr(*stats) : nullptr, AttnStatusWord(qkv.get_device()), StreamOf(qkv)),
+        "attention forward");
+  return out;
+}
+
+struct SelfAttentionNode : public torch::autograd::Function<SelfAttentionNode> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& qkv0, int64_t h, int64_t hkv, const c10::optional<at::Tensor>& boundaries,
+                            double scale) {
+    const at::Tensor cu = OrUndefined(boundaries);
+    const at::Tensor qkv = QkvRows(qkv0);
+    at::Tensor stats;
+    at::Tensor out = QkvForward(qkv, h, hkv, cu, scale, &stats);
+    ctx->save_for_backward({qkv, cu, out, stats});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["h"] = h;
+    ctx->saved_data["hkv"] = hkv;
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    const at::Tensor &qkv = saved[0], &out = saved[2], &stats = saved[3];
+    const c10::cuda::CUDAGuard guard(qkv.get_device());
+    const int64_t h = ctx->saved_data["h"].toInt(), hkv = ctx->saved_data["hkv"].toInt();
+    const AttnShape s = QkvShape(qkv, h, hkv, saved[1], ctx->saved_data["scale"].toDouble());
+    const at::Tensor dout = Rows(grads[0]);
+    at::Tensor dqkv = at::empty(qkv.sizes(), qkv.options()), delta = at::empty_like(stats);
+    Check(LaunchAttnBackward(s, QkvPart(qkv, 0, s.dim), QkvPart(qkv, h, s.dim), QkvPart(qkv, h + hkv, s.dim), Described(out), Described(dout),
+                             StatsPtr(stats), StatsPtr(delta), QkvPart(dqkv, 0, s.dim), QkvPart(dqkv, h, s.dim), QkvPart(dqkv, h + hkv, s.dim),
+                             AttnStatusWord(qkv.get_device()), StreamOf(qkv)), "attention backward");
+    return {Once("attention", {dqkv})[0], at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+
+// ---- dropout -------------------------------------------------------------------------------------------------------
+
+at::Tensor DropoutLaunch(const at::Tensor& x, const at::Tensor& residual, int64_t threshold, double factor, const at::Tensor& key, int64_t site) {
+  int type = -1;
+  switch (x.scalar_type()) {
+    case at::kFloat: type = kDropF32; break;
+    case at::kHalf: type = kDropF16; break;
+    case at::kBFloat16: type = kDropBF16; break;
+    default: TORCH_CHECK(false, "dropout_add: fp32, fp16 or bf16");
+  }
+  TORCH_CHECK(x.is_cuda() && x.numel() > 0 && key.is_cuda() && key.get_device() == x.get_device() && key.scalar_type() == at::kLong &&
+              key.numel() == 2 && threshold >= 0 && threshold <= 65536 && site >= 0 && site <= 65535, "dropout_add: bad arguments");
+  if (residual.defined())
+    TORCH_CHECK(residual.get_device() == x.get_device() && residual.sizes() == x.sizes() && residual.scalar_type() == x.scalar_type(),
+                "dropout_add: residual does not match x");
+  const at::Tensor a = Dense(x), r = residual.defined() ? Dense(residual) : residual, k = key.contiguous();
+  at::Tensor out = at::empty(x.sizes(), x.options());
+  Check(LaunchDropoutAdd(a.data_ptr(), r.defined() ? r.data_ptr() : nullptr, out.data_ptr(), a.numel(), type, static_cast<unsigned int>(threshold),
+                         static_cast<float>(factor), reinterpret_cast<const long long*>(k.data_ptr<int64_t>()),
+                         static_cast<unsigned int>(site), StreamOf(x)), "dropout_add");
+  return out;
+}
+
+struct DropoutNode : public torch::autograd::Function<DropoutNode> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const c10::optional<at::Tensor>& residual, int64_t threshold,
+                            double factor, const at::Tensor& key, int64_t site) {
+    ctx->save_for_backward({key});
+    ctx->saved_data["threshold"] = threshold;
+    ctx->saved_data["factor"] = factor;
+    ctx->saved_data["site"] = site;
+    ctx->saved_data["residual"] = residual.has_value();
+    return DropoutLaunch(x, OrUndefined(residual), threshold, factor, key, site);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    at::Tensor dx;
+    const at::Tensor dy = grads[0];
+    if (ctx->needs_input_grad(0))                       // the operator itself without a residual: differentiable again
+      dx = DropoutAdd(dy, c10::nullopt, ctx->saved_data["threshold"].toInt(), ctx->saved_data["factor"].toDouble(),
+                      ctx->get_saved_variables()[0], ctx->saved_data["site"].toInt());
+    // needs_input_grad counts the tensors that were given
+    return {dx, ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(1) ? dy : at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+
+// ---- gated feed-forward block --------------------------------------------------------------------------------------
+
+unsigned int* GemmStatus(const at::Tensor& like) { return reinterpret_cast<unsigned int*>(GemmStatusWord(like).data_ptr()); }
+
+at::Tensor GatedProduct(const at::Tensor& a, const at::Tensor& w_gate_up, int64_t act, at::Tensor* pre) {
+  const int64_t m = a.size(0), f = w_gate_up.size(0) / 2;
+  at::Tensor h = at::empty({m, f}, a.options());
+  if (pre != nullptr) *pre = at::empty({m, 2 * f}, a.options());
+  Check(LaunchGemmBf16Gated(a.data_ptr(), w_gate_up.data_ptr(), h.data_ptr(), pre != nullptr ? pre->data_ptr() : nullptr, static_cast<int>(m),
+                            static_cast<int>(f), static_cast<int>(a.size(1)), static_cast<int>(act), GemmStatus(a), StreamOf(a)),
+        "gated_mlp");
+  return h;
+}
+at::Tensor DownProduct(const at::Tensor& h, const at::Tensor& w_down, const at::Tensor& residual) {
+  at::Tensor y = at::empty({h.size(0), w_down.size(0)}, h.options());
+  Check(LaunchGemmBf16NT(h.data_ptr(), w_down.data_ptr(), y.data_ptr(), nullptr, static_cast<int>(h.size(0)), static_cast<int>(w_down.size(0)),
+                         static_cast<int>(h.size(1)), kActNone, GemmStatus(h), StreamOf(h), nullptr, nullptr,
+                         residual.defined() ? residual.data_ptr() : nullptr), "gated_mlp");
+  return y;
+}
+// a^T b of two matrices with the same rows: a weight's gradient
+at::Tensor TransposedProduct(const at::Tensor& a, const at::Tensor& b) {
+  at::Tensor out = at::empty({a.size(1), b.size(1)}, a.options());
+  Check(LaunchGemmBf16TN(a.data_ptr(), b.data_ptr(), out.data_ptr(), static_cast<int>(a.size(1)), static_cast<int>(b.size(1)),
+                         static_cast<int>(a.size(0)), GemmStatus(a), StreamOf(a)), "gated_mlp backward");
+  return out;
+}
+at::Tensor Rows2d(const at::Tensor& t) { return Dense(t.reshape({-1, t.size(-1)})); }
+std::vector<int64_t> WithColumns(const at::Tensor& a, int64_t columns) {
+  std::vector<int64_t> s(a.sizes().begin(), a.sizes().end());
+  s.back() = columns;
+  return s;
+}
+
+// Kept for the backward pass: both pre-activations and their gated product, rounded to bf16 like every activation.
+struct GatedMlpNode : public torch::autograd::Function<GatedMlpNode> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& a0, const at::Tensor& wgu0, const at::Tensor& wd0, int64_t act,
+                            const c10::optional<at::Tensor>& residual) {
+    const at::Tensor a = Rows2d(a0), wgu = Dense(wgu0), wd = Dense(wd0);
+    at::Tensor pre;
+    const at::Tensor h = GatedProduct(a, wgu, act, &pre);
+    at::Tensor y = DownProduct(h, wd, residual.has_value() ? Rows2d(*residual) : at::Tensor());
+    ctx->save_for_backward({a, wgu, wd, pre, h});
+    ctx->saved_data["residual"] = residual.has_value();
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["sizes"] = a0.sizes().vec();
+    return y.view(WithColumns(a0, wd.size(0)));
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    const at::Tensor &a = saved[0], &wgu = saved[1], &wd = saved[2], &pre = saved[3], &h = saved[4];
+    const c10::cuda::CUDAGuard guard(a.get_device());
+    const at::Tensor dy = Rows2d(grads[0]);
+    const int m = static_cast<int>(a.size(0)), f = static_cast<int>(h.size(1)), k = static_cast<int>(a.size(1));
+    at::Tensor da, dwgu, dwd;
+    if (ctx->needs_input_grad(0) || ctx->needs_input_grad(1)) {
+      // [dG dU] straight from the epilogue of dH = dy Wd
+      at::Tensor dpre = at::empty(pre.sizes(), pre.options());
+      Check(LaunchGemmBf16NNGatedGrad(dy.data_ptr(), wd.data_ptr(), pre.data_ptr(), dpre.data_ptr(), m, f, static_cast<int>(wd.size(0)),
+                                      static_cast<int>(ctx->saved_data["act"].toInt()), GemmStatus(a), StreamOf(a)), "gated_mlp backward");
+      if (ctx->needs_input_grad(0)) {
+        da = at::empty(a.sizes(), a.options());
+        Check(LaunchGemmBf16NN(dpre.data_ptr(), wgu.data_ptr(), da.data_ptr(), m, k, 2 * f, GemmStatus(a), StreamOf(a)), "gated_mlp backward");
+        da = da.view(ctx->saved_data["sizes"].toIntVector());
+      }
+      if (ctx->needs_input_grad(1)) dwgu = TransposedProduct(dpre, a);
+    }
+    if (ctx->needs_input_grad(2)) dwd = TransposedProduct(dy, h);
+    variable_list g = Once("gated_mlp", {da, dwgu, dwd});
+    return {g[0], g[1], g[2], at::Tensor(), ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(3) ? grads[0] : at::Tensor()};
+  }
+};
+
+}  // namespace
+
+unsigned int* AttnStatusWord(int device) {
+  static std::mutex mu;
+  static std::map<int, at::Tensor> words;
+  std::lock_guard<std::mutex> lock(mu);
+  at::Tensor& w = words[device];
+  if (!w.defined()) w = at::zeros({1}, at::TensorOptions().device(at::kCUDA, device).dtype(at::kInt));
+  return reinterpret_cast<unsigned int*>(w.data_ptr<int>());
+}
+
+at::Tensor CausalAttention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const c10::optional<at::Tensor>& cu, double scale) {
+  TORCH_CHECK(q.is_cuda() && k.is_cuda() && v.is_cuda(), "attention expects CUDA tensors");
+  const c10::cuda::CUDAGuard guard(q.get_device());
+  if (NeedsGrad({q, k, v})) return AttentionNode::apply(q, k, v, cu, scale);
+  return SeparateForward(Rows(q), Rows(k), Rows(v), OrUndefined(cu), scale, nullptr);
+}
+
+at::Tensor CausalSelfAttention(const at::Tensor& qkv, int64_t heads, int64_t kv_heads, const c10::optional<at::Tensor>& cu, double scale) {
+  TORCH_CHECK(qkv.is_cuda(), "attention expects CUDA tensors");
+  const c10::cuda::CUDAGuard guard(qkv.get_device());
+  if (NeedsGrad({qkv})) return SelfAttentionNode::apply(qkv, heads, kv_heads, cu, scale);
+  return QkvForward(QkvRows(qkv), heads, kv_heads, OrUndefined(cu), scale, nullptr);
+}
+
+at::Tensor DropoutAdd(const at::Tensor& x, const c10::optional<at::Tensor>& residual, int64_t threshold, double factor,
+                      const at::Tensor& key, int64_t site) {
+  TORCH_CHECK(x.is_cuda(), "dropout_add expects a CUDA tensor");
+  const c10::cuda::CUDAGuard guard(x.get_device());
+  const at::Tensor r = OrUndefined(residual);
+  if (NeedsGrad({x, r})) return DropoutNode::apply(x, residual, threshold, factor, key, site);
+  return DropoutLaunch(x, r, threshold, factor, key, site);
+}
+
+at::Tensor GatedMlp(const at::Tensor& a, const at::Tensor& w_gate_up, const at::Tensor& w_down, int64_t act,
+                    const c10::optional<at::Tensor>& residual) {
+  const at::Tensor r = OrUndefined(residual);
+  for (const at::Tensor& t : {a, w_gate_up, w_down, r})
+    TORCH_CHECK(!t.defined() || (t.is_cuda() && t.get_device() == a.get_device() && t.scalar_type() == at::kBFloat16),
+                "gated_mlp expects bf16 tensors on one CUDA device");
+  TORCH_CHECK(a.dim() >= 1 && w_gate_up.dim() == 2 && w_down.dim() == 2 && a.numel() > 0 && w_gate_up.numel() > 0 && w_down.numel() > 0 &&
+              w_gate_up.size(1) == a.size(-1) && w_gate_up.size(0) == 2 * w_down.size(1) && a.size(-1) % 8 == 0 && w_down.size(0) % 8 == 0 &&
+              w_down.size(1) % 8 == 0 && a.numel() / a.size(-1) < (1ll << 31) - 256, "gated_mlp: sizes do not match");
+  if (r.defined()) TORCH_CHECK(r.sizes() == at::IntArrayRef(WithColumns(a, w_down.size(0))), "gated_mlp: residual does not match");
+  const c10::cuda::CUDAGuard guard(a.get_device());
+  if (NeedsGrad({a, w_gate_up, w_down, r})) return GatedMlpNode::apply(a, w_gate_up, w_down, act, residual);
+  const at::Tensor h = GatedProduct(Rows2d(a), Dense(w_gate_up), act, nullptr);
+  return DownProduct(h, Dense(w_down), r.defined() ? Rows2d(r) : r).view(WithColumns(a, w_down.size(0)));
+}
+
+}  // namespace bfb

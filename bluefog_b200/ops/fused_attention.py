@@ -19,28 +19,16 @@ import math
 
 import torch
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 
 from bluefog_b200.common.basics import get_basics
 
 _b = get_basics()
 
 
-def _eligible(q, k, v):
-    return (q.is_cuda and q.dtype == torch.bfloat16 and k.dtype == q.dtype and v.dtype == q.dtype and q.shape[-1] % 8 == 0
-            and 8 <= q.shape[-1] <= 128 and q.numel() // (q.shape[-1] * q.shape[-2]) < 2 ** 31 - 256
-            and _b.native is not None and hasattr(_b.native, "attn_forward") and _b.native.gemm_supported())
-
-
-def _rows(t):
-    """``t`` [tokens, heads, D] or [batch, tokens, heads, D] itself if the kernels can address it, else a copy."""
-    h, d = t.shape[-2:]
-    head = t.stride(-2) if h > 1 else (d + 7) // 8 * 8
-    tokens = [(n, s) for n, s in zip(t.shape[:-2], t.stride()[:-2]) if n > 1]
-    ok = (t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and head % 8 == 0 and head >= d
-          and all(s % 8 == 0 and s >= h * head for _, s in tokens)
-          and (len(tokens) < 2 or tokens[0][1] == tokens[1][0] * tokens[1][1]))
-    return t if ok else t.clone(memory_format=torch.contiguous_format)
+def _eligible(t, d):
+    """Whether the kernels take ``t`` (q, or q, k and v side by side) with heads of width ``d``."""
+    return (t.is_cuda and t.dtype == torch.bfloat16 and d % 8 == 0 and 8 <= d <= 128 and t.numel() // d < 2 ** 31 - 256
+            and _b.native.gemm_supported())
 
 
 def _split(qkv, h, hkv):
@@ -48,43 +36,6 @@ def _split(qkv, h, hkv):
     lead = qkv.shape[:-1]
     return (qkv[..., :h * d].view(*lead, h, d), qkv[..., h * d:(h + hkv) * d].view(*lead, hkv, d),
             qkv[..., (h + hkv) * d:].view(*lead, hkv, d))
-
-
-class _AttentionFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, cu, scale):
-        q, k, v = _rows(q), _rows(k), _rows(v)
-        out, stats = _b.native.attn_forward(q, k, v, cu, scale, True)
-        ctx.save_for_backward(q, k, v, out, stats, cu)
-        ctx.scale = scale
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dout):
-        q, k, v, out, stats, cu = ctx.saved_tensors
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        _b.native.attn_backward(_rows(dout), q, k, v, out, stats, cu, ctx.scale, dq, dk, dv)
-        return dq, dk, dv, None, None
-
-
-class _SelfAttentionFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, qkv, h, hkv, cu, scale):
-        q, k, v = (_rows(t) for t in _split(qkv, h, hkv))
-        out, stats = _b.native.attn_forward(q, k, v, cu, scale, True)
-        ctx.save_for_backward(q, k, v, out, stats, cu)
-        ctx.args = h, hkv, scale, qkv.shape
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dout):
-        q, k, v, out, stats, cu = ctx.saved_tensors
-        h, hkv, scale, shape = ctx.args
-        dqkv = torch.empty(shape, dtype=q.dtype, device=q.device)
-        _b.native.attn_backward(_rows(dout), q, k, v, out, stats, cu, scale, *_split(dqkv, h, hkv))
-        return dqkv, None, None, None, None
 
 
 def _plain(q, k, v, cu, scale):
@@ -131,12 +82,9 @@ def causal_attention(q, k, v, cu_seqlens=None, scale=None):
     scale = _check(q.shape[-2], k.shape[-2], q.shape[-1], q.device, cu_seqlens, scale)
     if q.numel() == 0:
         return q + (k.sum() + v.sum()) * 0
-    if not _eligible(q, k, v):
+    if not _eligible(q, q.shape[-1]):
         return _plain(q, k, v, cu_seqlens, scale)
-    cu = None if cu_seqlens is None else cu_seqlens.contiguous()
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return _AttentionFn.apply(q, k, v, cu, scale)
-    return _b.native.attn_forward(_rows(q), _rows(k), _rows(v), cu, scale, False)[0]
+    return _b.native.causal_attention(q, k, v, None if cu_seqlens is None else cu_seqlens.contiguous(), scale)
 
 
 def causal_self_attention(qkv, n_head, n_kv_head=None, cu_seqlens=None, scale=None):
@@ -146,13 +94,10 @@ def causal_self_attention(qkv, n_head, n_kv_head=None, cu_seqlens=None, scale=No
         raise ValueError("causal_self_attention: %d columns are not (%d + 2 * %d) heads of equal width in a [.., T, columns] tensor"
                          % (qkv.shape[-1], n_head, hkv))
     scale = _check(n_head, hkv, qkv.shape[-1] // (n_head + 2 * hkv), qkv.device, cu_seqlens, scale)
-    q, k, v = _split(qkv, n_head, hkv)
-    if qkv.numel() == 0 or not _eligible(q, k, v):
-        return causal_attention(q, k, v, cu_seqlens, scale)
-    cu = None if cu_seqlens is None else cu_seqlens.contiguous()
-    if torch.is_grad_enabled() and qkv.requires_grad:
-        return _SelfAttentionFn.apply(qkv, n_head, hkv, cu, scale)
-    return _b.native.attn_forward(_rows(q), _rows(k), _rows(v), cu, scale, False)[0]
+    d = qkv.shape[-1] // (n_head + 2 * hkv)
+    if qkv.numel() == 0 or not _eligible(qkv, d):
+        return causal_attention(*_split(qkv, n_head, hkv), cu_seqlens, scale)
+    return _b.native.causal_self_attention(qkv, n_head, hkv, None if cu_seqlens is None else cu_seqlens.contiguous(), scale)
 
 
 def check_sequences(device=None):

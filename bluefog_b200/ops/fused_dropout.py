@@ -13,7 +13,6 @@ elements are zero whatever x holds.  CUDA tensors in fp32, fp16 or bf16 take the
 takes the same generator in PyTorch's operators.  The reference has no dropout of its own.
 """
 import torch
-from torch.autograd.function import once_differentiable
 
 from bluefog_b200.common.basics import get_basics
 
@@ -26,12 +25,7 @@ def new_key(seed, device=None):
 
 
 def _eligible(x):
-    return x.is_cuda and x.dtype in (torch.float32, torch.float16, torch.bfloat16) and _b.native is not None and hasattr(_b.native, "dropout_add")
-
-
-def _dense(t):
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    return x.is_cuda and x.dtype in (torch.float32, torch.float16, torch.bfloat16) and x.numel() < 2 ** 51
 
 
 def _keep(count, threshold, key, site):
@@ -49,22 +43,6 @@ def _keep(count, threshold, key, site):
     return torch.stack((words & 0xFFFF, words >> 16), 2).reshape(-1)[:count] >= threshold
 
 
-class _DropoutAddFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, residual, threshold, factor, key, site):
-        ctx.save_for_backward(key)
-        ctx.args = threshold, factor, site
-        return _b.native.dropout_add(_dense(x), None if residual is None else _dense(residual), threshold, factor, key, site)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        (key,) = ctx.saved_tensors
-        threshold, factor, site = ctx.args
-        dx = _b.native.dropout_add(_dense(dy), None, threshold, factor, key, site) if ctx.needs_input_grad[0] else None
-        return dx, (dy if ctx.needs_input_grad[1] else None), None, None, None, None
-
-
 def dropout_add(x, residual, p, key, site=0):
     """``residual + dropout(x, p)`` (``residual`` may be None); ``key``: int64 ``[seed, step]``, see the module's notes."""
     if not 0.0 <= p <= 1.0:
@@ -80,7 +58,7 @@ def dropout_add(x, residual, p, key, site=0):
     threshold = round(p * 65536)
     factor = 65536.0 / (65536 - threshold) if threshold < 65536 else 0.0
     if x.numel() > 0 and _eligible(x):
-        return _DropoutAddFn.apply(x, residual, threshold, factor, key.contiguous(), site)
+        return _b.native.dropout_add(x, residual, threshold, factor, key, site)
     keep = _keep(x.numel(), threshold, key, site).view(x.shape)
     y = torch.where(keep, x * factor, torch.zeros((), dtype=x.dtype, device=x.device))
     return y if residual is None else y + residual

@@ -7,7 +7,6 @@ MN-major (products with too few output tiles for a kernel without split-K go to 
 ``_LinearFn.backward``).
 """
 import torch
-from torch.autograd.function import once_differentiable
 
 from bluefog_b200.common.basics import get_basics
 from bluefog_b200.ops import fused_ln
@@ -258,41 +257,11 @@ def mlp_gelu(a: torch.Tensor, w1: torch.Tensor, b1, w2: torch.Tensor, b2, residu
 _GATES = {"gelu": 2, "silu": 3}
 
 
-class _GatedMlpFn(torch.autograd.Function):
-    """y = (act(a Wg^T) * (a Wu^T)) Wd^T with the activation and the product inside GEMM epilogues: one product makes gate
-    and up columns side by side in its accumulator, and the input gradient of the down projection leaves as the gradients
-    of both.  Kept for the backward pass: both pre-activations and their product, rounded to bf16 like every activation."""
-
-    @staticmethod
-    def forward(ctx, a, w_gate_up, w_down, act, residual):
-        h, pre = _b.native.gemm_bf16_gated(a, w_gate_up, act, True)
-        y = _b.native.gemm_bf16_nt(h, w_down, None, 0, None, residual)        # residual joins in the epilogue
-        ctx.save_for_backward(a, w_gate_up, w_down, pre, h)
-        ctx.act = act
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        a, w_gate_up, w_down, pre, h = ctx.saved_tensors
-        dy = _aligned(dy)
-        C = _b.native
-        dpre = C.gemm_bf16_nn_gated_grad(dy, w_down, pre, ctx.act)            # dH, then [dG dU], in one epilogue
-        da = C.gemm_bf16_nn(dpre, w_gate_up) if ctx.needs_input_grad[0] else None
-        dw_gate_up = C.gemm_bf16_tn(dpre, a) if ctx.needs_input_grad[1] else None
-        dw_down = C.gemm_bf16_tn(dy, h) if ctx.needs_input_grad[2] else None
-        return da, dw_gate_up, dw_down, None, (dy if ctx.needs_input_grad[4] else None)
-
-
-def _aligned(t):
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
-
-
 def gated_mlp(a: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor, act: str = "silu", residual=None) -> torch.Tensor:
     """``(act(a @ Wg.T) * (a @ Wu.T)) @ w_down.T (+ residual)`` with ``w_gate_up`` = [Wg; Wu] ``[2 F, K]`` and ``w_down``
     ``[N, F]``; ``a`` [.., K], ``residual`` [.., N]; ``act`` "silu" or "gelu" (the tanh approximation).  bf16 CUDA tensors
-    with K, F and N multiples of 8 take the tcgen05 kernels; other inputs take PyTorch's ops."""
+    with K, F and N multiples of 8 take the tcgen05 kernels, the activation and the product with the gate inside GEMM
+    epilogues in both directions; other inputs take PyTorch's ops."""
     if act not in _GATES:
         raise ValueError("gated_mlp: act has to be one of %s, got %r" % (sorted(_GATES), act))
     if (a.dim() < 1 or w_gate_up.dim() != 2 or w_down.dim() != 2 or w_gate_up.shape[1] != a.shape[-1]
@@ -306,14 +275,10 @@ def gated_mlp(a: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor, ac
     if any(t.device != a.device or t.dtype != a.dtype for t in tensors):
         raise ValueError("gated_mlp: all tensors have to share a device and a type")
     ok = (a.is_cuda and a.dtype == torch.bfloat16 and a.numel() > 0 and w_down.numel() > 0
-          and all(n % 8 == 0 for n in (a.shape[-1], *w_down.shape)) and hasattr(_b.native, "gemm_bf16_gated") and _b.native.gemm_supported())
+          and all(n % 8 == 0 for n in (a.shape[-1], *w_down.shape)) and _b.native.gemm_supported())
     if not ok:
         gate, up = torch.nn.functional.linear(a, w_gate_up).chunk(2, -1)
         gate = torch.nn.functional.silu(gate) if act == "silu" else torch.nn.functional.gelu(gate, approximate="tanh")
         y = torch.nn.functional.linear(gate * up, w_down)
         return y if residual is None else y + residual
-    a2, wgu, wd = _aligned(a.reshape(-1, a.shape[-1])), _aligned(w_gate_up), _aligned(w_down)
-    res2 = None if residual is None else _aligned(residual.reshape(-1, shape[-1]))
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        return _GatedMlpFn.apply(a2, wgu, wd, _GATES[act], res2).view(shape)
-    return _b.native.gemm_bf16_nt(_b.native.gemm_bf16_gated(a2, wgu, _GATES[act], False)[0], wd, None, 0, None, res2).view(shape)
+    return _b.native.gated_mlp(a, w_gate_up, w_down, _GATES[act], residual)

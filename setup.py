@@ -16,7 +16,7 @@ CSRC = os.path.join("bluefog_b200", "csrc")
 
 
 def sources():
-    files = [os.path.join(CSRC, "bindings.cc")]
+    files = [os.path.join(CSRC, "bindings.cc"), os.path.join(CSRC, "block_ops.cc")]
     files += sorted(glob.glob(os.path.join(CSRC, "common", "*.cc")))
     files += sorted(glob.glob(os.path.join(CSRC, "cuda", "*.cc")))
     files += sorted(glob.glob(os.path.join(CSRC, "cuda", "*.cu")))

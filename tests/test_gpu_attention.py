@@ -64,7 +64,7 @@ def _inputs(tokens, h, hkv, d, seed=0):
 
 def _run(q, k, v, dout, **kw):
     from bluefog_b200.ops import fused_attention as fa
-    assert fa._eligible(q, k, v)
+    assert fa._eligible(q, q.shape[-1])
     leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
     out = fa.causal_attention(*leaves, **kw)
     return [out.detach(), *torch.autograd.grad(out, leaves, dout)]
@@ -153,7 +153,6 @@ def test_strided_and_unaligned_inputs():
     def columns(z):                                                   # last dimension not contiguous
         return z.transpose(-1, -2).contiguous().transpose(-1, -2)
 
-    assert fa._rows(gap(q)).data_ptr() != q.data_ptr()
     for change in (gap, heads_first, off, columns):
         for a, w in zip(_run(*(change(z) for z in (q, k, v, dout))), want):
             assert torch.equal(a, w), change.__name__
