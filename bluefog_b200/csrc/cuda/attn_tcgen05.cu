@@ -37,6 +37,21 @@ constexpr int kTile = 128;                       // rows of a query tile and of 
 constexpr uint32_t kBoxBytes = kTile * 128;      // 128 rows of 64 bf16 values, 128-byte swizzle
 constexpr float kLog2e = 1.4426950408889634f;
 
+// x / d for 0 <= x < 2^31 without a division (a 64-bit product; m = ceil(2^(31 + s) / d), 2^(s - 1) < d <= 2^s)
+struct Divisor {
+  unsigned int d, m;
+  int s;
+};
+Divisor MakeDivisor(int d) {
+  Divisor v{static_cast<unsigned int>(d), 0, 0};
+  while ((1ll << v.s) < d) ++v.s;
+  v.m = static_cast<unsigned int>(((1ull << (31 + v.s)) + d - 1) / d);
+  return v;
+}
+__device__ __forceinline__ int divide(int x, const Divisor& v) {
+  return int((static_cast<unsigned long long>(static_cast<unsigned int>(x)) * v.m) >> (31 + v.s));
+}
+
 struct Geo {
   const int* cu;
   int batch;
@@ -46,6 +61,7 @@ struct Geo {
   int heads;
   int group;            // query heads per key head
   int dim;
+  Divisor by_heads, by_kv_heads, by_batch, by_group;
 };
 
 struct Tile {
@@ -62,7 +78,7 @@ __device__ __forceinline__ int cu_at(const Geo& g, int b) { return b <= 0 ? 0 : 
 // Called by whole warps.  False when the slot holds no tile.
 __device__ __forceinline__ bool find_tile(const Geo& g, int order, bool late_first, Tile& t) {
   if (g.cu == nullptr) {
-    const int i = order / g.batch;
+    const int i = divide(order, g.by_batch);
     t.batch = order - i * g.batch;
     t.index = late_first ? g.tiles_per_seq - 1 - i : i;
     t.slot = t.batch * g.tiles_per_seq + t.index;
@@ -183,13 +199,15 @@ __device__ __forceinline__ void stage_rows(uint32_t taddr, float factor, unsigne
     }
   }
 }
-// Chunks [chunk0, chunk0 + chunks) of the warp's 32 staged rows to memory; consecutive lanes write consecutive 16 bytes.
+// Chunks [chunk0, chunk0 + CHUNKS) of the warp's 32 staged rows to memory; consecutive lanes write consecutive 16 bytes.
+template <int CHUNKS>
 __device__ __forceinline__ void store_rows(const AttnTensor& t, int head, int token0, int rows_left, int dim, const unsigned char* box,
-                                           int row0, int chunk0, int chunks) {
+                                           int row0, int chunk0) {
   const int lane = threadIdx.x & 31;
-  const int last = min(chunk0 + chunks, dim / 8) - chunk0;
-  for (int i = lane; i < 32 * chunks; i += 32) {
-    const int r = i / chunks, c = i - r * chunks;
+  const int last = min(chunk0 + CHUNKS, dim / 8) - chunk0;
+#pragma unroll
+  for (int k = 0; k < CHUNKS; ++k) {
+    const int r = (k * 32 + lane) / CHUNKS, c = (k * 32 + lane) % CHUNKS;
     if (r >= rows_left || c >= last) continue;
     const int row = row0 + r, chunk = chunk0 + c;
     const uint4 v = *reinterpret_cast<const uint4*>(box + size_t(chunk >> 3) * kBoxBytes + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
@@ -199,18 +217,21 @@ __device__ __forceinline__ void store_rows(const AttnTensor& t, int head, int to
 }
 
 // ---------------------------------------------------------------------------------------------------------------- //
-// Forward.  One CTA per query tile and head, two CTAs per SM: while the four softmax warps of one wait for a product, those
-// of the other keep the exponential unit busy.  Key tiles are taken from the diagonal downwards, so only the first one
-// needs a mask.  Tensor memory (256 of 512 columns per CTA): scores 128, output DP, and P in a place of its own where
-// there is room (DP = 64: the next scores are computed while this tile's exponentials are taken), over the scores
-// otherwise.  The output is rescaled only when a row's maximum grew by more than 2^8 (the sums stay far inside fp32).
+// Forward.  One CTA per query tile and head, two CTAs per SM: while the softmax warps of one wait for a product, those of
+// the other keep the exponential unit busy.  Eight softmax warps: two threads share a row, 64 columns each, and exchange
+// their maxima through shared memory (with one thread per row the 128 scores in its registers spilled and one warp per
+// scheduler and CTA could not hide the latency of its own exponentials: 12 cycles per element against the 8 that the unit
+// needs).  Key tiles are taken from the diagonal downwards, so only the first one needs a mask.  Tensor memory (256 of 512
+// columns per CTA): scores 128, output DP, and P in a place of its own where there is room (DP = 64: the next scores are
+// computed while this tile's exponentials are taken), over the scores otherwise.  The output is rescaled only when a row's
+// maximum grew by more than 2^8 (the sums stay far inside fp32).
 // ---------------------------------------------------------------------------------------------------------------- //
 template <int DP>
 struct FwdCfg {
   static constexpr int kBoxes = DP / 64;
   static constexpr int kSlots = DP == 64 ? 5 : 2;       // ring of key / value tiles
   static constexpr uint32_t kTileBytes = kBoxes * kBoxBytes;
-  static constexpr int kThreads = 192;
+  static constexpr int kThreads = 320;
   static constexpr uint32_t kColO = 128;
   static constexpr bool kOwnP = DP == 64;
   static constexpr uint32_t kColP = kOwnP ? 192 : 0;
@@ -228,6 +249,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   unsigned char* smem_q = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   unsigned char* ring = smem_q + Cfg::kTileBytes;
   __shared__ uint64_t bars[2 * NS + 6];
+  __shared__ float maxima[2][2][kTile];
   __shared__ uint32_t tmem_base_s;
   __shared__ int failed_s;
   volatile int* failed = &failed_s;
@@ -238,7 +260,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   auto empty = [&](int s) { return bar0 + 8u * (NS + s); };
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int order = blockIdx.x / g.heads;
+  const int order = divide(blockIdx.x, g.by_heads);
   const int head = blockIdx.x - order * g.heads;
   if (g.cu != nullptr && blockIdx.x == 0) {
     bool bad = false;
@@ -256,9 +278,9 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     return;
   }
   const int n = t.index + 1;                           // key tiles
-  const int kv_head = head / g.group;
+  const int kv_head = divide(head, g.by_group);
 
-  if (threadIdx.x == 0) {
+  if (warp == 8 && lane == 0) {
     failed_s = 0;
     for (int s = 0; s < NS; ++s) {
       mbar_init(full(s), 1);
@@ -266,14 +288,20 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     }
     mbar_init(bar_q, 1);
     mbar_init(bar_s, 1);
-    mbar_init(bar_sfree, 4);
-    mbar_init(bar_p, 4);
+    mbar_init(bar_sfree, 8);
+    mbar_init(bar_p, 8);
     mbar_init(bar_pv, 1);
     mbar_init(bar_end, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    // the first tiles travel while tensor memory is allocated
+    mbar_expect_tx(bar_q, Cfg::kTileBytes);
+    for (int b = 0; b < Cfg::kBoxes; ++b) tma_load_3d(smem_u32(smem_q) + b * kBoxBytes, &map_q, bar_q, b * 64, head, t.start + row0);
+    mbar_expect_tx(full(0), Cfg::kTileBytes);
+    for (int b = 0; b < Cfg::kBoxes; ++b)
+      tma_load_3d(smem_u32(ring) + b * kBoxBytes, &map_k, full(0), b * 64, kv_head, t.start + (n - 1) * kTile);
   }
-  if (warp == 5) {
+  if (warp == 9) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 256;" ::"r"(smem_u32(&tmem_base_s)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -282,12 +310,10 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   fence_after_sync();
   const uint32_t tmem = tmem_base_s;
 
-  if (warp == 4) {
+  if (warp == 8) {
     if (lane == 0) {
-      mbar_expect_tx(bar_q, Cfg::kTileBytes);
-      for (int b = 0; b < Cfg::kBoxes; ++b) tma_load_3d(smem_u32(smem_q) + b * kBoxBytes, &map_q, bar_q, b * 64, head, t.start + row0);
-      // in the order of use: K0 K1 V0 K2 V1 ... where scores run ahead, else K0 V0 K1 V1 ...
-      int armed = 0;
+      // in the order of use: K0 K1 V0 K2 V1 ... where scores run ahead, else K0 V0 K1 V1 ...; K0 is under way
+      int armed = 1;
       bool ok = true;
       auto load = [&](const CUtensorMap* map, int it) {
         const int s = armed % NS;
@@ -300,13 +326,12 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         return true;
       };
       if (Cfg::kOwnP) {
-        ok = load(&map_k, 0);
         for (int it = 0; it < n && ok; ++it) {
           if (it + 1 < n) ok = load(&map_k, it + 1);
           if (ok) ok = load(&map_v, it);
         }
       } else {
-        for (int it = 0; it < n && ok; ++it) ok = load(&map_k, it) && load(&map_v, it);
+        for (int it = 0; it < n && ok; ++it) ok = (it == 0 || load(&map_k, it)) && load(&map_v, it);
       }
       if (!ok || *failed) {
         // copies in flight have to land before this shared memory goes away
@@ -318,7 +343,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         while (!mbar_try(bar_q, 0) && clock64() - t0 < kWaitLimitCycles) {}
       }
     }
-  } else if (warp == 5) {
+  } else if (warp == 9) {
     // the whole warp walks along, lane 0 issues; `used` counts ring slots in the order of the loads
     int used = 0;
     bool ok = mbar_wait(bar_q, 0, failed);
@@ -369,25 +394,24 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       __syncwarp();
     }
   } else {
-    const int row = warp * 32 + lane;
-    const uint32_t lanes = uint32_t(warp * 32) << 16;
-    const uint32_t tS = tmem + lanes, tO = tmem + lanes + Cfg::kColO, tP = tmem + lanes + Cfg::kColP;
+    const int half = warp >> 2;                        // columns 64 half .. 64 half + 63
+    const int row = (warp & 3) * 32 + lane;
+    const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
+    const uint32_t tS = tmem + lanes + half * 64, tO = tmem + lanes + Cfg::kColO + half * (DP / 2), tP = tmem + lanes + Cfg::kColP + half * 32;
+    auto pair_sync = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 3)) : "memory"); };   // the two warps of 32 rows
     float m = 0.f, l = 0.f;
     bool ok = true;
     for (int it = 0; it < n; ++it) {
-      ok = mbar_wait(bar_s, it & 1, failed);
-      if (!ok) break;
+      // no way out of this loop: after a wait that failed the others fail at once, and the two warps of a pair meet in
+      // every iteration
+      ok = mbar_wait(bar_s, it & 1, failed) && ok;
       fence_after_sync();
-      uint32_t r[128];
+      uint32_t r[64];
       tmem_ld32(tS, r);
       tmem_ld32(tS + 32, r + 32);
-      tmem_ld32(tS + 64, r + 64);
-      tmem_ld32(tS + 96, r + 96);
       tmem_wait_ld();
       tie32(r);
       tie32(r + 32);
-      tie32(r + 64);
-      tie32(r + 96);
       if (Cfg::kOwnP) {
         fence_before_sync();
         __syncwarp();
@@ -395,77 +419,83 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       }
       if (it == 0) {
 #pragma unroll
-        for (int c = 0; c < 128; ++c)
-          if (c > row) r[c] = 0xff800000u;             // -inf
+        for (int c = 0; c < 64; ++c)
+          if (half * 64 + c > row) r[c] = 0xff800000u;             // -inf
       }
       float mx[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) mx[k] = max_nan(__uint_as_float(r[k]), __uint_as_float(r[k + 4]));
 #pragma unroll
-      for (int c = 8; c < 128; c += 8)
+      for (int c = 8; c < 64; c += 8)
 #pragma unroll
         for (int k = 0; k < 4; ++k) mx[k] = max3_nan(mx[k], __uint_as_float(r[c + k]), __uint_as_float(r[c + k + 4]));
-      const float top = max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3]));
+      float top = max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3]));
+      // two sets of cells in turn: a thread is at most one tile ahead of its partner
+      maxima[it & 1][half][row] = top;
+      pair_sync();
+      top = max_nan(top, maxima[it & 1][half ^ 1][row]);
       if (it == 0) {
         m = top;
       } else {
-        if (Cfg::kOwnP && !mbar_wait(bar_pv, (it - 1) & 1, failed)) { ok = false; break; }   // P is free, the output at rest
         const bool grown = !((top - m) * scale_log2 <= 8.f);
         if (__any_sync(0xffffffffu, grown)) {
-          // for P over the scores the product before these scores is complete already; a row that did not grow keeps its
-          // reference, so that its bits do not depend on what the warp's other rows hold
+          // rare; the product before has to be complete.  A row that did not grow keeps its reference, so that its bits do
+          // not depend on what the warp's other rows hold.
+          ok = mbar_wait(bar_pv, (it - 1) & 1, failed) && ok;
           const float next = grown ? max_nan(m, top) : m;
           const float f = ex2((m - (next == -INFINITY ? 0.f : next)) * scale_log2);
           m = next;
           l *= f;
           fence_after_sync();
-#pragma unroll
-          for (int c = 0; c < DP / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld32(tO + c * 32, o);
+#pragma unroll 1
+          for (int c = 0; c < DP / 2; c += 16) {
+            uint32_t o[16];
+            tmem_ld16(tO + c, o);
             tmem_wait_ld();
-            tie32(o);
+            tie16(o);
 #pragma unroll
-            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-            tmem_st32(tO + c * 32, o);
+            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+            tmem_st16(tO + c, o);
           }
         }
       }
       // a row whose scores are all -inf so far takes 0 as its reference: exp(-inf - 0) = 0 instead of NaN
       const float shift = m == -INFINITY ? 0.f : -m * scale_log2;
       float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      uint32_t p[32];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t p[32];
-#pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          const float a = ex2(fmaf(__uint_as_float(r[h * 64 + 2 * c]), scale_log2, shift));
-          const float b = ex2(fmaf(__uint_as_float(r[h * 64 + 2 * c + 1]), scale_log2, shift));
-          sum[(2 * c) & 3] += a;
-          sum[(2 * c + 1) & 3] += b;
-          p[c] = pack_bf16(a, b);
-        }
-        tmem_st32(tP + h * 32, p);
+      for (int c = 0; c < 32; ++c) {
+        const float a = ex2(fmaf(__uint_as_float(r[2 * c]), scale_log2, shift));
+        const float b = ex2(fmaf(__uint_as_float(r[2 * c + 1]), scale_log2, shift));
+        sum[(2 * c) & 3] += a;
+        sum[(2 * c + 1) & 3] += b;
+        p[c] = pack_bf16(a, b);
       }
+      if (Cfg::kOwnP && it > 0) ok = mbar_wait(bar_pv, (it - 1) & 1, failed) && ok;   // P has been read
+      tmem_st32(tP, p);
       l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
       tmem_wait_st();
       fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar_p);
     }
+    // the row's sum is in two places
+    maxima[n & 1][half][row] = l;
+    pair_sync();
+    l += maxima[n & 1][half ^ 1][row];
     if (ok && mbar_wait(bar_pv, (n - 1) & 1, failed)) {
       fence_after_sync();
-      stage_rows<DP / 32>(tO, 1.f / l, smem_q, row, 0);
+      stage_rows<DP / 64>(tO, 1.f / l, smem_q, row, half * (DP / 16));
       __syncwarp();
-      const int left = t.len - row0 - warp * 32;
-      store_rows(out, head, t.start + row0 + warp * 32, left, g.dim, smem_q, warp * 32, 0, DP / 8);
-      if (stats != nullptr)
+      const int left = t.len - row0 - (row & ~31);
+      store_rows<DP / 16>(out, head, t.start + row0 + (row & ~31), left, g.dim, smem_q, row & ~31, half * (DP / 16));
+      if (stats != nullptr && half == 0)
         stats[((long long)head * g.tiles + t.slot) * kTile + row] = lane < left ? fmaf(m, scale_log2, log2f(l)) : INFINITY;
     }
   }
   fence_before_sync();
   __syncthreads();
-  if (warp == 5) {
+  if (warp == 9) {
     fence_after_sync();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 256;" ::"r"(tmem) : "memory");
   }
@@ -476,7 +506,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
 // delta[head, row] = sum_d dout * out, one tile and head per block; rows that belong to no token get 0.
 // ---------------------------------------------------------------------------------------------------------------- //
 __global__ void __launch_bounds__(256) attn_delta_kernel(const Geo g, const AttnTensor out, const AttnTensor dout, float* __restrict__ delta) {
-  const int order = blockIdx.x / g.heads;
+  const int order = divide(blockIdx.x, g.by_heads);
   const int head = blockIdx.x - order * g.heads;
   Tile t;
   if (!find_tile(g, order, true, t) || (g.cu != nullptr && t.batch == g.batch)) return;
@@ -552,7 +582,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int own_heads = KV ? g.heads / g.group : g.heads;
-  const int order = blockIdx.x / own_heads;
+  const int order = divide(blockIdx.x, KV ? g.by_kv_heads : g.by_heads);
   const int own_head = blockIdx.x - order * own_heads;
   Tile t;
   if (!find_tile(g, order, !KV, t)) return;
@@ -613,7 +643,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         ok = mbar_wait(empty(s), ((it / NS) & 1) ^ 1, failed);
         if (!ok) break;
         const int j = other_tile(it);
-        const int head = KV ? own_head * g.group + it / per_head : own_head / g.group;
+        const int head = KV ? own_head * g.group + it / per_head : divide(own_head, g.by_group);
         const uint32_t dst = smem_u32(ring + size_t(s) * 2 * Cfg::kTileBytes);
         mbar_expect_tx(full(s), 2 * Cfg::kTileBytes + Cfg::kStatBytes);
         for (int b = 0; b < Cfg::kBoxes; ++b) {
@@ -799,11 +829,11 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         unsigned char* box = ring + size_t(half) * Cfg::kTileBytes;
         stage_rows<DP / 32>(tmem + lanes + (half ? Cfg::kCol1 : Cfg::kCol0), half ? scale : 1.f, box, row, 0);
         __syncwarp();
-        store_rows(half ? d1 : d0, own_head, token0, left, g.dim, box, row & ~31, 0, DP / 8);
+        store_rows<DP / 8>(half ? d1 : d0, own_head, token0, left, g.dim, box, row & ~31, 0);
       } else {
         stage_rows<DP / 64>(tmem + lanes + Cfg::kCol1 + half * (DP / 2), scale, ring, row, half * (DP / 16));
         __syncwarp();
-        store_rows(d1, own_head, token0, left, g.dim, ring, row & ~31, half * (DP / 16), DP / 16);
+        store_rows<DP / 16>(d1, own_head, token0, left, g.dim, ring, row & ~31, half * (DP / 16));
       }
     }
   }
@@ -840,6 +870,10 @@ Geo MakeGeo(const AttnShape& s) {
   g.heads = s.heads;
   g.group = s.heads / s.kv_heads;
   g.dim = s.dim;
+  g.by_heads = MakeDivisor(s.heads);
+  g.by_kv_heads = MakeDivisor(s.kv_heads);
+  g.by_batch = MakeDivisor(s.batch);
+  g.by_group = MakeDivisor(g.group);
   return g;
 }
 
