@@ -5,7 +5,7 @@
 //             dv = P^T dout (summed over the query heads of a group),  dk = scale dS^T q (ditto),  dq = scale dS k
 //
 // Every kernel works on tiles of 128 queries x 128 keys, one row of the score tile per thread, and never writes a score
-// to memory.  The backward pass is two kernels, one that owns a key tile (dk, dv) and one that owns a query tile (dq):
+// to memory.  The backward pass has two kinds of CTAs: those that own a key tile (dk, dv) and those that own a query tile (dq),
 // seven products per tile instead of five, but no atomics, so gradients do not depend on the order in which CTAs run, and
 // no fp32 copy of dq.
 //
@@ -58,7 +58,7 @@ struct Geo {
   int seq;              // tokens per sequence, or of all sequences together when cu is given
   int tiles_per_seq;    // without cu
   int tiles;
-  int heads;
+  int heads, kv_heads;
   int group;            // query heads per key head
   int dim;
   Divisor by_heads, by_kv_heads, by_batch, by_group;
@@ -128,39 +128,70 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   return y;
 }
 
+// two floats in one 64-bit register, and the packed instructions on them
+typedef unsigned long long float2_t;
+__device__ __forceinline__ float2_t pair(float lo, float hi) {
+  float2_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+  return v;
+}
+__device__ __forceinline__ void unpair(float2_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ float2_t fma2(float2_t a, float2_t b, float2_t c) {
+  float2_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ float2_t add2(float2_t a, float2_t b) {
+  float2_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float2_t mul2(float2_t a, float2_t b) {
+  float2_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
 // instruction descriptors: fp32 accumulator, bf16 operands, M = 128, N as given; B K-major or MN-major (bit 16)
 constexpr uint32_t idesc(int n, bool b_mn) {
   return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn ? 1u << 16 : 0u) | (uint32_t(n >> 3) << 17) | (uint32_t(kTile >> 4) << 24);
 }
 
-// scores[128 x 128] = A B^T over DP columns; A, B: DP / 64 boxes of [128 rows x 64 columns]
-template <int DP>
+// scores[128 x N] = A B^T over DP columns; A: DP / 64 boxes of [128 rows x 64 columns] in shared memory, or 128 rows of DP bf16
+// values in tensor memory; B: DP / 64 boxes of [N rows x 64 columns]
+template <int DP, int N>
 __device__ __forceinline__ void mma_scores(uint32_t tmem_d, uint32_t a, uint32_t b) {
   const uint64_t da = make_desc(a), db = make_desc(b);
 #pragma unroll
-  for (int k = 0; k < DP / 16; ++k) {
-    const uint64_t off = uint64_t(k >> 2) * (kBoxBytes >> 4) + uint64_t(k & 3) * 2;
-    umma_f16(tmem_d, da + off, db + off, idesc(kTile, false), k != 0 ? 1u : 0u);
-  }
+  for (int k = 0; k < DP / 16; ++k)
+    umma_f16(tmem_d, da + uint64_t(k >> 2) * (kBoxBytes >> 4) + uint64_t(k & 3) * 2, db + uint64_t(k >> 2) * (N * 128 >> 4) + uint64_t(k & 3) * 2,
+             idesc(N, false), k != 0 ? 1u : 0u);
 }
-// acc[128 x DP] += A B: A 128 x 128 bf16 in tensor memory (K elements 0-63 at `a`, 64-127 at `a` + a_half columns), B =
-// DP / 64 boxes of [128 K-rows x 64 columns], read as an MN-major operand
-template <int DP>
-__device__ __forceinline__ void mma_accumulate(uint32_t tmem_d, uint32_t a, uint32_t a_half, uint32_t b, bool first) {
-  const uint64_t db = make_desc_mn(b, kBoxBytes, 1024);
+template <int DP, int N>
+__device__ __forceinline__ void mma_scores_ts(uint32_t tmem_d, uint32_t tmem_a, uint32_t b) {
+  const uint64_t db = make_desc(b);
 #pragma unroll
-  for (int k = 0; k < kTile / 16; ++k)
-    umma_f16_ts(tmem_d, a + uint32_t(k >> 2) * a_half + uint32_t(k & 3) * 8, db + uint64_t(k) * (2048 >> 4), idesc(DP, true),
+  for (int k = 0; k < DP / 16; ++k)
+    umma_f16_ts(tmem_d, tmem_a + k * 8, db + uint64_t(k >> 2) * (N * 128 >> 4) + uint64_t(k & 3) * 2, idesc(N, false), k != 0 ? 1u : 0u);
+}
+// acc[128 x DP] += A B: A 128 x K bf16 in tensor memory, 32 elements (16 columns) every `a_step` columns; B = DP / 64 boxes of
+// [K rows x 64 columns], read as an MN-major operand
+template <int DP, int K>
+__device__ __forceinline__ void mma_accumulate(uint32_t tmem_d, uint32_t a, uint32_t a_step, uint32_t b, bool first) {
+  const uint64_t db = make_desc_mn(b, K * 128, 1024);
+#pragma unroll
+  for (int k = 0; k < K / 16; ++k)
+    umma_f16_ts(tmem_d, a + uint32_t(k >> 1) * a_step + uint32_t(k & 1) * 8, db + uint64_t(k) * (2048 >> 4), idesc(DP, true),
                 (first && k == 0) ? 0u : 1u);
 }
 
-// Zeros in rows [first, 128) of DP / 64 boxes; called by a whole warp, visible to the tensor cores afterwards.
-template <int DP>
+// Zeros in rows [first, N) of DP / 64 boxes of N rows; called by a whole warp, visible to the tensor cores afterwards.
+template <int DP, int N>
 __device__ __forceinline__ void zero_rows(unsigned char* boxes, int first) {
   const int lane = threadIdx.x & 31;
   const uint4 z = make_uint4(0u, 0u, 0u, 0u);
   for (int b = 0; b < DP / 64; ++b)
-    for (int c = first * 8 + lane; c < kTile * 8; c += 32) *reinterpret_cast<uint4*>(boxes + size_t(b) * kBoxBytes + size_t(c) * 16) = z;
+    for (int c = first * 8 + lane; c < N * 8; c += 32) *reinterpret_cast<uint4*>(boxes + size_t(b) * (N * 128) + size_t(c) * 16) = z;
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   __syncwarp();
 }
@@ -351,8 +382,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       const int s = used % NS;
       if (!mbar_wait(full(s), (used / NS) & 1, failed)) return false;
       ++used;
-      if (lane == 0) {
-        mma_scores<DP>(tmem, smem_u32(smem_q), smem_u32(ring + size_t(s) * Cfg::kTileBytes));
+      if (elect_one()) {
+        mma_scores<DP, kTile>(tmem, smem_u32(smem_q), smem_u32(ring + size_t(s) * Cfg::kTileBytes));
         umma_commit(empty(s));
         umma_commit(bar_s);
       }
@@ -373,12 +404,12 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       ++used;
       unsigned char* v = ring + size_t(s) * Cfg::kTileBytes;
       // P is zero behind the end of the sequence, which is not enough when the rows there hold infinities or NaN
-      if (it == 0 && t.len - row0 < kTile) zero_rows<DP>(v, t.len - row0);
+      if (it == 0 && t.len - row0 < kTile) zero_rows<DP, kTile>(v, t.len - row0);
       ok = mbar_wait(bar_p, it & 1, failed);
       if (!ok) break;
       fence_after_sync();
-      if (lane == 0) {
-        mma_accumulate<DP>(tmem + Cfg::kColO, tmem + Cfg::kColP, 32, smem_u32(v), it == 0);
+      if (elect_one()) {
+        mma_accumulate<DP, kTile>(tmem + Cfg::kColO, tmem + Cfg::kColP, 16, smem_u32(v), it == 0);
         umma_commit(empty(s));
         umma_commit(bar_pv);
       }
@@ -386,7 +417,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       if (!Cfg::kOwnP && it + 1 < n) ok = scores();    // over P: products run in the order of issue
     }
     if (!ok || *failed) {
-      if (lane == 0) {
+      if (elect_one()) {
         umma_commit(bar_end);                          // tensor memory is not freed under a product
         const long long t0 = clock64();
         while (!mbar_try(bar_end, 0) && clock64() - t0 < kWaitLimitCycles) {}
@@ -490,7 +521,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       const int left = t.len - row0 - (row & ~31);
       store_rows<DP / 16>(out, head, t.start + row0 + (row & ~31), left, g.dim, smem_q, row & ~31, half * (DP / 16));
       if (stats != nullptr && half == 0)
-        stats[((long long)head * g.tiles + t.slot) * kTile + row] = lane < left ? fmaf(m, scale_log2, log2f(l)) : INFINITY;
+        stats[((long long)head * g.tiles + t.slot) * kTile + row] = lane < left ? -fmaf(m, scale_log2, log2f(l)) : -INFINITY;
     }
   }
   fence_before_sync();
@@ -503,125 +534,149 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
 }
 
 // ---------------------------------------------------------------------------------------------------------------- //
-// delta[head, row] = sum_d dout * out, one tile and head per block; rows that belong to no token get 0.
+// delta[head, row] = - sum_d dout * out, one tile and head per block; rows that belong to no token get 0.  LANES threads per row,
+// eight values each.
 // ---------------------------------------------------------------------------------------------------------------- //
+template <int LANES>
 __global__ void __launch_bounds__(256) attn_delta_kernel(const Geo g, const AttnTensor out, const AttnTensor dout, float* __restrict__ delta) {
   const int order = divide(blockIdx.x, g.by_heads);
   const int head = blockIdx.x - order * g.heads;
   Tile t;
   if (!find_tile(g, order, true, t) || (g.cu != nullptr && t.batch == g.batch)) return;
-  const int sub = threadIdx.x & 15;                    // sixteen threads per row, eight values each
-  for (int r = threadIdx.x >> 4; r < kTile; r += 16) {
-    float s = 0.f;
-    const int row = t.index * kTile + r;
+  constexpr int kRows = 256 / LANES, kSteps = kTile / kRows;
+  const int sub = threadIdx.x % LANES, r0 = threadIdx.x / LANES;
+  uint4 a[kSteps], b[kSteps];
+#pragma unroll
+  for (int k = 0; k < kSteps; ++k) {
+    const int row = t.index * kTile + r0 + k * kRows;
+    a[k] = b[k] = make_uint4(0u, 0u, 0u, 0u);
     if (row < t.len && sub * 8 < g.dim) {
       const long long tok = t.start + row;
-      const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(out.ptr) + tok * out.token_stride +
-                                                      (long long)head * out.head_stride + sub * 8);
-      const uint4 b = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(dout.ptr) + tok * dout.token_stride +
-                                                      (long long)head * dout.head_stride + sub * 8);
-      const __nv_bfloat162* x = reinterpret_cast<const __nv_bfloat162*>(&a);
-      const __nv_bfloat162* y = reinterpret_cast<const __nv_bfloat162*>(&b);
+      a[k] = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(out.ptr) + tok * out.token_stride + (long long)head * out.head_stride + sub * 8);
+      b[k] = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(dout.ptr) + tok * dout.token_stride + (long long)head * dout.head_stride + sub * 8);
+    }
+  }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 u = __bfloat1622float2(x[i]), v = __bfloat1622float2(y[i]);
-        s = fmaf(u.x, v.x, fmaf(u.y, v.y, s));
-      }
+  for (int k = 0; k < kSteps; ++k) {
+    const __nv_bfloat162* x = reinterpret_cast<const __nv_bfloat162*>(&a[k]);
+    const __nv_bfloat162* y = reinterpret_cast<const __nv_bfloat162*>(&b[k]);
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 u = __bfloat1622float2(x[i]), v = __bfloat1622float2(y[i]);
+      s = fmaf(u.x, v.x, fmaf(u.y, v.y, s));
     }
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (sub == 0) delta[((long long)head * g.tiles + t.slot) * kTile + r] = s;
+    for (int o = LANES / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (sub == 0) delta[((long long)head * g.tiles + t.slot) * kTile + r0 + k * kRows] = -s;
   }
 }
 
 // ---------------------------------------------------------------------------------------------------------------- //
-// Backward.  KV: a CTA owns a key tile of one key head and walks over the query tiles at and after it, for every query
-// head of the group; scores are held transposed (rows = keys), so P^T and dS^T are the tensor-memory operands of
-// dv += P^T dout and dk += dS^T q, and the row statistics are per column.  Otherwise a CTA owns a query tile of one head
-// and walks over the key tiles from the diagonal downwards: dq += dS k.  One CTA per SM; eight warps take the
-// exponentials, two per quarter of tensor memory, each with one half of the columns.
-// Tensor memory: scores (two buffers where 512 columns allow it, so that the next scores are ready when a tile's work
-// ends), dP, accumulators.  The bf16 operands replace the fp32 values they come from: elements 0-63 at the start of the
-// region, 64-127 at its middle, so each half of the warps writes where it alone has read.
+// Backward.  KV: a CTA owns a tile of 128 keys of one key head and walks over the queries at and after it, 64 at a time, for every
+// query head of the group; scores are held transposed (rows = keys), so P^T and dS^T are the tensor-memory operands of
+// dv += P^T dout and dk += dS^T q, and the row statistics are per column.  Otherwise a CTA owns a tile of 128 queries of one
+// head and walks over the keys from the diagonal downwards, 64 at a time: dq += dS k.  Both kinds are blocks of one launch.
+// What limits this is the chain products -> exponentials -> products of one tile, so two chains run side by side on an SM: two CTAs
+// of 256 tensor-memory columns for DP = 64, two sets of eight warps with score buffers of their own in one CTA for DP = 128
+// (with 128 columns at a time and one chain the layer of GPT-2 medium took 93 + 71 us, 3100 and 2270 cycles per 128 x 128 tile,
+// against the 1024 that its exponentials need).  Eight warps take one 128 x 64 tile, two per quarter of tensor memory with 32
+// columns each.  Their bf16 operands replace the fp32 values that the same warp has read.  Products with 64 columns whose first
+// operand comes from shared memory are bound by the reads of that operand (48 cycles instead of 32 per 16 elements), so the
+// query kind keeps q and dout in tensor memory; the key kind has no room for that.
 // ---------------------------------------------------------------------------------------------------------------- //
-template <int DP, bool KV>
+template <int DP>
 struct BwdCfg {
   static constexpr int kBoxes = DP / 64;
-  static constexpr uint32_t kTileBytes = kBoxes * kBoxBytes;
-  static constexpr int kStages = DP == 64 ? 4 : 2;
-  static constexpr bool kTwoScores = !(KV && DP == 128);
-  static constexpr int kThreads = 320;
-  static constexpr uint32_t kColDP = 128, kColS1 = 256;
-  static constexpr uint32_t kCol1 = 512 - DP, kCol0 = kCol1 - DP;      // accumulators of dk / dq and of dv
-  static constexpr uint32_t kStatBytes = KV ? 2 * kTile * 4 : 0;
-  static constexpr size_t kSmem = 1024 + 2 * size_t(kTileBytes) + size_t(kStages) * (2 * kTileBytes + kStatBytes);
+  static constexpr int kN = 64;                                        // rows of a streamed tile
+  static constexpr uint32_t kXBytes = kBoxes * kBoxBytes;              // each of the two resident tiles
+  static constexpr uint32_t kYBytes = kBoxes * kN * 128;               // each of the two streamed tiles of a stage
+  static constexpr int kStages = 4;
+  static constexpr int kSets = DP == 64 ? 1 : 2;
+  static constexpr int kWarps = 8 * kSets;                             // those that take exponentials
+  static constexpr int kThreads = 32 * (kWarps + 2);
+  static constexpr int kCtasPerSm = DP == 64 ? 2 : 1;
+  static constexpr uint32_t kCols = DP == 64 ? 256 : 512;
+  static constexpr uint32_t kCol1 = kCols - DP, kCol0 = kCol1 - DP;    // accumulators of dk / dq and of dv
+  static constexpr uint32_t kColX = 128 * kSets;                       // queries: q and dout as operands, DP / 2 columns each
+  static constexpr size_t kSmem = 1024 + 2 * size_t(kXBytes) + size_t(kStages) * (2 * kYBytes + 2 * kN * 4);
 };
 
 template <int DP, bool KV>
-__global__ void __launch_bounds__((BwdCfg<DP, KV>::kThreads), 1)
-attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do, const Geo g,
-                const float* __restrict__ stats, const float* __restrict__ delta, const AttnTensor d0, const AttnTensor d1,
-                const float scale, const float scale_log2, unsigned int* __restrict__ status) {
-  using Cfg = BwdCfg<DP, KV>;
-  constexpr int NS = Cfg::kStages;
-  constexpr bool kTwo = Cfg::kTwoScores;
+__device__ __forceinline__ void attn_bwd_body(const CUtensorMap* map_q, const CUtensorMap* map_k, const CUtensorMap* map_v, const CUtensorMap* map_do,
+                                              const Geo& g, const int block, const int split, const float* __restrict__ stats, const float* __restrict__ delta,
+                                              const AttnTensor& d0, const AttnTensor& d1, const float scale, const float scale_log2,
+                                              unsigned int* __restrict__ status) {
+  using Cfg = BwdCfg<DP>;
+  constexpr int NS = Cfg::kStages, SETS = Cfg::kSets, N = Cfg::kN;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem_x = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  unsigned char* ring = smem_x + 2 * Cfg::kTileBytes;
-  float* ring_stats = reinterpret_cast<float*>(ring + size_t(NS) * 2 * Cfg::kTileBytes);      // KV: per stage lse[128], delta[128]
-  __shared__ uint64_t bars[2 * NS + 10];
+  unsigned char* ring = smem_x + 2 * Cfg::kXBytes;
+  float* ring_stats = reinterpret_cast<float*>(ring + size_t(NS) * 2 * Cfg::kYBytes);      // KV: per stage -lse[64], -delta[64]
+  __shared__ uint64_t bars[2 * NS + 3 + 3 * SETS];
   __shared__ uint32_t tmem_base_s;
   __shared__ int failed_s;
   volatile int* failed = &failed_s;
   const uint32_t bar0 = smem_u32(bars);
-  const uint32_t bar_x = bar0 + 8u * (2 * NS), bar_s = bar_x + 8u /* two */, bar_dp = bar_x + 24u, bar_dpfree = bar_x + 32u,
-                 bar_p = bar_x + 40u /* two */, bar_ds = bar_x + 56u /* two */, bar_end = bar_x + 72u;
+  const uint32_t bar_x = bar0 + 8u * (2 * NS), bar_xa = bar_x + 8u, bar_end = bar_x + 16u;
   auto full = [&](int s) { return bar0 + 8u * s; };
   auto empty = [&](int s) { return bar0 + 8u * (NS + s); };
+  auto bar_s = [&](int set) { return bar_x + 24u + 24u * set; };
+  auto bar_dp = [&](int set) { return bar_x + 32u + 24u * set; };
+  auto bar_ds = [&](int set) { return bar_x + 40u + 24u * set; };
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int own_heads = KV ? g.heads / g.group : g.heads;
-  const int order = divide(blockIdx.x, KV ? g.by_kv_heads : g.by_heads);
-  const int own_head = blockIdx.x - order * own_heads;
+  // KV: `split` CTAs of a cluster (a power of two) share a tile, each with its part of the group's query heads
+  const int part_of_group = KV ? block & (split - 1) : 0;
+  const int item = KV ? block >> (__ffs(split) - 1) : block;
+  const int own_heads = KV ? g.kv_heads : g.heads;
+  const int order = divide(item, KV ? g.by_kv_heads : g.by_heads);
+  const int own_head = item - order * own_heads;
+  const int first_head = KV ? own_head * g.group + part_of_group * (g.group >> (__ffs(split) - 1)) : divide(own_head, g.by_group);
   Tile t;
   if (!find_tile(g, order, !KV, t)) return;
   const int row0 = t.index * kTile;
   if (g.cu != nullptr && t.batch == g.batch) {
+    if (part_of_group != 0) return;
     if (KV) zero_result(d0, own_head, t.start + row0, t.start + t.len, g.dim);
     zero_result(d1, own_head, t.start + row0, t.start + t.len, g.dim);
     return;
   }
-  const int seq_tiles = (t.len + kTile - 1) / kTile;
-  const int per_head = KV ? seq_tiles - t.index : t.index + 1;
-  const int n = KV ? per_head * g.group : per_head;
+  const int seq_parts = (t.len + N - 1) / N;           // streamed tiles of the sequence
+  const int first_part = KV ? 2 * t.index : min(2 * t.index + 1, seq_parts - 1);
+  const int per_head = KV ? seq_parts - first_part : first_part + 1;
+  const int n = KV ? per_head * (g.group >> (__ffs(split) - 1)) : per_head;
   const int first_slot = t.slot - t.index;
-  // tile of the other side (query tile for KV, key tile otherwise) in iteration `it`
-  auto other_tile = [&](int it) { return KV ? t.index + it % per_head : t.index - it; };
 
-  if (threadIdx.x == 0) {
+  if (warp == Cfg::kWarps && lane == 0) {
     failed_s = 0;
     for (int s = 0; s < NS; ++s) {
       mbar_init(full(s), 1);
       mbar_init(empty(s), 1);
     }
     mbar_init(bar_x, 1);
-    mbar_init(bar_s, 1);
-    mbar_init(bar_s + 8u, 1);
-    mbar_init(bar_dp, 1);
-    mbar_init(bar_dpfree, 8);
-    // two each, for even and odd iterations: a warp may be one iteration ahead of another, and its arrival must not
-    // count for the other's
-    for (int k = 0; k < 2; ++k) {
-      mbar_init(bar_p + 8u * k, 8);
-      mbar_init(bar_ds + 8u * k, 8);
-    }
+    mbar_init(bar_xa, 8);
     mbar_init(bar_end, 1);
+    for (int k = 0; k < SETS; ++k) {
+      mbar_init(bar_s(k), 1);
+      mbar_init(bar_dp(k), 1);
+      mbar_init(bar_ds(k), 8);
+    }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    // the resident tiles travel while tensor memory is allocated; every box holds 64 rows
+    mbar_expect_tx(bar_x, 2 * Cfg::kXBytes);
+    const CUtensorMap* m0 = KV ? map_k : map_q;
+    const CUtensorMap* m1 = KV ? map_v : map_do;
+    for (int b = 0; b < Cfg::kBoxes; ++b)
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t dst = smem_u32(smem_x) + b * kBoxBytes + h * (kBoxBytes / 2);
+        tma_load_3d(dst, m0, bar_x, b * 64, own_head, t.start + row0 + h * 64);
+        tma_load_3d(dst + Cfg::kXBytes, m1, bar_x, b * 64, own_head, t.start + row0 + h * 64);
+      }
   }
-  if (warp == 9) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_base_s)) : "memory");
+  if (warp == Cfg::kWarps + 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)), "r"(Cfg::kCols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   fence_before_sync();
@@ -629,35 +684,35 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   fence_after_sync();
   const uint32_t tmem = tmem_base_s;
 
-  if (warp == 8) {
+  if (warp == Cfg::kWarps) {
     if (lane == 0) {
-      mbar_expect_tx(bar_x, 2 * Cfg::kTileBytes);
-      for (int b = 0; b < Cfg::kBoxes; ++b) {
-        tma_load_3d(smem_u32(smem_x) + b * kBoxBytes, KV ? &map_k : &map_q, bar_x, b * 64, own_head, t.start + row0);
-        tma_load_3d(smem_u32(smem_x) + Cfg::kTileBytes + b * kBoxBytes, KV ? &map_v : &map_do, bar_x, b * 64, own_head, t.start + row0);
-      }
-      int armed = 0;
+      int armed = 0, part = first_part, head = first_head;
       bool ok = true;
       for (int it = 0; it < n; ++it) {
         const int s = it % NS;
         ok = mbar_wait(empty(s), ((it / NS) & 1) ^ 1, failed);
         if (!ok) break;
-        const int j = other_tile(it);
-        const int head = KV ? own_head * g.group + it / per_head : divide(own_head, g.by_group);
-        const uint32_t dst = smem_u32(ring + size_t(s) * 2 * Cfg::kTileBytes);
-        mbar_expect_tx(full(s), 2 * Cfg::kTileBytes + Cfg::kStatBytes);
+        const uint32_t dst = smem_u32(ring + size_t(s) * 2 * Cfg::kYBytes);
+        mbar_expect_tx(full(s), 2 * Cfg::kYBytes + (KV ? 2 * N * 4 : 0));
         for (int b = 0; b < Cfg::kBoxes; ++b) {
-          tma_load_3d(dst + b * kBoxBytes, KV ? &map_q : &map_k, full(s), b * 64, head, t.start + j * kTile);
-          tma_load_3d(dst + Cfg::kTileBytes + b * kBoxBytes, KV ? &map_do : &map_v, full(s), b * 64, head, t.start + j * kTile);
+          tma_load_3d(dst + b * (N * 128), KV ? map_q : map_k, full(s), b * 64, head, t.start + part * N);
+          tma_load_3d(dst + Cfg::kYBytes + b * (N * 128), KV ? map_do : map_v, full(s), b * 64, head, t.start + part * N);
         }
         if (KV) {
-          const long long at = ((long long)head * g.tiles + first_slot + j) * kTile;
-          bulk_load(smem_u32(ring_stats + s * 2 * kTile), stats + at, full(s), kTile * 4);
-          bulk_load(smem_u32(ring_stats + s * 2 * kTile + kTile), delta + at, full(s), kTile * 4);
+          const long long at = ((long long)head * g.tiles + first_slot) * kTile + part * N;
+          bulk_load(smem_u32(ring_stats + s * 2 * N), stats + at, full(s), N * 4);
+          bulk_load(smem_u32(ring_stats + s * 2 * N + N), delta + at, full(s), N * 4);
+          if (++part == seq_parts) {
+            part = first_part;
+            ++head;
+          }
+        } else {
+          --part;
         }
         armed = it + 1;
       }
       if (!ok || *failed) {
+        // copies in flight have to land before this shared memory goes away
         for (int f = armed > NS ? armed - NS : 0; f < armed; ++f) {
           const long long t0 = clock64();
           while (!mbar_try(full(f % NS), (f / NS) & 1) && clock64() - t0 < kWaitLimitCycles) {}
@@ -666,192 +721,260 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         while (!mbar_try(bar_x, 0) && clock64() - t0 < kWaitLimitCycles) {}
       }
     }
-  } else if (warp == 9) {
-    const uint32_t x0 = smem_u32(smem_x), x1 = x0 + Cfg::kTileBytes;
-    auto stage = [&](int it) { return ring + size_t(it % NS) * 2 * Cfg::kTileBytes; };
-    auto s_col = [&](int it) { return tmem + ((kTwo && (it & 1)) ? Cfg::kColS1 : 0u); };
-    bool ok = mbar_wait(bar_x, 0, failed);
-    // waits for the tiles of an iteration and issues its scores
-    auto scores = [&](int it) {
+  } else if (warp == Cfg::kWarps + 1) {
+    const uint32_t x0 = smem_u32(smem_x), x1 = x0 + Cfg::kXBytes;
+    auto stage = [&](int it) { return ring + size_t(it % NS) * 2 * Cfg::kYBytes; };
+    auto s_col = [&](int it) { return tmem + uint32_t(it % SETS) * 128u; };
+    bool ok = mbar_wait(KV ? bar_x : bar_xa, 0, failed);
+    fence_after_sync();
+    int part = first_part;
+    // waits for the tiles of an iteration and issues its scores and dP, over the operands of the set's tile before: products
+    // run in the order of issue
+    auto products = [&](int it) {
       if (!mbar_wait(full(it % NS), (it / NS) & 1, failed)) return false;
-      const int j = other_tile(it);
-      if (t.len - j * kTile < kTile) {                 // rows behind the end of the sequence take part in the reductions
-        zero_rows<DP>(stage(it), t.len - j * kTile);
-        zero_rows<DP>(stage(it) + Cfg::kTileBytes, t.len - j * kTile);
+      if (t.len - part * N < N) {                      // rows behind the end of the sequence take part in the reductions
+        zero_rows<DP, N>(stage(it), t.len - part * N);
+        zero_rows<DP, N>(stage(it) + Cfg::kYBytes, t.len - part * N);
       }
-      if (lane == 0) {
-        mma_scores<DP>(s_col(it), x0, smem_u32(stage(it)));
-        umma_commit(bar_s + (kTwo ? 8u * (it & 1) : 0u));
+      if (KV) {
+        if (++part == seq_parts) part = first_part;
+      } else {
+        --part;
+      }
+      if (elect_one()) {
+        const uint32_t y = smem_u32(stage(it));
+        if (KV) mma_scores<DP, N>(s_col(it), x0, y);
+        else mma_scores_ts<DP, N>(s_col(it), tmem + Cfg::kColX, y);
+        umma_commit(bar_s(it % SETS));
+        if (KV) mma_scores<DP, N>(s_col(it) + N, x1, y + Cfg::kYBytes);
+        else mma_scores_ts<DP, N>(s_col(it) + N, tmem + Cfg::kColX + DP / 2, y + Cfg::kYBytes);
+        umma_commit(bar_dp(it % SETS));
       }
       __syncwarp();
       return true;
     };
-    auto grad_scores = [&](int it) {
-      if (lane == 0) {
-        mma_scores<DP>(tmem + Cfg::kColDP, x1, smem_u32(stage(it)) + Cfg::kTileBytes);
-        umma_commit(bar_dp);
-      }
-      __syncwarp();
-    };
-    ok = ok && scores(0);
-    if (ok) grad_scores(0);
+    for (int it = 0; it < SETS && it < n; ++it) ok = ok && products(it);
     for (int it = 0; it < n && ok; ++it) {
-      const bool more = it + 1 < n;
-      if (kTwo && more) {
-        // the other score buffer: its operand was read by a product issued before these
-        ok = scores(it + 1);
-        if (!ok) break;
-      }
-      if (KV) {
-        ok = mbar_wait(bar_p + 8u * (it & 1), (it >> 1) & 1, failed);
-        if (!ok) break;
-        fence_after_sync();
-        if (lane == 0) mma_accumulate<DP>(tmem + Cfg::kCol0, s_col(it), 64, smem_u32(stage(it)) + Cfg::kTileBytes, it == 0);
-        __syncwarp();
-        if (!kTwo && more) {
-          ok = scores(it + 1);                         // over P: products run in the order of issue
-          if (!ok) break;
-        }
-      } else if (more) {
-        ok = mbar_wait(bar_dpfree, it & 1, failed);
-        if (!ok) break;
-        fence_after_sync();
-        grad_scores(it + 1);
-      }
-      ok = mbar_wait(bar_ds + 8u * (it & 1), (it >> 1) & 1, failed);
+      ok = mbar_wait(bar_ds(it % SETS), (it / SETS) & 1, failed);
       if (!ok) break;
       fence_after_sync();
-      if (lane == 0) {
-        mma_accumulate<DP>(tmem + Cfg::kCol1, KV ? tmem + Cfg::kColDP : s_col(it), 64, smem_u32(stage(it)), it == 0);
+      if (elect_one()) {
+        const uint32_t y = smem_u32(stage(it));
+        if (KV) mma_accumulate<DP, N>(tmem + Cfg::kCol0, s_col(it), 32, y + Cfg::kYBytes, it == 0);
+        mma_accumulate<DP, N>(tmem + Cfg::kCol1, s_col(it) + N, 32, y, it == 0);
         umma_commit(empty(it % NS));
       }
       __syncwarp();
-      if (KV && more) grad_scores(it + 1);             // over dS
+      if (it + SETS < n) ok = products(it + SETS);
     }
-    if (lane == 0) {
+    if (elect_one()) {
       umma_commit(bar_end);
-      if (!ok || *failed) {
+      if (!ok || *failed) {                            // tensor memory is not freed under a product
         const long long t0 = clock64();
         while (!mbar_try(bar_end, 0) && clock64() - t0 < kWaitLimitCycles) {}
       }
     }
     __syncwarp();
   } else {
-    const int half = warp >> 2;
+    const int set = warp >> 3, half = (warp >> 2) & 1;
     const int row = (warp & 3) * 32 + lane;
     const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
     float lse = 0.f, dlt = 0.f;
+    bool ok = true;
     if (!KV) {
       const long long at = ((long long)own_head * g.tiles + t.slot) * kTile + row;
       lse = stats[at];
       dlt = delta[at];
-    }
-    bool ok = true;
-    for (int it = 0; it < n; ++it) {
-      const bool diagonal = other_tile(it) == t.index;
-      const float* st = ring_stats + (it % NS) * 2 * kTile + half * 64;
-      const uint32_t tS = tmem + lanes + ((kTwo && (it & 1)) ? Cfg::kColS1 : 0u) + half * 64;
-      const uint32_t tD = tmem + lanes + Cfg::kColDP + half * 64;
-      ok = kTwo ? mbar_wait(bar_s + 8u * (it & 1), (it >> 1) & 1, failed) : mbar_wait(bar_s, it & 1, failed);
-      if (!ok) break;
-      if (KV) {
-        // the statistics came with the tiles of this stage: acquire their barrier too
-        ok = mbar_wait(full(it % NS), (it / NS) & 1, failed);
-        if (!ok) break;
-      }
-      fence_after_sync();
-      uint32_t r[64];
-      tmem_ld32(tS, r);
-      tmem_ld32(tS + 32, r + 32);
-      tmem_wait_ld();
-      tie32(r);
-      tie32(r + 32);
-      float p[64];
+      if (set == 0) {
+        // q (first half of the warps) or dout (second) from shared to tensor memory, a row per thread
+        ok = mbar_wait(bar_x, 0, failed);
 #pragma unroll
-      for (int c = 0; c < 64; c += 4) {
-        float4 s4 = make_float4(lse, lse, lse, lse);
-        if (KV) s4 = *reinterpret_cast<const float4*>(st + c);
-        p[c + 0] = ex2(fmaf(__uint_as_float(r[c + 0]), scale_log2, -s4.x));
-        p[c + 1] = ex2(fmaf(__uint_as_float(r[c + 1]), scale_log2, -s4.y));
-        p[c + 2] = ex2(fmaf(__uint_as_float(r[c + 2]), scale_log2, -s4.z));
-        p[c + 3] = ex2(fmaf(__uint_as_float(r[c + 3]), scale_log2, -s4.w));
-      }
-      if (diagonal) {
+        for (int b = 0; b < Cfg::kBoxes; ++b) {
+          uint32_t r[32];
 #pragma unroll
-        for (int c = 0; c < 64; ++c) {
-          const int col = half * 64 + c;
-          if (KV ? col < row : col > row) p[c] = 0.f;
+          for (int c = 0; c < 8; ++c) {
+            const uint4 v = *reinterpret_cast<const uint4*>(smem_x + half * Cfg::kXBytes + b * kBoxBytes + row * 128 + ((c ^ (row & 7)) << 4));
+            r[c * 4] = v.x;
+            r[c * 4 + 1] = v.y;
+            r[c * 4 + 2] = v.z;
+            r[c * 4 + 3] = v.w;
+          }
+          tmem_st32(tmem + lanes + Cfg::kColX + half * (DP / 2) + b * 32, r);
         }
-      }
-      if (KV) {
-        uint32_t pk[32];
-#pragma unroll
-        for (int c = 0; c < 32; ++c) pk[c] = pack_bf16(p[2 * c], p[2 * c + 1]);
-        tmem_st32(tS, pk);
         tmem_wait_st();
         fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar_p + 8u * (it & 1));
+        if (lane == 0) mbar_arrive(bar_xa);
       }
-      ok = mbar_wait(bar_dp, it & 1, failed);
+    }
+    const float2_t scale2 = pair(scale_log2, scale_log2), lse2 = pair(lse, lse), dlt2 = pair(dlt, dlt);
+    const uint32_t tS = tmem + lanes + set * 128u + half * 32u, tD = tS + N;
+    int part = 0;                                      // streamed tile, counted from the first one of a head
+    for (int it = set; it < n; it += SETS) {
+      if (it == set) part = set;
+      else part += SETS;
+      while (part >= per_head) part -= per_head;
+      // columns from here on belong to rows of the tile (KV: queries at and after the first key), so a mask is needed
+      const bool diagonal = KV ? part < 2 : it < first_part - 2 * t.index + 1;
+      const float* st = ring_stats + (it % NS) * 2 * N + half * 32;
+      const uint32_t phase = (it / SETS) & 1;
+      ok = ok && mbar_wait(bar_s(set), phase, failed);
+      if (KV) ok = ok && mbar_wait(full(it % NS), (it / NS) & 1, failed);       // the statistics came with the tiles
+      if (!ok) break;
+      fence_after_sync();
+      uint32_t r[32];
+      tmem_ld32(tS, r);
+      tmem_wait_ld();
+      tie32(r);
+      float p[32];
+#pragma unroll
+      for (int c = 0; c < 32; c += 4) {
+        float2_t a = lse2, b = lse2;
+        if (KV) {
+          const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(st + c);
+          a = v.x;
+          b = v.y;
+        }
+        unpair(fma2(pair(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), scale2, a), p[c], p[c + 1]);
+        unpair(fma2(pair(__uint_as_float(r[c + 2]), __uint_as_float(r[c + 3])), scale2, b), p[c + 2], p[c + 3]);
+      }
+#pragma unroll
+      for (int c = 0; c < 32; ++c) p[c] = ex2(p[c]);
+      if (diagonal) {
+        const int col0 = half * 32 + (KV ? part * N : (first_part - it - 2 * t.index) * N);
+#pragma unroll
+        for (int c = 0; c < 32; ++c)
+          if (KV ? col0 + c < row : col0 + c > row) p[c] = 0.f;
+      }
+      uint32_t pk[16];
+      if (KV) {
+#pragma unroll
+        for (int c = 0; c < 16; ++c) pk[c] = pack_bf16(p[2 * c], p[2 * c + 1]);
+        tmem_st16(tS, pk);
+      }
+      ok = mbar_wait(bar_dp(set), phase, failed);
       if (!ok) break;
       fence_after_sync();
       tmem_ld32(tD, r);
-      tmem_ld32(tD + 32, r + 32);
       tmem_wait_ld();
       tie32(r);
-      tie32(r + 32);
-      if (!KV) {
-        fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar_dpfree);
-      }
-      uint32_t pk[32];
 #pragma unroll
-      for (int c = 0; c < 64; c += 4) {
-        float4 d4 = make_float4(dlt, dlt, dlt, dlt);
-        if (KV) d4 = *reinterpret_cast<const float4*>(st + kTile + c);
-        pk[c / 2] = pack_bf16(p[c] * (__uint_as_float(r[c]) - d4.x), p[c + 1] * (__uint_as_float(r[c + 1]) - d4.y));
-        pk[c / 2 + 1] = pack_bf16(p[c + 2] * (__uint_as_float(r[c + 2]) - d4.z), p[c + 3] * (__uint_as_float(r[c + 3]) - d4.w));
+      for (int c = 0; c < 32; c += 4) {
+        float2_t a = dlt2, b = dlt2;
+        if (KV) {
+          const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(st + N + c);
+          a = v.x;
+          b = v.y;
+        }
+        float x, y;
+        unpair(mul2(pair(p[c], p[c + 1]), add2(pair(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), a)), x, y);
+        pk[c / 2] = pack_bf16(x, y);
+        unpair(mul2(pair(p[c + 2], p[c + 3]), add2(pair(__uint_as_float(r[c + 2]), __uint_as_float(r[c + 3])), b)), x, y);
+        pk[c / 2 + 1] = pack_bf16(x, y);
       }
-      tmem_st32(KV ? tD : tS, pk);
+      tmem_st16(tD, pk);
       tmem_wait_st();
       fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar_ds + 8u * (it & 1));
+      if (lane == 0) mbar_arrive(bar_ds(set));
     }
     if (ok && mbar_wait(bar_end, 0, failed) && !*failed) {
       fence_after_sync();
       // the ring is at rest: staging boxes for the results
-      const int left = t.len - row0 - (warp & 3) * 32;
-      const int token0 = t.start + row0 + (warp & 3) * 32;
-      if (KV) {
-        unsigned char* box = ring + size_t(half) * Cfg::kTileBytes;
-        stage_rows<DP / 32>(tmem + lanes + (half ? Cfg::kCol1 : Cfg::kCol0), half ? scale : 1.f, box, row, 0);
+      const int left = t.len - row0 - (row & ~31);
+      const int token0 = t.start + row0 + (row & ~31);
+      if (KV && split > 1) {
+        // fp32 sums of this CTA's query heads for the cluster: rows of DP values, 16-byte chunks swizzled within 128 bytes
+        const bool second = SETS == 1 ? half == 1 : set == 1;
+        const int col = SETS == 1 ? 0 : half * 64;
+        unsigned char* sums = ring + (second ? kTile * DP * 4 : 0) + row * (DP * 4);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t r[32];
+          tmem_ld32(tmem + lanes + (second ? Cfg::kCol1 : Cfg::kCol0) + col + c * 32, r);
+          tmem_wait_ld();
+          tie32(r);
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            *reinterpret_cast<uint4*>(sums + (col / 32 + c) * 128 + ((j ^ (row & 7)) << 4)) = make_uint4(r[j * 4], r[j * 4 + 1], r[j * 4 + 2], r[j * 4 + 3]);
+        }
+      } else if (KV) {
+        // dv by the first half of the warps, dk by the second; 64 columns per thread
+        const bool second = SETS == 1 ? half == 1 : set == 1;
+        const int col = SETS == 1 ? 0 : half * 64;
+        unsigned char* box = ring + (second ? Cfg::kXBytes : 0);
+        stage_rows<2>(tmem + lanes + (second ? Cfg::kCol1 : Cfg::kCol0) + col, second ? scale : 1.f, box, row, col / 8);
         __syncwarp();
-        store_rows<DP / 8>(half ? d1 : d0, own_head, token0, left, g.dim, box, row & ~31, 0);
+        store_rows<8>(second ? d1 : d0, own_head, token0, left, g.dim, box, row & ~31, col / 8);
       } else {
-        stage_rows<DP / 64>(tmem + lanes + Cfg::kCol1 + half * (DP / 2), scale, ring, row, half * (DP / 16));
+        const int col = (set * 2 + half) * 32;
+        stage_rows<1>(tmem + lanes + Cfg::kCol1 + col, scale, ring, row, col / 8);
         __syncwarp();
-        store_rows<DP / 16>(d1, own_head, token0, left, g.dim, ring, row & ~31, half * (DP / 16));
+        store_rows<4>(d1, own_head, token0, left, g.dim, ring, row & ~31, col / 8);
       }
     }
   }
+  if (KV && split > 1) {
+    // every CTA of the cluster adds up 128 / split rows of all of them, in the order of the heads
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (warp < Cfg::kWarps) {
+      const int rows = kTile >> (__ffs(split) - 1);
+      for (int i = threadIdx.x; i < 2 * rows * (DP / 8); i += 32 * Cfg::kWarps) {
+        const int chunk = i & (DP / 8 - 1), rest = i / (DP / 8);
+        const bool second = rest >= rows;
+        const int row = part_of_group * rows + (second ? rest - rows : rest);
+        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        const uint32_t at = smem_u32(ring) + (second ? kTile * DP * 4 : 0) + row * (DP * 4) + (chunk >> 2) * 128;
+        for (int c = 0; c < split; ++c) {
+          const float4 a = ld_cluster_v4(mapa_u32(at + ((((chunk & 3) * 2) ^ (row & 7)) << 4), c));
+          const float4 b = ld_cluster_v4(mapa_u32(at + ((((chunk & 3) * 2 + 1) ^ (row & 7)) << 4), c));
+          v[0] += a.x, v[1] += a.y, v[2] += a.z, v[3] += a.w;
+          v[4] += b.x, v[5] += b.y, v[6] += b.z, v[7] += b.w;
+        }
+        if (row0 + row < t.len && chunk * 8 < g.dim) {
+          const float f = second ? scale : 1.f;
+          const AttnTensor& d = second ? d1 : d0;
+          const uint4 out = make_uint4(pack_bf16(v[0] * f, v[1] * f), pack_bf16(v[2] * f, v[3] * f), pack_bf16(v[4] * f, v[5] * f), pack_bf16(v[6] * f, v[7] * f));
+          *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(d.ptr) + (long long)(t.start + row0 + row) * d.token_stride +
+                                    (long long)own_head * d.head_stride + chunk * 8) = out;
+        }
+      }
+    }
+    // nobody leaves while another may still read its shared memory
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
   fence_before_sync();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == Cfg::kWarps + 1) {
     fence_after_sync();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Cfg::kCols) : "memory");
   }
   if (threadIdx.x == 0 && failed_s) atomicOr(status, kAttnTimeout);
 }
 
+// The first kv_blocks blocks own key tiles (`split` of a cluster share one), the others query tiles.
+template <int DP>
+__global__ void __launch_bounds__(BwdCfg<DP>::kThreads, BwdCfg<DP>::kCtasPerSm)
+attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do, const Geo g, const int kv_blocks, const int split,
+                const float* __restrict__ stats, const float* __restrict__ delta, const AttnTensor dq, const AttnTensor dk,
+                const AttnTensor dv, const float scale, const float scale_log2, unsigned int* __restrict__ status) {
+  if (int(blockIdx.x) < kv_blocks)
+    attn_bwd_body<DP, true>(&map_q, &map_k, &map_v, &map_do, g, blockIdx.x, split, stats, delta, dv, dk, scale, scale_log2, status);
+  else
+    attn_bwd_body<DP, false>(&map_q, &map_k, &map_v, &map_do, g, blockIdx.x - kv_blocks, 1, stats, delta, dq, dq, scale, scale_log2, status);
+}
+
 // ---- host side ---------------------------------------------------------------------------------------------------
 
-bool MakeMap(CUtensorMap* map, const AttnTensor& t, int heads, int dim, long long tokens) {
+bool MakeMap(CUtensorMap* map, const AttnTensor& t, int heads, int dim, long long tokens, int rows) {
   const cuuint64_t dims[3] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(tokens)};
   const cuuint64_t strides[2] = {static_cast<cuuint64_t>(t.head_stride) * 2, static_cast<cuuint64_t>(t.token_stride) * 2};
-  const cuuint32_t box[3] = {64, 1, kTile};
+  const cuuint32_t box[3] = {64, 1, static_cast<cuuint32_t>(rows)};
   return EncodeTiled(map, 3, t.ptr, dims, strides, box);
 }
 
@@ -868,6 +991,7 @@ Geo MakeGeo(const AttnShape& s) {
   g.tiles_per_seq = static_cast<int>((s.seq + kTile - 1) / kTile);
   g.tiles = static_cast<int>(AttnTiles(s));
   g.heads = s.heads;
+  g.kv_heads = s.kv_heads;
   g.group = s.heads / s.kv_heads;
   g.dim = s.dim;
   g.by_heads = MakeDivisor(s.heads);
@@ -904,18 +1028,45 @@ cudaError_t Forward(const AttnShape& s, const CUtensorMap& mq, const CUtensorMap
   return cudaGetLastError();
 }
 
-template <int DP, bool KV>
+template <int DP>
 cudaError_t Backward(const AttnShape& s, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& md,
-                     const float* stats, const float* delta, const AttnTensor& d0, const AttnTensor& d1, unsigned int* status,
-                     cudaStream_t stream) {
-  constexpr auto kernel = attn_bwd_kernel<DP, KV>;
-  using Cfg = BwdCfg<DP, KV>;
+                     const float* stats, const float* delta, const AttnTensor& dq, const AttnTensor& dk, const AttnTensor& dv,
+                     unsigned int* status, cudaStream_t stream) {
+  constexpr auto kernel = attn_bwd_kernel<DP>;
+  using Cfg = BwdCfg<DP>;
   const cudaError_t e = AllowSmem<kernel>(Cfg::kSmem);
   if (e != cudaSuccess) return e;
   const Geo g = MakeGeo(s);
-  kernel<<<static_cast<unsigned>(g.tiles) * (KV ? s.kv_heads : s.heads), Cfg::kThreads, Cfg::kSmem, stream>>>(
-      mq, mk, mv, md, g, stats, delta, d0, d1, s.scale, s.scale * kLog2e, status);
+  // The query heads of a group add to the same key tile.  Up to eight CTAs of a cluster (the portable size) share them and add up
+  // their sums through distributed shared memory: without it one CTA walked over all of them, and few key heads left SMs idle
+  // (packed documents, four query heads to a key head: 380 against 330 us, forward included).  The query kind then has a
+  // launch of its own, since blocks that need no cluster would still be started as one.
+  int split = 1;
+  while (split < 8 && g.group % (2 * split) == 0) split *= 2;
+  const int kv_blocks = g.tiles * s.kv_heads * split, q_blocks = g.tiles * s.heads;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(split > 1 ? kv_blocks : kv_blocks + q_blocks));
+  cfg.blockDim = dim3(Cfg::kThreads);
+  cfg.dynamicSmemBytes = Cfg::kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = split;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = split > 1 ? 1 : 0;
+  const float scale_log2 = s.scale * kLog2e;
+  cudaError_t r = cudaLaunchKernelEx(&cfg, kernel, mq, mk, mv, md, g, kv_blocks, split, stats, delta, dq, dk, dv, s.scale, scale_log2, status);
+  if (r != cudaSuccess) return r;
   CountKernelLaunch();
+  if (split > 1) {
+    cfg.gridDim = dim3(static_cast<unsigned>(q_blocks));
+    cfg.numAttrs = 0;
+    r = cudaLaunchKernelEx(&cfg, kernel, mq, mk, mv, md, g, 0, 1, stats, delta, dq, dk, dv, s.scale, scale_log2, status);
+    if (r != cudaSuccess) return r;
+    CountKernelLaunch();
+  }
   return cudaGetLastError();
 }
 
@@ -929,7 +1080,7 @@ bool AttnSupported(const AttnShape& s) {
   const long long tokens = s.cu == nullptr ? s.batch * s.seq : s.seq;
   return GetEncodeFn() != nullptr && s.batch > 0 && s.seq > 0 && s.heads > 0 && s.kv_heads > 0 && s.heads % s.kv_heads == 0 &&
          s.dim >= 8 && s.dim <= 128 && s.dim % 8 == 0 && s.scale > 0.f && tokens < (1ll << 31) - 2 * kTile &&
-         AttnTiles(s) * s.heads < (1ll << 31);
+         AttnTiles(s) * s.heads * 2 < (1ll << 31);
 }
 
 cudaError_t LaunchAttnForward(const AttnShape& s, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v,
@@ -939,8 +1090,8 @@ cudaError_t LaunchAttnForward(const AttnShape& s, const AttnTensor& q, const Att
     return cudaErrorInvalidValue;
   const long long tokens = s.cu == nullptr ? s.batch * s.seq : s.seq;
   CUtensorMap mq, mk, mv;
-  if (!MakeMap(&mq, q, s.heads, s.dim, tokens) || !MakeMap(&mk, k, s.kv_heads, s.dim, tokens) ||
-      !MakeMap(&mv, v, s.kv_heads, s.dim, tokens))
+  if (!MakeMap(&mq, q, s.heads, s.dim, tokens, kTile) || !MakeMap(&mk, k, s.kv_heads, s.dim, tokens, kTile) ||
+      !MakeMap(&mv, v, s.kv_heads, s.dim, tokens, kTile))
     return cudaErrorInvalidValue;
   return s.dim <= 64 ? Forward<64>(s, mq, mk, mv, out, stats, status, stream) : Forward<128>(s, mq, mk, mv, out, stats, status, stream);
 }
@@ -956,19 +1107,18 @@ cudaError_t LaunchAttnBackward(const AttnShape& s, const AttnTensor& q, const At
   if (!AttnSupported(s) || stats == nullptr || delta == nullptr || status == nullptr) return cudaErrorInvalidValue;
   const long long tokens = s.cu == nullptr ? s.batch * s.seq : s.seq;
   CUtensorMap mq, mk, mv, md;
-  if (!MakeMap(&mq, q, s.heads, s.dim, tokens) || !MakeMap(&mk, k, s.kv_heads, s.dim, tokens) ||
-      !MakeMap(&mv, v, s.kv_heads, s.dim, tokens) || !MakeMap(&md, dout, s.heads, s.dim, tokens))
+  if (!MakeMap(&mq, q, s.heads, s.dim, tokens, 64) || !MakeMap(&mk, k, s.kv_heads, s.dim, tokens, 64) ||
+      !MakeMap(&mv, v, s.kv_heads, s.dim, tokens, 64) || !MakeMap(&md, dout, s.heads, s.dim, tokens, 64))
     return cudaErrorInvalidValue;
   const Geo g = MakeGeo(s);
-  attn_delta_kernel<<<static_cast<unsigned>(g.tiles) * g.heads, 256, 0, stream>>>(g, out, dout, delta);
+  const unsigned blocks = static_cast<unsigned>(g.tiles) * g.heads;
+  if (s.dim <= 64) attn_delta_kernel<8><<<blocks, 256, 0, stream>>>(g, out, dout, delta);
+  else attn_delta_kernel<16><<<blocks, 256, 0, stream>>>(g, out, dout, delta);
   CountKernelLaunch();
-  cudaError_t e = cudaGetLastError();
+  const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  e = s.dim <= 64 ? Backward<64, true>(s, mq, mk, mv, md, stats, delta, dv, dk, status, stream)
-                  : Backward<128, true>(s, mq, mk, mv, md, stats, delta, dv, dk, status, stream);
-  if (e != cudaSuccess) return e;
-  return s.dim <= 64 ? Backward<64, false>(s, mq, mk, mv, md, stats, delta, dq, dq, status, stream)
-                     : Backward<128, false>(s, mq, mk, mv, md, stats, delta, dq, dq, status, stream);
+  return s.dim <= 64 ? Backward<64>(s, mq, mk, mv, md, stats, delta, dq, dk, dv, status, stream)
+                     : Backward<128>(s, mq, mk, mv, md, stats, delta, dq, dk, dv, status, stream);
 }
 
 }  // namespace bfb

@@ -33,8 +33,8 @@ enum AttnStatus : unsigned int { kAttnTimeout = 1u, kAttnBadSequences = 2u };
 long long AttnTiles(const AttnShape& s);
 bool AttnSupported(const AttnShape& s);
 
-// out = softmax(scale q k^T, causal within each sequence) v.  stats (optional, heads * AttnTiles * 128 floats): base-2
-// logarithm of the row sums of exp, for the backward pass; +inf in rows that belong to no token.
+// out = softmax(scale q k^T, causal within each sequence) v.  stats (optional, heads * AttnTiles * 128 floats): minus
+// the base-2 logarithm of the row sums of exp, for the backward pass; -inf in rows that belong to no token.
 cudaError_t LaunchAttnForward(const AttnShape& s, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v,
                               const AttnTensor& out, float* stats, unsigned int* status, cudaStream_t stream);
 

@@ -181,6 +181,15 @@ __device__ __forceinline__ void tie32(uint32_t* r) {
   asm volatile("" : "+r"(r[30]), "+r"(r[31]));
 }
 
+// One lane of a converged warp, the same one at every call.  The compiler knows that one lane alone runs what this guards, so the
+// descriptors of a tcgen05.mma stay in uniform registers; behind `lane == 0` every MMA first moves them there, which limits
+// the issue to one MMA in 61 cycles (measured: 128 x 64 x 16 out of shared memory 48 cycles with this, 32 with A in tensor memory).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
 // tcgen05.mma whose A operand lies in tensor memory: lane = row, one 32-bit column holds two consecutive K elements
 __device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
                                             uint32_t accumulate) {
