@@ -581,7 +581,7 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const Geo g, const Attn
 // of 256 tensor-memory columns for DP = 64, two sets of eight warps with score buffers of their own in one CTA for DP = 128
 // (with 128 columns at a time and one chain the layer of GPT-2 medium took 93 + 71 us, 3100 and 2270 cycles per 128 x 128 tile,
 // against the 1024 that its exponentials need).  Eight warps take one 128 x 64 tile, two per quarter of tensor memory with 32
-// columns each.  Their bf16 operands replace the fp32 values that the same warp has read.  Products with 64 columns whose first
+// columns of it.  Their bf16 operands replace the fp32 values that the same warp has read.  Products with 64 columns whose first
 // operand comes from shared memory are bound by the reads of that operand (48 cycles instead of 32 per 16 elements), so the
 // query kind keeps q and dout in tensor memory; the key kind has no room for that.
 // ---------------------------------------------------------------------------------------------------------------- //
@@ -648,6 +648,29 @@ __device__ __forceinline__ void attn_bwd_body(const CUtensorMap* map_q, const CU
   const int n = KV ? per_head * (g.group >> (__ffs(split) - 1)) : per_head;
   const int first_slot = t.slot - t.index;
 
+  // the producer's place: tiles loaded so far, the next one and its head
+  int armed = 0, next_part = first_part, next_head = first_head;
+  auto load = [&] {
+    const int s = armed % NS;
+    const uint32_t dst = smem_u32(ring + size_t(s) * 2 * Cfg::kYBytes);
+    mbar_expect_tx(full(s), 2 * Cfg::kYBytes + (KV ? 2 * N * 4 : 0));
+    for (int b = 0; b < Cfg::kBoxes; ++b) {
+      tma_load_3d(dst + b * (N * 128), KV ? map_q : map_k, full(s), b * 64, next_head, t.start + next_part * N);
+      tma_load_3d(dst + Cfg::kYBytes + b * (N * 128), KV ? map_do : map_v, full(s), b * 64, next_head, t.start + next_part * N);
+    }
+    if (KV) {
+      const long long at = ((long long)next_head * g.tiles + first_slot) * kTile + next_part * N;
+      bulk_load(smem_u32(ring_stats + s * 2 * N), stats + at, full(s), N * 4);
+      bulk_load(smem_u32(ring_stats + s * 2 * N + N), delta + at, full(s), N * 4);
+      if (++next_part == seq_parts) {
+        next_part = first_part;
+        ++next_head;
+      }
+    } else {
+      --next_part;
+    }
+    ++armed;
+  };
   if (warp == Cfg::kWarps && lane == 0) {
     failed_s = 0;
     for (int s = 0; s < NS; ++s) {
@@ -664,7 +687,7 @@ __device__ __forceinline__ void attn_bwd_body(const CUtensorMap* map_q, const CU
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    // the resident tiles travel while tensor memory is allocated; every box holds 64 rows
+    // the resident tiles and the first streamed ones travel while tensor memory is allocated; every box holds 64 rows
     mbar_expect_tx(bar_x, 2 * Cfg::kXBytes);
     const CUtensorMap* m0 = KV ? map_k : map_q;
     const CUtensorMap* m1 = KV ? map_v : map_do;
@@ -674,6 +697,7 @@ __device__ __forceinline__ void attn_bwd_body(const CUtensorMap* map_q, const CU
         tma_load_3d(dst, m0, bar_x, b * 64, own_head, t.start + row0 + h * 64);
         tma_load_3d(dst + Cfg::kXBytes, m1, bar_x, b * 64, own_head, t.start + row0 + h * 64);
       }
+    for (int it = 0; it < NS && it < n; ++it) load();
   }
   if (warp == Cfg::kWarps + 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)), "r"(Cfg::kCols) : "memory");
@@ -686,30 +710,11 @@ __device__ __forceinline__ void attn_bwd_body(const CUtensorMap* map_q, const CU
 
   if (warp == Cfg::kWarps) {
     if (lane == 0) {
-      int armed = 0, part = first_part, head = first_head;
       bool ok = true;
-      for (int it = 0; it < n; ++it) {
-        const int s = it % NS;
-        ok = mbar_wait(empty(s), ((it / NS) & 1) ^ 1, failed);
+      while (armed < n) {
+        ok = mbar_wait(empty(armed % NS), ((armed / NS) & 1) ^ 1, failed);
         if (!ok) break;
-        const uint32_t dst = smem_u32(ring + size_t(s) * 2 * Cfg::kYBytes);
-        mbar_expect_tx(full(s), 2 * Cfg::kYBytes + (KV ? 2 * N * 4 : 0));
-        for (int b = 0; b < Cfg::kBoxes; ++b) {
-          tma_load_3d(dst + b * (N * 128), KV ? map_q : map_k, full(s), b * 64, head, t.start + part * N);
-          tma_load_3d(dst + Cfg::kYBytes + b * (N * 128), KV ? map_do : map_v, full(s), b * 64, head, t.start + part * N);
-        }
-        if (KV) {
-          const long long at = ((long long)head * g.tiles + first_slot) * kTile + part * N;
-          bulk_load(smem_u32(ring_stats + s * 2 * N), stats + at, full(s), N * 4);
-          bulk_load(smem_u32(ring_stats + s * 2 * N + N), delta + at, full(s), N * 4);
-          if (++part == seq_parts) {
-            part = first_part;
-            ++head;
-          }
-        } else {
-          --part;
-        }
-        armed = it + 1;
+        load();
       }
       if (!ok || *failed) {
         // copies in flight have to land before this shared memory goes away
@@ -779,12 +784,18 @@ __device__ __forceinline__ void attn_bwd_body(const CUtensorMap* map_q, const CU
     const int set = warp >> 3, half = (warp >> 2) & 1;
     const int row = (warp & 3) * 32 + lane;
     const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
-    float lse = 0.f, dlt = 0.f;
     bool ok = true;
+    // A thread holds eight columns of four rows: with a row per thread every thread would read the statistics of all its columns,
+    // and the shared memory that the products read from was what the exponentials of the key kind waited for.
+    const int sub_row = (warp & 3) * 32 + (lane >> 2), sub_col = half * 32 + (lane & 3) * 2;
+    float2_t lse2[4], dlt2[4];                         // KV: column pairs 8 g + sub_col; otherwise rows sub_row + 8 k, twice
     if (!KV) {
-      const long long at = ((long long)own_head * g.tiles + t.slot) * kTile + row;
-      lse = stats[at];
-      dlt = delta[at];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const long long at = ((long long)own_head * g.tiles + t.slot) * kTile + sub_row + 8 * k;
+        lse2[k] = pair(stats[at], stats[at]);
+        dlt2[k] = pair(delta[at], delta[at]);
+      }
       if (set == 0) {
         // q (first half of the warps) or dout (second) from shared to tensor memory, a row per thread
         ok = mbar_wait(bar_x, 0, failed);
@@ -807,8 +818,8 @@ __device__ __forceinline__ void attn_bwd_body(const CUtensorMap* map_q, const CU
         if (lane == 0) mbar_arrive(bar_xa);
       }
     }
-    const float2_t scale2 = pair(scale_log2, scale_log2), lse2 = pair(lse, lse), dlt2 = pair(dlt, dlt);
-    const uint32_t tS = tmem + lanes + set * 128u + half * 32u, tD = tS + N;
+    const float2_t scale2 = pair(scale_log2, scale_log2);
+    const uint32_t tS = tmem + lanes + set * 128u + half * 32u, tD = tS + N, kUpper = 16u << 16;
     int part = 0;                                      // streamed tile, counted from the first one of a head
     for (int it = set; it < n; it += SETS) {
       if (it == set) part = set;
@@ -816,63 +827,63 @@ __device__ __forceinline__ void attn_bwd_body(const CUtensorMap* map_q, const CU
       while (part >= per_head) part -= per_head;
       // columns from here on belong to rows of the tile (KV: queries at and after the first key), so a mask is needed
       const bool diagonal = KV ? part < 2 : it < first_part - 2 * t.index + 1;
-      const float* st = ring_stats + (it % NS) * 2 * N + half * 32;
       const uint32_t phase = (it / SETS) & 1;
+      if (KV) {
+        const float* st = ring_stats + (it % NS) * 2 * N + sub_col;
+        ok = ok && mbar_wait(full(it % NS), (it / NS) & 1, failed);
+        if (!ok) break;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          lse2[k] = *reinterpret_cast<const float2_t*>(st + 8 * k);
+          dlt2[k] = *reinterpret_cast<const float2_t*>(st + N + 8 * k);
+        }
+      }
       ok = ok && mbar_wait(bar_s(set), phase, failed);
-      if (KV) ok = ok && mbar_wait(full(it % NS), (it / NS) & 1, failed);       // the statistics came with the tiles
       if (!ok) break;
       fence_after_sync();
-      uint32_t r[32];
-      tmem_ld32(tS, r);
+      uint32_t r[32];                                  // 16 u + 4 g + 2 b + e: row sub_row + 16 u + 8 b, column sub_col + 8 g + e
+      tmem_ld_16x256b_x4(tS, r);
+      tmem_ld_16x256b_x4(tS + kUpper, r + 16);
       tmem_wait_ld();
       tie32(r);
       float p[32];
 #pragma unroll
-      for (int c = 0; c < 32; c += 4) {
-        float2_t a = lse2, b = lse2;
-        if (KV) {
-          const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(st + c);
-          a = v.x;
-          b = v.y;
-        }
-        unpair(fma2(pair(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), scale2, a), p[c], p[c + 1]);
-        unpair(fma2(pair(__uint_as_float(r[c + 2]), __uint_as_float(r[c + 3])), scale2, b), p[c + 2], p[c + 3]);
-      }
+      for (int i = 0; i < 32; i += 2)
+        unpair(fma2(pair(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), scale2, lse2[KV ? (i >> 2) & 3 : i >> 4 << 1 | ((i >> 1) & 1)]),
+               p[i], p[i + 1]);
 #pragma unroll
-      for (int c = 0; c < 32; ++c) p[c] = ex2(p[c]);
+      for (int i = 0; i < 32; ++i) p[i] = ex2(p[i]);
       if (diagonal) {
-        const int col0 = half * 32 + (KV ? part * N : (first_part - it - 2 * t.index) * N);
+        const int over = sub_col + (KV ? part * N : (first_part - it - 2 * t.index) * N) - sub_row;
 #pragma unroll
-        for (int c = 0; c < 32; ++c)
-          if (KV ? col0 + c < row : col0 + c > row) p[c] = 0.f;
+        for (int i = 0; i < 32; ++i) {
+          const int d = over + ((i >> 2) & 3) * 8 + (i & 1) - (i >> 4) * 16 - ((i >> 1) & 1) * 8;       // column - row
+          if (KV ? d < 0 : d > 0) p[i] = 0.f;
+        }
       }
       uint32_t pk[16];
       if (KV) {
 #pragma unroll
-        for (int c = 0; c < 16; ++c) pk[c] = pack_bf16(p[2 * c], p[2 * c + 1]);
-        tmem_st16(tS, pk);
+        for (int i = 0; i < 16; ++i) pk[i] = pack_bf16(p[2 * i], p[2 * i + 1]);
+        tmem_st_16x128b_x4(tS, pk);
+        tmem_st_16x128b_x4(tS + kUpper, pk + 8);
       }
       ok = mbar_wait(bar_dp(set), phase, failed);
       if (!ok) break;
       fence_after_sync();
-      tmem_ld32(tD, r);
+      tmem_ld_16x256b_x4(tD, r);
+      tmem_ld_16x256b_x4(tD + kUpper, r + 16);
       tmem_wait_ld();
       tie32(r);
 #pragma unroll
-      for (int c = 0; c < 32; c += 4) {
-        float2_t a = dlt2, b = dlt2;
-        if (KV) {
-          const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(st + N + c);
-          a = v.x;
-          b = v.y;
-        }
+      for (int i = 0; i < 32; i += 2) {
         float x, y;
-        unpair(mul2(pair(p[c], p[c + 1]), add2(pair(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), a)), x, y);
-        pk[c / 2] = pack_bf16(x, y);
-        unpair(mul2(pair(p[c + 2], p[c + 3]), add2(pair(__uint_as_float(r[c + 2]), __uint_as_float(r[c + 3])), b)), x, y);
-        pk[c / 2 + 1] = pack_bf16(x, y);
+        unpair(mul2(pair(p[i], p[i + 1]), add2(pair(__uint_as_float(r[i]), __uint_as_float(r[i + 1])),
+                                               dlt2[KV ? (i >> 2) & 3 : i >> 4 << 1 | ((i >> 1) & 1)])), x, y);
+        pk[i / 2] = pack_bf16(x, y);
       }
-      tmem_st16(tD, pk);
+      tmem_st_16x128b_x4(tD, pk);
+      tmem_st_16x128b_x4(tD + kUpper, pk + 8);
       tmem_wait_st();
       fence_before_sync();
       __syncwarp();
