@@ -602,6 +602,39 @@ struct BwdCfg {
   static constexpr size_t kSmem = 1024 + 2 * size_t(kXBytes) + size_t(kStages) * (2 * kYBytes + 2 * kN * 4);
 };
 
+// dv and dk of a key tile from the fp32 sums of the SPLIT CTAs of the cluster ([2][128][DP] at `sums` in each, 16-byte chunks swizzled
+// within 128 bytes): this CTA's 128 / SPLIT rows, the CTAs in the order of their heads.  All loads of a chunk are in flight
+// together, since each takes about a microsecond.
+template <int DP, int SPLIT>
+__device__ __forceinline__ void add_up(const uint32_t sums, const int rank, const int head, const int token0, const int rows_left, const int dim,
+                                       const float scale, const AttnTensor& dv, const AttnTensor& dk, const int threads) {
+  constexpr int kRows = kTile / SPLIT, kChunks = DP / 8;
+  for (int i = threadIdx.x; i < 2 * kRows * kChunks; i += threads) {
+    const int chunk = i % kChunks, rest = i / kChunks;
+    const bool second = rest >= kRows;
+    const int row = rank * kRows + rest % kRows;
+    const uint32_t at = sums + (second ? kTile * DP * 4 : 0) + row * (DP * 4) + (chunk >> 2) * 128;
+    const uint32_t lo = at + ((((chunk & 3) * 2) ^ (row & 7)) << 4), hi = at + ((((chunk & 3) * 2 + 1) ^ (row & 7)) << 4);
+    float4 a[SPLIT], b[SPLIT];
+#pragma unroll
+    for (int c = 0; c < SPLIT; ++c) {
+      a[c] = ld_cluster_v4(mapa_u32(lo, c));
+      b[c] = ld_cluster_v4(mapa_u32(hi, c));
+    }
+#pragma unroll
+    for (int c = 1; c < SPLIT; ++c) {
+      a[0].x += a[c].x, a[0].y += a[c].y, a[0].z += a[c].z, a[0].w += a[c].w;
+      b[0].x += b[c].x, b[0].y += b[c].y, b[0].z += b[c].z, b[0].w += b[c].w;
+    }
+    if (row < rows_left && chunk * 8 < dim) {
+      const float f = second ? scale : 1.f;
+      const AttnTensor& d = second ? dk : dv;
+      *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(d.ptr) + (long long)(token0 + row) * d.token_stride + (long long)head * d.head_stride + chunk * 8) =
+          make_uint4(pack_bf16(a[0].x * f, a[0].y * f), pack_bf16(a[0].z * f, a[0].w * f), pack_bf16(b[0].x * f, b[0].y * f), pack_bf16(b[0].z * f, b[0].w * f));
+    }
+  }
+}
+
 template <int DP, bool KV>
 __device__ __forceinline__ void attn_bwd_body(const CUtensorMap* map_q, const CUtensorMap* map_k, const CUtensorMap* map_v, const CUtensorMap* map_do,
                                               const Geo& g, const int block, const int split, const float* __restrict__ stats, const float* __restrict__ delta,
@@ -733,9 +766,8 @@ __device__ __forceinline__ void attn_bwd_body(const CUtensorMap* map_q, const CU
     bool ok = mbar_wait(KV ? bar_x : bar_xa, 0, failed);
     fence_after_sync();
     int part = first_part;
-    // waits for the tiles of an iteration and issues its scores and dP, over the operands of the set's tile before: products
-    // run in the order of issue
-    auto products = [&](int it) {
+    // waits for the tiles of an iteration
+    auto tiles = [&](int it) {
       if (!mbar_wait(full(it % NS), (it / NS) & 1, failed)) return false;
       if (t.len - part * N < N) {                      // rows behind the end of the sequence take part in the reductions
         zero_rows<DP, N>(stage(it), t.len - part * N);
@@ -746,21 +778,27 @@ __device__ __forceinline__ void attn_bwd_body(const CUtensorMap* map_q, const CU
       } else {
         --part;
       }
-      if (elect_one()) {
-        const uint32_t y = smem_u32(stage(it));
-        if (KV) mma_scores<DP, N>(s_col(it), x0, y);
-        else mma_scores_ts<DP, N>(s_col(it), tmem + Cfg::kColX, y);
-        umma_commit(bar_s(it % SETS));
-        if (KV) mma_scores<DP, N>(s_col(it) + N, x1, y + Cfg::kYBytes);
-        else mma_scores_ts<DP, N>(s_col(it) + N, tmem + Cfg::kColX + DP / 2, y + Cfg::kYBytes);
-        umma_commit(bar_dp(it % SETS));
-      }
-      __syncwarp();
       return true;
     };
-    for (int it = 0; it < SETS && it < n; ++it) ok = ok && products(it);
+    // scores and dP of an iteration, over the operands of the set's tile before: products run in the order of issue
+    auto products = [&](int it) {
+      const uint32_t y = smem_u32(stage(it));
+      if (KV) mma_scores<DP, N>(s_col(it), x0, y);
+      else mma_scores_ts<DP, N>(s_col(it), tmem + Cfg::kColX, y);
+      umma_commit(bar_s(it % SETS));
+      if (KV) mma_scores<DP, N>(s_col(it) + N, x1, y + Cfg::kYBytes);
+      else mma_scores_ts<DP, N>(s_col(it) + N, tmem + Cfg::kColX + DP / 2, y + Cfg::kYBytes);
+      umma_commit(bar_dp(it % SETS));
+    };
+    for (int it = 0; it < SETS && it < n && ok; ++it) {
+      ok = tiles(it);
+      if (ok && elect_one()) products(it);
+      __syncwarp();
+    }
     for (int it = 0; it < n && ok; ++it) {
-      ok = mbar_wait(bar_ds(it % SETS), (it / SETS) & 1, failed);
+      const bool more = it + SETS < n;
+      // the next tiles have arrived long ago; looked at here, their barrier is not between the operands and the products
+      ok = (!more || tiles(it + SETS)) && mbar_wait(bar_ds(it % SETS), (it / SETS) & 1, failed);
       if (!ok) break;
       fence_after_sync();
       if (elect_one()) {
@@ -768,9 +806,9 @@ __device__ __forceinline__ void attn_bwd_body(const CUtensorMap* map_q, const CU
         if (KV) mma_accumulate<DP, N>(tmem + Cfg::kCol0, s_col(it), 32, y + Cfg::kYBytes, it == 0);
         mma_accumulate<DP, N>(tmem + Cfg::kCol1, s_col(it) + N, 32, y, it == 0);
         umma_commit(empty(it % NS));
+        if (more) products(it + SETS);
       }
       __syncwarp();
-      if (it + SETS < n) ok = products(it + SETS);
     }
     if (elect_one()) {
       umma_commit(bar_end);
@@ -931,27 +969,9 @@ __device__ __forceinline__ void attn_bwd_body(const CUtensorMap* map_q, const CU
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     if (warp < Cfg::kWarps) {
-      const int rows = kTile >> (__ffs(split) - 1);
-      for (int i = threadIdx.x; i < 2 * rows * (DP / 8); i += 32 * Cfg::kWarps) {
-        const int chunk = i & (DP / 8 - 1), rest = i / (DP / 8);
-        const bool second = rest >= rows;
-        const int row = part_of_group * rows + (second ? rest - rows : rest);
-        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        const uint32_t at = smem_u32(ring) + (second ? kTile * DP * 4 : 0) + row * (DP * 4) + (chunk >> 2) * 128;
-        for (int c = 0; c < split; ++c) {
-          const float4 a = ld_cluster_v4(mapa_u32(at + ((((chunk & 3) * 2) ^ (row & 7)) << 4), c));
-          const float4 b = ld_cluster_v4(mapa_u32(at + ((((chunk & 3) * 2 + 1) ^ (row & 7)) << 4), c));
-          v[0] += a.x, v[1] += a.y, v[2] += a.z, v[3] += a.w;
-          v[4] += b.x, v[5] += b.y, v[6] += b.z, v[7] += b.w;
-        }
-        if (row0 + row < t.len && chunk * 8 < g.dim) {
-          const float f = second ? scale : 1.f;
-          const AttnTensor& d = second ? d1 : d0;
-          const uint4 out = make_uint4(pack_bf16(v[0] * f, v[1] * f), pack_bf16(v[2] * f, v[3] * f), pack_bf16(v[4] * f, v[5] * f), pack_bf16(v[6] * f, v[7] * f));
-          *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(d.ptr) + (long long)(t.start + row0 + row) * d.token_stride +
-                                    (long long)own_head * d.head_stride + chunk * 8) = out;
-        }
-      }
+      if (split == 2) add_up<DP, 2>(smem_u32(ring), part_of_group, own_head, t.start + row0, t.len - row0, g.dim, scale, d0, d1, 32 * Cfg::kWarps);
+      else if (split == 4) add_up<DP, 4>(smem_u32(ring), part_of_group, own_head, t.start + row0, t.len - row0, g.dim, scale, d0, d1, 32 * Cfg::kWarps);
+      else add_up<DP, 8>(smem_u32(ring), part_of_group, own_head, t.start + row0, t.len - row0, g.dim, scale, d0, d1, 32 * Cfg::kWarps);
     }
     // nobody leaves while another may still read its shared memory
     __syncwarp();
@@ -1012,6 +1032,12 @@ Geo MakeGeo(const AttnShape& s) {
   return g;
 }
 
+int SmCount() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
+  return n;
+}
+
 // Shared memory above 48 KB has to be allowed per device; a call costs about a microsecond, so it is made once for each.
 template <auto kernel>
 cudaError_t AllowSmem(size_t bytes) {
@@ -1050,10 +1076,11 @@ cudaError_t Backward(const AttnShape& s, const CUtensorMap& mq, const CUtensorMa
   const Geo g = MakeGeo(s);
   // The query heads of a group add to the same key tile.  Up to eight CTAs of a cluster (the portable size) share them and add up
   // their sums through distributed shared memory: without it one CTA walked over all of them, and few key heads left SMs idle
-  // (packed documents, four query heads to a key head: 380 against 330 us, forward included).  The query kind then has a
+  // (packed documents, four query heads to a key head: 380 against 330 us, forward included).  Three times as many blocks as run
+  // together even out what they differ by; more only add sums.  The query kind then has a
   // launch of its own, since blocks that need no cluster would still be started as one.
   int split = 1;
-  while (split < 8 && g.group % (2 * split) == 0) split *= 2;
+  while (split < 8 && g.group % (2 * split) == 0 && g.tiles * s.kv_heads * split < 3 * SmCount() * Cfg::kCtasPerSm) split *= 2;
   const int kv_blocks = g.tiles * s.kv_heads * split, q_blocks = g.tiles * s.heads;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(split > 1 ? kv_blocks : kv_blocks + q_blocks));
