@@ -383,6 +383,8 @@ gemm_bf16_nt_persistent_kernel(const __grid_constant__ CUtensorMap map_a, const 
       mbar_init(smem_u32(&bars[2 * S + a]), 1);        // one tcgen05.commit
       mbar_init(smem_u32(&bars[2 * S + 2 + a]), (PAIR ? 2 : 1) * Cfg::kEpiWarps);    // one arrive per epilogue warp (of both CTAs)
     }
+    if (EPI == kEpiGatedGrad)
+      for (int a = 0; a < 2 * Cfg::kEpiWarps; ++a) mbar_init(smem_u32(&bars[2 * S + 4 + a]), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -544,6 +546,31 @@ gemm_bf16_nt_persistent_kernel(const __grid_constant__ CUtensorMap map_a, const 
       for (int i = lane; i < 2 * BN_; i += 32) wstat[i] = 0.f;
       __syncwarp();
     }
+    // kEpiGatedGrad: the kept g and u come through TMA boxes of 32 rows x 32 columns, one chunk ahead, into two sets of a g and a u
+    // box per warp; dG and dU replace them there and leave from there.  (Read by the threads row by row, 32 sectors per load,
+    // the epilogue took four times as long as the main loop of a reduction of 1024.)
+    constexpr int kParts = Cfg::kTileN / 32 / (Cfg::kEpiWarps == 8 ? 2 : 1);
+    const int part_first = Cfg::kEpiWarps == 8 ? (ew >> 2) * kParts : 0;
+    int pre_tile = first_tile, pre_part = part_first, loaded = 0, used = 0;
+    auto pre_bar = [&](int set) { return smem_u32(&bars[2 * S + 4 + ew * 2 + set]); };
+    auto prefetch = [&]() {
+      for (; pre_tile < num_tiles; pre_tile += tile_step, pre_part = part_first) {
+        int tm, tn;
+        tile_coords(pre_tile, tiles_m, tiles_n, tm, tn);
+        const int row = tm * Cfg::kTileM + int(rank) * BM + q * 32, col = tn * Cfg::kTileN + pre_part * 32;
+        if (pre_part == part_first + kParts || row >= M || col >= N) continue;
+        if (lane == 0) {
+          const uint32_t bar = pre_bar(loaded & 1), dst = smem_u32(my_out) + (loaded & 1) * 4096u;
+          mbar_expect_tx(bar, 4096);
+          tma_load_2d(dst, &map_b2, bar, col, row);
+          tma_load_2d(dst + 2048, &map_aux2, bar, col, row);
+        }
+        ++loaded;
+        ++pre_part;
+        return;
+      }
+    };
+    if constexpr (EPI == kEpiGatedGrad) prefetch();
     for (int tile = first_tile; tile < num_tiles; tile += tile_step, ++local) {
       const int acc = local & 1;
       int tm, tn;
@@ -601,6 +628,60 @@ gemm_bf16_nt_persistent_kernel(const __grid_constant__ CUtensorMap map_a, const 
             leave(&map_aux2, [&](int i) { return __uint_as_float(u[i]); });
           }
           leave(&map_c, [&](int i) { return gate_fn(__uint_as_float(g[i]), act, nullptr) * __uint_as_float(u[i]); });
+        }
+      } else if constexpr (EPI == kEpiGatedGrad) {
+        // accumulator = dH:  dG = dH u act'(g) through map_c, dU = dH act(g) through map_aux
+#pragma unroll 1
+        for (int c = part_first; c < part_first + kParts; ++c) {
+          const int nbase = n0 + c * 32;
+          if (nbase >= N || m0 + q * 32 >= M) break;           // warp-uniform; prefetch() walks the same chunks
+          uint32_t r[32];
+          tmem_ld32(tmem_base + (uint32_t(q * 32) << 16) + uint32_t(acc * BN_ + c * 32), r);
+          unsigned char* box = my_out + (used & 1) * 4096;
+          if (!mbar_wait(pre_bar(used & 1), (used >> 1) & 1, failed)) {
+            tmem_wait_ld();
+            break;
+          }
+          tmem_wait_ld();
+          tie32(r);
+          uint4 dg[4], du[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            int off = lane * 64 + j * 16;
+            off ^= ((off >> 7) & 3) << 4;                      // 64-byte swizzle
+            const uint4 gv = *reinterpret_cast<const uint4*>(box + off), uv = *reinterpret_cast<const uint4*>(box + 2048 + off);
+            const __nv_bfloat162* gh = reinterpret_cast<const __nv_bfloat162*>(&gv);
+            const __nv_bfloat162* uh = reinterpret_cast<const __nv_bfloat162*>(&uv);
+            float a[8], b[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float2 g2 = __bfloat1622float2(gh[i >> 1]), u2 = __bfloat1622float2(uh[i >> 1]);
+              const float dh = __uint_as_float(r[j * 8 + i]);
+              float slope;
+              b[i] = dh * gate_fn((i & 1) ? g2.y : g2.x, act, &slope);
+              a[i] = dh * ((i & 1) ? u2.y : u2.x) * slope;
+            }
+            dg[j] = pack8(a);
+            du[j] = pack8(b);
+          }
+          if (lane == 0) tma_store_wait_read<0>();             // the other set has left: the next chunk may come in
+          __syncwarp();
+          prefetch();
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            int off = lane * 64 + j * 16;
+            off ^= ((off >> 7) & 3) << 4;
+            *reinterpret_cast<uint4*>(box + off) = dg[j];
+            *reinterpret_cast<uint4*>(box + 2048 + off) = du[j];
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&map_c, smem_u32(box), nbase, m0 + q * 32);
+            tma_store_2d(&map_aux, smem_u32(box + 2048), nbase, m0 + q * 32);
+            tma_store_commit();
+          }
+          ++used;
         }
       } else if (tma_out) {
 #pragma unroll 1
@@ -725,42 +806,6 @@ gemm_bf16_nt_persistent_kernel(const __grid_constant__ CUtensorMap map_a, const 
               tma_store_commit();
             }
             ++boxes;
-          } else if constexpr (EPI == kEpiGatedGrad) {
-            // accumulator = dH; with the kept g (aux_in) and u (N values behind it in the same row of 2 N):
-            // dG = dH u act'(g) through map_c, dU = dH act(g) through map_aux
-            if (lane == 0) tma_store_wait_read<0>();
-            __syncwarp();
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              uint4 gv = make_uint4(0u, 0u, 0u, 0u), uv = gv;
-              if (m < M && nbase + j * 8 < N) {
-                const __nv_bfloat16* src = aux_in + size_t(m) * (2 * size_t(N)) + nbase + j * 8;
-                gv = __ldg(reinterpret_cast<const uint4*>(src));
-                uv = __ldg(reinterpret_cast<const uint4*>(src + N));
-              }
-              const __nv_bfloat162* gh = reinterpret_cast<const __nv_bfloat162*>(&gv);
-              const __nv_bfloat162* uh = reinterpret_cast<const __nv_bfloat162*>(&uv);
-              float dg[8], du[8];
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const float2 g2 = __bfloat1622float2(gh[i >> 1]), u2 = __bfloat1622float2(uh[i >> 1]);
-                const float dh = __uint_as_float(r[j * 8 + i]);
-                float slope;
-                du[i] = dh * gate_fn((i & 1) ? g2.y : g2.x, act, &slope);
-                dg[i] = dh * ((i & 1) ? u2.y : u2.x) * slope;
-              }
-              const int off = (j ^ (lane & 7)) << 4;                                // 128-byte swizzle
-              *reinterpret_cast<uint4*>(my_out + lane * 128 + off) = pack8(dg);
-              *reinterpret_cast<uint4*>(my_out + Cfg::kBytesOutBox + lane * 128 + off) = pack8(du);
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) {
-              tma_store_2d(&map_c, smem_u32(my_out), nbase, m0 + q * 32);
-              tma_store_2d(&map_aux, smem_u32(my_out + Cfg::kBytesOutBox), nbase, m0 + q * 32);
-              tma_store_commit();
-            }
-            boxes += 2;
           } else {
             // kEpiStorePreact: two boxes leave per chunk, x = accumulator + bias through map_aux and act(x)
             // through map_c; both staging boxes are in use, so every earlier store must have been read
@@ -846,8 +891,14 @@ gemm_bf16_nt_persistent_kernel(const __grid_constant__ CUtensorMap map_a, const 
       }
     }
     if constexpr (EPI == kEpiColumnStats) flush_stats();
-    // the stores of this warp must be complete before its shared memory goes away
+    // the stores of this warp must be complete before its shared memory goes away, and after a failure its loads too
     if (lane == 0) tma_store_wait_all();
+    if constexpr (EPI == kEpiGatedGrad) {
+      for (; used < loaded; ++used) {
+        const unsigned long long t0 = now_ns();
+        while (!mbar_try(pre_bar(used & 1), (used >> 1) & 1) && now_ns() - t0 < kWaitLimitNs) {}
+      }
+    }
   }
   if (warp == 0 && lane == 0 && *failed && leader) {
     const int first = armed > S ? armed - S : 0;
@@ -871,12 +922,12 @@ gemm_bf16_nt_persistent_kernel(const __grid_constant__ CUtensorMap map_a, const 
   if (threadIdx.x == 0 && failed_s && status != nullptr) atomicExch(status, 1u);
 }
 
-// pitch: elements from row to row (0: the rows follow one another)
-bool MakeMap(CUtensorMap* map, const void* base, int rows, int cols /*K*/, int box_rows, long long pitch = 0) {
+// pitch: elements from row to row (0: the rows follow one another); boxes of 64 columns in the 128-byte swizzle, of 32 in the 64-byte one
+bool MakeMap(CUtensorMap* map, const void* base, int rows, int cols /*K*/, int box_rows, long long pitch = 0, int box_cols = BK) {
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
   const cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch != 0 ? pitch : cols) * 2};
-  const cuuint32_t box[2] = {static_cast<cuuint32_t>(BK), static_cast<cuuint32_t>(box_rows)};
-  return EncodeTiled(map, 2, base, dims, strides, box);
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows)};
+  return EncodeTiled(map, 2, base, dims, strides, box, nullptr, box_cols == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 // Launches one instantiation of the persistent kernel on min(tiles, SMs) CTAs; PAIR: on clusters of two CTAs, one
@@ -1140,15 +1191,18 @@ cudaError_t LaunchGemmBf16NNGatedGrad(const void* a, const void* b, const void* 
   const int sm_count = SmCount();
   __nv_bfloat16* o = static_cast<__nv_bfloat16*>(dpre);
   const __nv_bfloat16* pre = static_cast<const __nv_bfloat16*>(preact);
-  CUtensorMap map_a, map_b, map_g, map_u;
-  if (!MakeMap(&map_a, a, M, K, BM) || !MakeMap(&map_b, b, K, F, 64) || !MakeMap(&map_g, o, M, F, 32, 2ll * F) ||
-      !MakeMap(&map_u, o + F, M, F, 32, 2ll * F))
+  CUtensorMap map_a, map_b, map_dg, map_du, map_g, map_u;
+  if (!MakeMap(&map_a, a, M, K, BM) || !MakeMap(&map_b, b, K, F, 64) || !MakeMap(&map_dg, o, M, F, 32, 2ll * F, 32) ||
+      !MakeMap(&map_du, o + F, M, F, 32, 2ll * F, 32) || !MakeMap(&map_g, pre, M, F, 32, 2ll * F, 32) ||
+      !MakeMap(&map_u, pre + F, M, F, 32, 2ll * F, 32))
     return cudaErrorInvalidValue;
   const cudaError_t e =
-      UsePair(M, F, K, sm_count) ? LaunchPersistent<256, 1, 0, kEpiGatedGrad, 1>(map_a, map_b, map_g, map_u, o, nullptr, pre, M, F, K, act, 1,
-                                                                                 sm_count, status, stream)
-      : F > 128 ? LaunchPersistent<256, 1, 0, kEpiGatedGrad>(map_a, map_b, map_g, map_u, o, nullptr, pre, M, F, K, act, 1, sm_count, status, stream)
-                : LaunchPersistent<128, 1, 0, kEpiGatedGrad>(map_a, map_b, map_g, map_u, o, nullptr, pre, M, F, K, act, 1, sm_count, status, stream);
+      UsePair(M, F, K, sm_count) ? LaunchPersistent<256, 1, 0, kEpiGatedGrad, 1>(map_a, map_b, map_dg, map_du, o, nullptr, nullptr, M, F, K, act, 1,
+                                                                                 sm_count, status, stream, nullptr, &map_g, &map_u)
+      : F > 128 ? LaunchPersistent<256, 1, 0, kEpiGatedGrad>(map_a, map_b, map_dg, map_du, o, nullptr, nullptr, M, F, K, act, 1, sm_count, status,
+                                                             stream, nullptr, &map_g, &map_u)
+                : LaunchPersistent<128, 1, 0, kEpiGatedGrad>(map_a, map_b, map_dg, map_du, o, nullptr, nullptr, M, F, K, act, 1, sm_count, status,
+                                                             stream, nullptr, &map_g, &map_u);
   if (e != cudaSuccess) return e;
   CountKernelLaunch();
   return cudaGetLastError();

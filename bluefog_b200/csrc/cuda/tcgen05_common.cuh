@@ -304,14 +304,15 @@ inline EncodeTiledFn GetEncodeFn() {
 // CUDA_ERROR_INVALID_CONTEXT from the driver entry point: bind the context and encode once more.
 // elem_strides (optional, one per dimension): traversal strides; a box of extent e*stride then delivers e elements.
 inline bool EncodeTiled(CUtensorMap* map, cuuint32_t rank, const void* base, const cuuint64_t* dims,
-                        const cuuint64_t* strides, const cuuint32_t* box, const cuuint32_t* elem_strides = nullptr) {
+                        const cuuint64_t* strides, const cuuint32_t* box, const cuuint32_t* elem_strides = nullptr,
+                        CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
   EncodeTiledFn fn = GetEncodeFn();
   if (fn == nullptr) return false;
   const cuuint32_t unit[5] = {1, 1, 1, 1, 1};
   const cuuint32_t* estr = elem_strides != nullptr ? elem_strides : unit;
   auto encode = [&] {
     return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims, strides, box, estr,
-              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   };
   CUresult r = encode();
