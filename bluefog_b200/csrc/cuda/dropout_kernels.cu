@@ -5,8 +5,9 @@
 // of 128 bits serves eight elements, sixteen bits each: p is a multiple of 2^-16, and the factor is the inverse of the
 // probability that is really used, so the expectation is exact.  A dropped element contributes zero whatever x holds.
 //
-// Bound by memory: x and residual are read and out is written once (6 bytes per bf16 element forward, 4 backward); a block
-// of Philox costs about 60 instructions, 8 per element, half of what the memory leaves time for.
+// Bound by memory: x and residual are read and out is written once (6 bytes per bf16 element forward, 4 backward), which on 65536 x
+// 2048 takes 121 and 95 us (6.6 and 5.7 TB/s).  Next to it stands the integer pipe: a block of Philox and eight tests take
+// about 50 of its instructions, some 55 us on that tensor.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -54,14 +55,18 @@ __device__ __forceinline__ Eight<T> load8(const T* p) {
   return e;
 }
 
+// x becomes res + (keep ? factor * x : 0), in fp32 with one rounding to T.  A 16-bit word is compared where it stands, shifted to
+// the upper half of its 32 bits (limit: threshold there), and the multiplication is predicated: what bounds the instruction count
+// is the integer pipe.
 template <typename T, bool RES>
-__device__ __forceinline__ void apply(Eight<T>& x, const Eight<T>& res, const uint4 bits, uint32_t threshold, float factor) {
+__device__ __forceinline__ void apply(Eight<T>& x, const Eight<T>& res, const uint4 bits, const uint32_t limit, const bool none, float factor) {
   const uint32_t w[4] = {bits.x, bits.y, bits.z, bits.w};
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const uint32_t u = (i & 1) ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu;
-    float y = u >= threshold ? to_f(x.v[i]) * factor : 0.f;
-    if (RES) y += to_f(res.v[i]);
+    const uint32_t u = (i & 1) ? w[i >> 1] : w[i >> 1] << 16;
+    const float v = to_f(x.v[i]);
+    float y = RES ? to_f(res.v[i]) : 0.f;
+    if (u >= limit && !none) y = RES ? fmaf(v, factor, y) : v * factor;
     x.v[i] = from_f<T>(y);
   }
 }
@@ -72,47 +77,45 @@ __device__ __forceinline__ void store8(T* p, const Eight<T>& e) {
   for (int i = 0; i < int(sizeof(Eight<T>) / 16); ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(&e)[i];
 }
 
-// A block takes 256 groups of eight elements per load; all UNROLL loads of a thread are in flight before the first is used: with one
-// 16-byte load per thread the backward pass, which has no residual to read beside it, reached 5.1 TB/s on 268 MB tensors.
 template <typename T, bool RES, int UNROLL>
 __global__ void __launch_bounds__(kThreads)
 dropout_add_kernel(const T* x, const T* residual, T* out, const long long n, const uint32_t threshold, const float factor,
                    const long long* __restrict__ key, const uint32_t site) {
   const unsigned long long seed = key[0], step = key[1];
+  const uint32_t limit = threshold << 16;              // 65536 does not fit: then nothing is kept
+  const bool none = threshold > 65535u;
   const long long groups = n / 8;
-  const long long stride = (long long)gridDim.x * (kThreads * UNROLL);
   auto bits = [&](long long g) {
     return philox(make_uint4(uint32_t(g), uint32_t(g >> 32) | site << 16, uint32_t(step), uint32_t(step >> 32)), uint32_t(seed), uint32_t(seed >> 32));
   };
-  for (long long g0 = (long long)blockIdx.x * (kThreads * UNROLL) + threadIdx.x; g0 <= groups; g0 += stride) {
+  const long long stride = (long long)gridDim.x * (kThreads * UNROLL);
+  long long g = (long long)blockIdx.x * (kThreads * UNROLL) + threadIdx.x;
+  for (; g + (UNROLL - 1) * kThreads < groups; g += stride) {
     Eight<T> a[UNROLL], r[UNROLL];
 #pragma unroll
     for (int k = 0; k < UNROLL; ++k) {
-      const long long g = g0 + k * kThreads;
-      if (g < groups) {
-        a[k] = load8(x + g * 8);
-        if (RES) r[k] = load8(residual + g * 8);
-      }
+      a[k] = load8(x + (g + k * kThreads) * 8);
+      if (RES) r[k] = load8(residual + (g + k * kThreads) * 8);
     }
 #pragma unroll
     for (int k = 0; k < UNROLL; ++k) {
-      const long long g = g0 + k * kThreads;
-      if (g < groups) {
-        apply<T, RES>(a[k], r[k], bits(g), threshold, factor);
-        store8(out + g * 8, a[k]);
-      } else if (g == groups && groups * 8 < n) {       // up to seven elements at the end
-        const int rest = int(n - groups * 8);
-        Eight<T> t = {}, u = {};
-        for (int i = 0; i < 7; ++i)
-          if (i < rest) {
-            t.v[i] = x[groups * 8 + i];
-            if (RES) u.v[i] = residual[groups * 8 + i];
-          }
-        apply<T, RES>(t, u, bits(g), threshold, factor);
-        for (int i = 0; i < 7; ++i)
-          if (i < rest) out[groups * 8 + i] = t.v[i];
-      }
+      apply<T, RES>(a[k], r[k], bits(g + k * kThreads), limit, none, factor);
+      store8(out + (g + k * kThreads) * 8, a[k]);
     }
+  }
+  for (; g <= groups; g += kThreads) {                 // what is left of the last round, and up to seven elements at the end
+    if (g >= groups && groups * 8 == n) break;
+    const int count = g < groups ? 8 : int(n - groups * 8);
+    Eight<T> a = {}, r = {};
+    for (int i = 0; i < 8; ++i)
+      if (i < count) {
+        a.v[i] = x[g * 8 + i];
+        if (RES) r.v[i] = residual[g * 8 + i];
+      }
+    apply<T, RES>(a, r, bits(g), limit, none, factor);
+    for (int i = 0; i < 8; ++i)
+      if (i < count) out[g * 8 + i] = a.v[i];
+    if (UNROLL == 1) break;
   }
 }
 
@@ -126,14 +129,16 @@ cudaError_t Launch(const void* x, const void* residual, void* out, long long n, 
   const T* a = static_cast<const T*>(x);
   const T* r = static_cast<const T*>(residual);
   T* o = static_cast<T*>(out);
-  // 32 bytes of each stream per thread in flight, as long as that leaves every SM two blocks
-  constexpr int kWide = sizeof(T) == 4 ? 2 : 4;
+  // Loads in flight: two groups per stream and thread with a residual, four without (fp32: two of 32 bytes), where that leaves every
+  // SM two blocks; with one, 65536 x 2048 bf16 takes 135 instead of 121 us with a residual and 102 instead of 95 us without.
+  constexpr int kAlone = sizeof(T) == 4 ? 2 : 4;
+  const int unroll = r != nullptr ? 2 : kAlone;
   const long long blocks = (n / 8 + kThreads) / kThreads;
-  const bool wide = blocks >= 2ll * sms * kWide;
-  const long long need = wide ? (blocks + kWide - 1) / kWide : blocks, most = (long long)sms * 8;
+  const bool wide = blocks >= 2ll * sms * unroll;
+  const long long need = wide ? (blocks + unroll - 1) / unroll : blocks, most = (long long)sms * 32;
   const unsigned grid = static_cast<unsigned>(need < most ? need : most);
   auto go = [&](auto kernel) { kernel<<<grid, kThreads, 0, stream>>>(a, r, o, n, threshold, factor, key, site); };
-  if (wide) r != nullptr ? go(dropout_add_kernel<T, true, kWide>) : go(dropout_add_kernel<T, false, kWide>);
+  if (wide) r != nullptr ? go(dropout_add_kernel<T, true, 2>) : go(dropout_add_kernel<T, false, kAlone>);
   else r != nullptr ? go(dropout_add_kernel<T, true, 1>) : go(dropout_add_kernel<T, false, 1>);
   CountKernelLaunch();
   return cudaGetLastError();
