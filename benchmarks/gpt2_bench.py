@@ -31,13 +31,18 @@ def main():
                     help="format in which neighbors read each other's parameters (the own term and the master "
                          "weights stay fp32)")
     ap.add_argument("--no-graphs", action="store_true", help="drive forward/backward op by op instead of a CUDA graph")
+    ap.add_argument("--b200-attention", action="store_true", help="attention on this library's kernels instead of PyTorch's")
+    ap.add_argument("--n-kv-head", type=int, default=None, help="key and value heads (grouped attention); default: as many as query heads")
+    ap.add_argument("--mlp", default="gelu", choices=["gelu", "swiglu", "geglu"])
+    ap.add_argument("--dropout", type=float, default=0.0)
     args = ap.parse_args()
     bf.init()
     rank, size = bf.rank(), bf.size()
     dev = torch.device("cuda", torch.cuda.current_device())
     bf.set_topology(bf.RingGraph(size), is_weighted=True)
     torch.manual_seed(1 + rank)
-    model = getattr(gpt2, args.model)(use_b200_gemm=not args.no_b200_gemm).to(dev)
+    model = getattr(gpt2, args.model)(use_b200_gemm=not args.no_b200_gemm, use_b200_attention=args.b200_attention,
+                                      n_kv_head=args.n_kv_head, mlp=args.mlp, dropout=args.dropout).to(dev)
     bf.broadcast_parameters(model.state_dict(), root_rank=0)
     opt = bf.DistributedAdaptThenCombineOptimizer(
         torch.optim.AdamW(model.parameters(), lr=3e-4, weight_decay=0.1), model,
@@ -81,7 +86,8 @@ def main():
         print(json.dumps({"metric": "GPT-2 training throughput (tokens/s), ATC AdamW, ring", "value": round(toks, 1),
                           "unit": "tokens/s", "n_gpus": size, "ms_per_step": round(ms / args.steps, 2),
                           "model": args.model, "batch_per_gpu": args.batch, "seq_len": args.seq, "dtype": "bf16",
-                          "exchange_dtype": args.exchange_dtype,
+                          "exchange_dtype": args.exchange_dtype, "b200_attention": args.b200_attention,
+                          "n_kv_head": args.n_kv_head, "mlp": args.mlp, "dropout": args.dropout,
                           "final_loss": float(loss)}), flush=True)
     bf.barrier()
     bf.shutdown()

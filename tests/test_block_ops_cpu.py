@@ -129,3 +129,51 @@ def test_gated_mlp_refuses(change):
     args.update(change)
     with pytest.raises(ValueError):
         gemm.gated_mlp(**args)
+
+
+def _gpt2(**kw):
+    from bluefog_b200.models import gpt2
+    torch.manual_seed(0)
+    return gpt2.GPT2(vocab_size=101, n_positions=16, d_model=32, n_layer=2, n_head=4, **kw)
+
+
+def test_gpt2_keeps_its_parameters_and_results_without_the_options():
+    a = _gpt2()
+    assert a.h[0].attn.c_attn.weight.shape == (96, 32) and a.h[0].mlp.c_fc.weight.shape == (128, 32)
+    assert not any("dropout" in n for n in a.state_dict())
+    idx = torch.randint(0, 101, (2, 16))
+    torch.testing.assert_close(_gpt2(use_b200_attention=True)(idx), a(idx))
+
+
+def test_gpt2_documents_do_not_see_each_other():
+    m = _gpt2(n_kv_head=2, mlp="swiglu")
+    assert m.h[0].attn.c_attn.weight.shape == (64, 32) and m.h[0].mlp.c_fc.weight.shape == (2 * 128, 32)
+    idx = torch.randint(0, 101, (1, 16))
+    cu = torch.tensor([0, 5, 16], dtype=torch.int32)
+    want = m(idx, cu_seqlens=cu)
+    other = idx.clone()
+    other[:, :5] = (other[:, :5] + 1) % 101
+    got = m(other, cu_seqlens=cu)
+    assert torch.equal(got[:, 5:], want[:, 5:]) and not torch.equal(got[:, :5], want[:, :5])
+    assert not torch.equal(m(other)[:, 5:], m(idx)[:, 5:])
+
+
+def test_gpt2_dropout_draws_a_mask_per_step_and_none_in_evaluation():
+    m = _gpt2(dropout=0.3, mlp="geglu")
+    assert m.dropout_key.tolist()[1] == 0 and "dropout_key" in m.state_dict()
+    idx = torch.randint(0, 101, (2, 16))
+    a, b = m(idx), m(idx)
+    assert not torch.equal(a, b) and m.dropout_key.tolist()[1] == 2
+    m.dropout_key[1] = 0
+    assert torch.equal(m(idx), a)
+    m.eval()
+    assert torch.equal(m(idx), m(idx)) and m.dropout_key.tolist()[1] == 1
+    m.train()
+    m(idx, torch.randint(0, 101, (2, 16))).backward()
+    assert all(p.grad is not None and torch.isfinite(p.grad).all() for p in m.parameters())
+
+
+@pytest.mark.parametrize("kw", [dict(n_kv_head=3), dict(n_kv_head=0), dict(mlp="relu"), dict(dropout=1.0), dict(dropout=-0.1)])
+def test_gpt2_refuses(kw):
+    with pytest.raises(ValueError):
+        _gpt2(**kw)
