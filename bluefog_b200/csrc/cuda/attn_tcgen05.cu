@@ -185,6 +185,17 @@ __device__ __forceinline__ void mma_accumulate(uint32_t tmem_d, uint32_t a, uint
                 (first && k == 0) ? 0u : 1u);
 }
 
+// All warps of a block learn that its barriers and its tensor memory are there; the producer, which made the barriers and has no
+// use for tensor memory, only says so and goes on loading.
+template <int THREADS>
+__device__ __forceinline__ void set_up_done(bool producer) {
+  fence_before_sync();
+  __syncwarp();
+  if (producer) asm volatile("barrier.cta.arrive 15, %0;" ::"n"(THREADS) : "memory");
+  else asm volatile("barrier.cta.sync 15, %0;" ::"n"(THREADS) : "memory");
+  fence_after_sync();
+}
+
 // Zeros in rows [first, N) of DP / 64 boxes of N rows; called by a whole warp, visible to the tensor cores afterwards.
 template <int DP, int N>
 __device__ __forceinline__ void zero_rows(unsigned char* boxes, int first) {
@@ -248,45 +259,47 @@ __device__ __forceinline__ void store_rows(const AttnTensor& t, int head, int to
 }
 
 // ---------------------------------------------------------------------------------------------------------------- //
-// Forward.  One CTA per query tile and head, two CTAs per SM: while the softmax warps of one wait for a product, those of
-// the other keep the exponential unit busy.  Eight softmax warps: two threads share a row, 64 columns each, and exchange
-// their maxima through shared memory (with one thread per row the 128 scores in its registers spilled and one warp per
-// scheduler and CTA could not hide the latency of its own exponentials: 12 cycles per element against the 8 that the unit
-// needs).  Key tiles are taken from the diagonal downwards, so only the first one needs a mask.  Tensor memory (256 of 512
-// columns per CTA): scores 128, output DP, and P in a place of its own where there is room (DP = 64: the next scores are
-// computed while this tile's exponentials are taken), over the scores otherwise.  The output is rescaled only when a row's
-// maximum grew by more than 2^8 (the sums stay far inside fp32).
+// Forward.  One CTA per tile of 128 queries and head, kN keys at a time.  The exponentials are what there is most of: 16 a cycle
+// and SM, 1024 cycles per 128 x 128 scores against 512 (DP = 64) or 1024 of products.  One tile's chain - scores, maximum,
+// exponentials, product - leaves that unit idle most of the time, so three CTAs (DP = 64: 64 keys, 128 tensor-memory columns each)
+// or two (DP = 128: 128 keys, 256 columns) run on an SM and fill each other's waits, their beginnings and ends included.  Every
+// softmax thread has 64 scores: a whole row of 64, or half a row of 128, the two threads of a row then exchanging maxima
+// through shared memory.  P replaces the scores.  The output is rescaled only when a row's maximum grew by more than 2^8
+// (the sums stay far inside fp32).  Keys are taken from the diagonal downwards, so that only the first tiles need a mask.
 // ---------------------------------------------------------------------------------------------------------------- //
 template <int DP>
 struct FwdCfg {
   static constexpr int kBoxes = DP / 64;
-  static constexpr int kSlots = DP == 64 ? 5 : 2;       // ring of key / value tiles
-  static constexpr uint32_t kTileBytes = kBoxes * kBoxBytes;
-  static constexpr int kThreads = 320;
-  static constexpr uint32_t kColO = 128;
-  static constexpr bool kOwnP = DP == 64;
-  static constexpr uint32_t kColP = kOwnP ? 192 : 0;
-  static constexpr size_t kSmem = 1024 + size_t(kSlots + 1) * kTileBytes;
+  static constexpr int kN = DP == 64 ? 64 : 128;        // keys of a tile
+  static constexpr int kHalves = kN / 64;               // threads per row
+  static constexpr int kWarps = 4 * kHalves;            // those that take exponentials
+  static constexpr int kThreads = 32 * (kWarps + 2);
+  static constexpr int kCtasPerSm = DP == 64 ? 3 : 2;
+  static constexpr int kSlots = DP == 64 ? 4 : 2;       // ring of key / value tiles
+  static constexpr uint32_t kQBytes = kBoxes * kBoxBytes;
+  static constexpr uint32_t kYBytes = kBoxes * kN * 128;
+  static constexpr uint32_t kCols = DP == 64 ? 128 : 256;
+  static constexpr uint32_t kColO = kN;
+  static constexpr size_t kSmem = 1024 + size_t(kQBytes) + size_t(kSlots) * kYBytes;
 };
 
 template <int DP>
-__global__ void __launch_bounds__(FwdCfg<DP>::kThreads, 2)
+__global__ void __launch_bounds__(FwdCfg<DP>::kThreads, FwdCfg<DP>::kCtasPerSm)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                 const __grid_constant__ CUtensorMap map_v, const Geo g, const AttnTensor out, float* __restrict__ stats,
                 const float scale_log2, unsigned int* __restrict__ status) {
   using Cfg = FwdCfg<DP>;
-  constexpr int NS = Cfg::kSlots;
+  constexpr int NS = Cfg::kSlots, N = Cfg::kN, H = Cfg::kHalves;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem_q = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  unsigned char* ring = smem_q + Cfg::kTileBytes;
-  __shared__ uint64_t bars[2 * NS + 6];
-  __shared__ float maxima[2][2][kTile];
+  unsigned char* ring = smem_q + Cfg::kQBytes;
+  __shared__ uint64_t bars[2 * NS + 5];
   __shared__ uint32_t tmem_base_s;
   __shared__ int failed_s;
+  __shared__ float maxima[2][H][kTile];
   volatile int* failed = &failed_s;
   const uint32_t bar0 = smem_u32(bars);
-  const uint32_t bar_q = bar0 + 8u * (2 * NS), bar_s = bar_q + 8u, bar_sfree = bar_q + 16u, bar_p = bar_q + 24u,
-                 bar_pv = bar_q + 32u, bar_end = bar_q + 40u;
+  const uint32_t bar_q = bar0 + 8u * (2 * NS), bar_s = bar_q + 8u, bar_p = bar_q + 16u, bar_pv = bar_q + 24u, bar_end = bar_q + 32u;
   auto full = [&](int s) { return bar0 + 8u * s; };
   auto empty = [&](int s) { return bar0 + 8u * (NS + s); };
 
@@ -308,10 +321,23 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     zero_result(out, head, t.start + row0, t.start + t.len, g.dim);
     return;
   }
-  const int n = t.index + 1;                           // key tiles
   const int kv_head = divide(head, g.by_group);
+  // key tiles: those that overlap the query tile in ascending order, so that every row sees a key in the first one, then downwards
+  const int first = t.index * (kTile / N);
+  const int diagonal = min((t.len - row0 + N - 1) / N, kTile / N);
+  const int n = first + diagonal;
+  auto key_tile = [&](int it) { return it < diagonal ? first + it : n - 1 - it; };
 
-  if (warp == 8 && lane == 0) {
+  int armed = 0;                                       // the producer's place: K0 V0 K1 V1 ...
+  auto load = [&] {
+    const int s = armed % NS;
+    mbar_expect_tx(full(s), Cfg::kYBytes);
+    for (int b = 0; b < Cfg::kBoxes; ++b)
+      tma_load_3d(smem_u32(ring + size_t(s) * Cfg::kYBytes) + b * (N * 128), (armed & 1) ? &map_v : &map_k, full(s), b * 64, kv_head,
+                  t.start + key_tile(armed >> 1) * N);
+    ++armed;
+  };
+  if (warp == Cfg::kWarps && lane == 0) {
     failed_s = 0;
     for (int s = 0; s < NS; ++s) {
       mbar_init(full(s), 1);
@@ -319,50 +345,29 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     }
     mbar_init(bar_q, 1);
     mbar_init(bar_s, 1);
-    mbar_init(bar_sfree, 8);
-    mbar_init(bar_p, 8);
+    mbar_init(bar_p, Cfg::kWarps);
     mbar_init(bar_pv, 1);
     mbar_init(bar_end, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    // the first tiles travel while tensor memory is allocated
-    mbar_expect_tx(bar_q, Cfg::kTileBytes);
+    // the first two tiles travel while tensor memory is allocated
+    mbar_expect_tx(bar_q, Cfg::kQBytes);
     for (int b = 0; b < Cfg::kBoxes; ++b) tma_load_3d(smem_u32(smem_q) + b * kBoxBytes, &map_q, bar_q, b * 64, head, t.start + row0);
-    mbar_expect_tx(full(0), Cfg::kTileBytes);
-    for (int b = 0; b < Cfg::kBoxes; ++b)
-      tma_load_3d(smem_u32(ring) + b * kBoxBytes, &map_k, full(0), b * 64, kv_head, t.start + (n - 1) * kTile);
+    load();
   }
-  if (warp == 9) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 256;" ::"r"(smem_u32(&tmem_base_s)) : "memory");
+  if (warp == Cfg::kWarps + 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)), "r"(Cfg::kCols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  fence_before_sync();
-  __syncthreads();
-  fence_after_sync();
-  const uint32_t tmem = tmem_base_s;
+  set_up_done<Cfg::kThreads>(warp == Cfg::kWarps);
 
-  if (warp == 8) {
+  if (warp == Cfg::kWarps) {
     if (lane == 0) {
-      // in the order of use: K0 K1 V0 K2 V1 ... where scores run ahead, else K0 V0 K1 V1 ...; K0 is under way
-      int armed = 1;
       bool ok = true;
-      auto load = [&](const CUtensorMap* map, int it) {
-        const int s = armed % NS;
-        if (!mbar_wait(empty(s), ((armed / NS) & 1) ^ 1, failed)) return false;
-        mbar_expect_tx(full(s), Cfg::kTileBytes);
-        for (int b = 0; b < Cfg::kBoxes; ++b)
-          tma_load_3d(smem_u32(ring + size_t(s) * Cfg::kTileBytes) + b * kBoxBytes, map, full(s), b * 64, kv_head,
-                      t.start + (n - 1 - it) * kTile);
-        ++armed;
-        return true;
-      };
-      if (Cfg::kOwnP) {
-        for (int it = 0; it < n && ok; ++it) {
-          if (it + 1 < n) ok = load(&map_k, it + 1);
-          if (ok) ok = load(&map_v, it);
-        }
-      } else {
-        for (int it = 0; it < n && ok; ++it) ok = (it == 0 || load(&map_k, it)) && load(&map_v, it);
+      while (armed < 2 * n) {
+        ok = mbar_wait(empty(armed % NS), ((armed / NS) & 1) ^ 1, failed);
+        if (!ok) break;
+        load();
       }
       if (!ok || *failed) {
         // copies in flight have to land before this shared memory goes away
@@ -374,47 +379,42 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         while (!mbar_try(bar_q, 0) && clock64() - t0 < kWaitLimitCycles) {}
       }
     }
-  } else if (warp == 9) {
-    // the whole warp walks along, lane 0 issues; `used` counts ring slots in the order of the loads
-    int used = 0;
-    bool ok = mbar_wait(bar_q, 0, failed);
-    auto scores = [&]() {
-      const int s = used % NS;
-      if (!mbar_wait(full(s), (used / NS) & 1, failed)) return false;
-      ++used;
-      if (elect_one()) {
-        mma_scores<DP, kTile>(tmem, smem_u32(smem_q), smem_u32(ring + size_t(s) * Cfg::kTileBytes));
-        umma_commit(empty(s));
-        umma_commit(bar_s);
-      }
-      __syncwarp();
-      return true;
+  } else if (warp == Cfg::kWarps + 1) {
+    const uint32_t tmem = tmem_base_s;
+    // the whole warp walks along, one lane issues; load 2 it is a key tile, 2 it + 1 a value tile
+    auto slot = [&](int load) { return ring + size_t(load % NS) * Cfg::kYBytes; };
+    auto arrived = [&](int load) { return mbar_wait(full(load % NS), (load / NS) & 1, failed); };
+    auto scores = [&](int it) {
+      mma_scores<DP, N>(tmem, smem_u32(smem_q), smem_u32(slot(2 * it)));
+      umma_commit(empty((2 * it) % NS));
+      umma_commit(bar_s);
     };
-    ok = ok && scores();
+    bool ok = mbar_wait(bar_q, 0, failed) && arrived(0);
+    if (ok && elect_one()) scores(0);
+    __syncwarp();
     for (int it = 0; it < n && ok; ++it) {
-      if (Cfg::kOwnP && it + 1 < n) {
-        ok = mbar_wait(bar_sfree, it & 1, failed);     // this tile's scores are in registers
-        fence_after_sync();
-        ok = ok && scores();
-        if (!ok) break;
-      }
-      const int s = used % NS;
-      ok = mbar_wait(full(s), (used / NS) & 1, failed);
+      const bool more = it + 1 < n;
+      ok = arrived(2 * it + 1);
       if (!ok) break;
-      ++used;
-      unsigned char* v = ring + size_t(s) * Cfg::kTileBytes;
       // P is zero behind the end of the sequence, which is not enough when the rows there hold infinities or NaN
-      if (it == 0 && t.len - row0 < kTile) zero_rows<DP, kTile>(v, t.len - row0);
-      ok = mbar_wait(bar_p, it & 1, failed);
+      const int left = t.len - key_tile(it) * N;
+      if (left < N) zero_rows<DP, N>(slot(2 * it + 1), left);
+      // the next keys have arrived long ago; looked at here, their barrier is not between P and the products
+      ok = (!more || NS == 2 || arrived(2 * it + 2)) && mbar_wait(bar_p, it & 1, failed);
       if (!ok) break;
       fence_after_sync();
       if (elect_one()) {
-        mma_accumulate<DP, kTile>(tmem + Cfg::kColO, tmem + Cfg::kColP, 16, smem_u32(v), it == 0);
-        umma_commit(empty(s));
+        mma_accumulate<DP, N>(tmem + Cfg::kColO, tmem, 16, smem_u32(slot(2 * it + 1)), it == 0);
+        umma_commit(empty((2 * it + 1) % NS));
         umma_commit(bar_pv);
+        if (more && NS > 2) scores(it + 1);            // over P: products run in the order of issue
       }
       __syncwarp();
-      if (!Cfg::kOwnP && it + 1 < n) ok = scores();    // over P: products run in the order of issue
+      if (more && NS == 2) {                           // two slots: these keys could only be loaded after the scores before
+        ok = arrived(2 * it + 2);
+        if (ok && elect_one()) scores(it + 1);
+        __syncwarp();
+      }
     }
     if (!ok || *failed) {
       if (elect_one()) {
@@ -425,11 +425,14 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       __syncwarp();
     }
   } else {
+    const uint32_t tmem = tmem_base_s;
     const int half = warp >> 2;                        // columns 64 half .. 64 half + 63
     const int row = (warp & 3) * 32 + lane;
     const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
-    const uint32_t tS = tmem + lanes + half * 64, tO = tmem + lanes + Cfg::kColO + half * (DP / 2), tP = tmem + lanes + Cfg::kColP + half * 32;
-    auto pair_sync = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 3)) : "memory"); };   // the two warps of 32 rows
+    const uint32_t tS = tmem + lanes + half * 64, tO = tmem + lanes + Cfg::kColO + half * (DP / H), tP = tmem + lanes + half * 32;
+    // the two warps of 32 rows
+    auto pair_sync = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 3)) : "memory"); };
+    const float2_t scale2 = pair(scale_log2, scale_log2);
     float m = 0.f, l = 0.f;
     bool ok = true;
     for (int it = 0; it < n; ++it) {
@@ -443,15 +446,11 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       tmem_wait_ld();
       tie32(r);
       tie32(r + 32);
-      if (Cfg::kOwnP) {
-        fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar_sfree);
-      }
-      if (it == 0) {
+      if (it < diagonal) {
+        const int last = row - it * N - half * 64;     // last column that this row sees
 #pragma unroll
         for (int c = 0; c < 64; ++c)
-          if (half * 64 + c > row) r[c] = 0xff800000u;             // -inf
+          if (c > last) r[c] = 0xff800000u;            // -inf
       }
       float mx[4];
 #pragma unroll
@@ -461,25 +460,25 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
 #pragma unroll
         for (int k = 0; k < 4; ++k) mx[k] = max3_nan(mx[k], __uint_as_float(r[c + k]), __uint_as_float(r[c + k + 4]));
       float top = max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3]));
-      // two sets of cells in turn: a thread is at most one tile ahead of its partner
-      maxima[it & 1][half][row] = top;
-      pair_sync();
-      top = max_nan(top, maxima[it & 1][half ^ 1][row]);
+      if (H == 2) {
+        // two sets of cells in turn: a thread is at most one tile ahead of its partner.  P may replace the scores afterwards.
+        maxima[it & 1][half][row] = top;
+        pair_sync();
+        top = max_nan(top, maxima[it & 1][half ^ (H - 1)][row]);
+      }
       if (it == 0) {
         m = top;
       } else {
         const bool grown = !((top - m) * scale_log2 <= 8.f);
         if (__any_sync(0xffffffffu, grown)) {
-          // rare; the product before has to be complete.  A row that did not grow keeps its reference, so that its bits do
-          // not depend on what the warp's other rows hold.
-          ok = mbar_wait(bar_pv, (it - 1) & 1, failed) && ok;
+          // rare.  The product before these scores is complete.  A row that did not grow keeps its reference, so that its
+          // bits do not depend on what the warp's other rows hold.
           const float next = grown ? max_nan(m, top) : m;
           const float f = ex2((m - (next == -INFINITY ? 0.f : next)) * scale_log2);
           m = next;
           l *= f;
-          fence_after_sync();
 #pragma unroll 1
-          for (int c = 0; c < DP / 2; c += 16) {
+          for (int c = 0; c < DP / H; c += 16) {
             uint32_t o[16];
             tmem_ld16(tO + c, o);
             tmem_wait_ld();
@@ -492,43 +491,51 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       }
       // a row whose scores are all -inf so far takes 0 as its reference: exp(-inf - 0) = 0 instead of NaN
       const float shift = m == -INFINITY ? 0.f : -m * scale_log2;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
-      uint32_t p[32];
+      const float2_t shift2 = pair(shift, shift);
+      float2_t sum[2] = {0ull, 0ull};
 #pragma unroll
-      for (int c = 0; c < 32; ++c) {
-        const float a = ex2(fmaf(__uint_as_float(r[2 * c]), scale_log2, shift));
-        const float b = ex2(fmaf(__uint_as_float(r[2 * c + 1]), scale_log2, shift));
-        sum[(2 * c) & 3] += a;
-        sum[(2 * c + 1) & 3] += b;
-        p[c] = pack_bf16(a, b);
+      for (int h = 0; h < 2; ++h) {
+        uint32_t p[16];
+#pragma unroll
+        for (int c = 0; c < 16; ++c) {
+          float a, b;
+          unpair(fma2(pair(__uint_as_float(r[h * 32 + 2 * c]), __uint_as_float(r[h * 32 + 2 * c + 1])), scale2, shift2), a, b);
+          a = ex2(a);
+          b = ex2(b);
+          sum[c & 1] = add2(sum[c & 1], pair(a, b));
+          p[c] = pack_bf16(a, b);
+        }
+        tmem_st16(tP + h * 16, p);
       }
-      if (Cfg::kOwnP && it > 0) ok = mbar_wait(bar_pv, (it - 1) & 1, failed) && ok;   // P has been read
-      tmem_st32(tP, p);
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      float lo, hi;
+      unpair(add2(sum[0], sum[1]), lo, hi);
+      l += lo + hi;
       tmem_wait_st();
       fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar_p);
     }
-    // the row's sum is in two places
-    maxima[n & 1][half][row] = l;
-    pair_sync();
-    l += maxima[n & 1][half ^ 1][row];
+    if (H == 2) {
+      // the row's sum is in two places
+      maxima[n & 1][half][row] = l;
+      pair_sync();
+      l += maxima[n & 1][half ^ (H - 1)][row];
+    }
     if (ok && mbar_wait(bar_pv, (n - 1) & 1, failed)) {
       fence_after_sync();
-      stage_rows<DP / 64>(tO, 1.f / l, smem_q, row, half * (DP / 16));
+      stage_rows<DP / H / 32>(tO, 1.f / l, smem_q, row, half * (DP / H / 8));
       __syncwarp();
       const int left = t.len - row0 - (row & ~31);
-      store_rows<DP / 16>(out, head, t.start + row0 + (row & ~31), left, g.dim, smem_q, row & ~31, half * (DP / 16));
+      store_rows<DP / H / 8>(out, head, t.start + row0 + (row & ~31), left, g.dim, smem_q, row & ~31, half * (DP / H / 8));
       if (stats != nullptr && half == 0)
         stats[((long long)head * g.tiles + t.slot) * kTile + row] = lane < left ? -fmaf(m, scale_log2, log2f(l)) : -INFINITY;
     }
   }
   fence_before_sync();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == Cfg::kWarps + 1) {
     fence_after_sync();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 256;" ::"r"(tmem) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base_s), "r"(Cfg::kCols) : "memory");
   }
   if (threadIdx.x == 0 && failed_s) atomicOr(status, kAttnTimeout);
 }
@@ -730,16 +737,13 @@ __device__ __forceinline__ void attn_bwd_body(const CUtensorMap* map_q, const CU
         tma_load_3d(dst, m0, bar_x, b * 64, own_head, t.start + row0 + h * 64);
         tma_load_3d(dst + Cfg::kXBytes, m1, bar_x, b * 64, own_head, t.start + row0 + h * 64);
       }
-    for (int it = 0; it < NS && it < n; ++it) load();
+    load();
   }
   if (warp == Cfg::kWarps + 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)), "r"(Cfg::kCols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  fence_before_sync();
-  __syncthreads();
-  fence_after_sync();
-  const uint32_t tmem = tmem_base_s;
+  set_up_done<Cfg::kThreads>(warp == Cfg::kWarps);
 
   if (warp == Cfg::kWarps) {
     if (lane == 0) {
@@ -760,6 +764,7 @@ __device__ __forceinline__ void attn_bwd_body(const CUtensorMap* map_q, const CU
       }
     }
   } else if (warp == Cfg::kWarps + 1) {
+    const uint32_t tmem = tmem_base_s;
     const uint32_t x0 = smem_u32(smem_x), x1 = x0 + Cfg::kXBytes;
     auto stage = [&](int it) { return ring + size_t(it % NS) * 2 * Cfg::kYBytes; };
     auto s_col = [&](int it) { return tmem + uint32_t(it % SETS) * 128u; };
@@ -819,6 +824,7 @@ __device__ __forceinline__ void attn_bwd_body(const CUtensorMap* map_q, const CU
     }
     __syncwarp();
   } else {
+    const uint32_t tmem = tmem_base_s;
     const int set = warp >> 3, half = (warp >> 2) & 1;
     const int row = (warp & 3) * 32 + lane;
     const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
@@ -982,7 +988,7 @@ __device__ __forceinline__ void attn_bwd_body(const CUtensorMap* map_q, const CU
   __syncthreads();
   if (warp == Cfg::kWarps + 1) {
     fence_after_sync();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Cfg::kCols) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base_s), "r"(Cfg::kCols) : "memory");
   }
   if (threadIdx.x == 0 && failed_s) atomicOr(status, kAttnTimeout);
 }
@@ -1127,9 +1133,10 @@ cudaError_t LaunchAttnForward(const AttnShape& s, const AttnTensor& q, const Att
   if (!AttnSupported(s) || !Addressable(q) || !Addressable(k) || !Addressable(v) || !Addressable(out) || status == nullptr)
     return cudaErrorInvalidValue;
   const long long tokens = s.cu == nullptr ? s.batch * s.seq : s.seq;
+  const int keys = s.dim <= 64 ? FwdCfg<64>::kN : FwdCfg<128>::kN;
   CUtensorMap mq, mk, mv;
-  if (!MakeMap(&mq, q, s.heads, s.dim, tokens, kTile) || !MakeMap(&mk, k, s.kv_heads, s.dim, tokens, kTile) ||
-      !MakeMap(&mv, v, s.kv_heads, s.dim, tokens, kTile))
+  if (!MakeMap(&mq, q, s.heads, s.dim, tokens, kTile) || !MakeMap(&mk, k, s.kv_heads, s.dim, tokens, keys) ||
+      !MakeMap(&mv, v, s.kv_heads, s.dim, tokens, keys))
     return cudaErrorInvalidValue;
   return s.dim <= 64 ? Forward<64>(s, mq, mk, mv, out, stats, status, stream) : Forward<128>(s, mq, mk, mv, out, stats, status, stream);
 }
