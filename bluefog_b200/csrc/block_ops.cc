@@ -273,6 +273,12 @@ at::Tensor GatedProduct(const at::Tensor& a, const at::Tensor& w_gate_up, int64_
 }
 at::Tensor DownProduct(const at::Tensor& h, const at::Tensor& w_down, const at::Tensor& residual) {
   at::Tensor y = at::empty({h.size(0), w_down.size(0)}, h.options());
+  if (h.size(0) <= kSkinnyRows) {
+    Check(LaunchGemmBf16FewRows(h.data_ptr(), w_down.data_ptr(), y.data_ptr(), static_cast<int>(h.size(0)), static_cast<int>(w_down.size(0)),
+                                static_cast<int>(h.size(1)), GemmStatus(h), StreamOf(h), residual.defined() ? residual.data_ptr() : nullptr),
+          "gated_mlp");
+    return y;
+  }
   Check(LaunchGemmBf16NT(h.data_ptr(), w_down.data_ptr(), y.data_ptr(), nullptr, static_cast<int>(h.size(0)), static_cast<int>(w_down.size(0)),
                          static_cast<int>(h.size(1)), kActNone, GemmStatus(h), StreamOf(h), nullptr, nullptr,
                          residual.defined() ? residual.data_ptr() : nullptr), "gated_mlp");

@@ -922,6 +922,174 @@ gemm_bf16_nt_persistent_kernel(const __grid_constant__ CUtensorMap map_a, const 
   if (threadIdx.x == 0 && failed_s && status != nullptr) atomicExch(status, 1u);
 }
 
+// ------------------------------------------------------------------------------------------ //
+// Few rows: out[M, N] = x[M, K] w[N, K]^T with M <= 64, where the weights are what is read (8 x 1024 x 2752: 17 MB, 2.6 us from
+// memory).  The roles are swapped - 128 weight rows are the M side of the MMA, NB >= M tokens its N side - so that a CTA reads
+// weights only once, and a cluster of `split` CTAs shares a tile's reduction so that all SMs read: with 128 x 256 tiles of
+// the kernel above the two products of that block kept 22 and 4 SMs busy and took 13 and 28 us.  The partial tiles meet in
+// distributed shared memory; every CTA adds up the cluster's sums for its share of the tokens, in the order of the slices.
+// GATED: 64 gate and 64 up rows make a tile, and act(g) u leaves (g and u themselves too when `pre` is given).
+// ------------------------------------------------------------------------------------------ //
+template <int NB>
+struct SkinnyCfg {
+  static constexpr int kStagesS = 4;
+  static constexpr uint32_t kBytesA = 128 * BK * 2;
+  static constexpr uint32_t kBytesB = NB * BK * 2;
+  static constexpr uint32_t kColsT = NB < 32 ? 32 : NB;
+  static constexpr size_t kSmem = 1024 + kStagesS * (kBytesA + kBytesB) + NB * 128 * 4;
+};
+
+template <int NB, bool GATED>
+__global__ void __launch_bounds__(192)
+gemm_bf16_skinny_kernel(const __grid_constant__ CUtensorMap map_lo, const __grid_constant__ CUtensorMap map_hi,
+                        const __grid_constant__ CUtensorMap map_x, __nv_bfloat16* __restrict__ out, __nv_bfloat16* __restrict__ pre,
+                        const __nv_bfloat16* __restrict__ residual, const int M, const int N, const int num_kb, const int split, const int act,
+                        unsigned int* __restrict__ status) {
+  using Cfg = SkinnyCfg<NB>;
+  constexpr int S = Cfg::kStagesS;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  unsigned char* stage_b = smem + S * Cfg::kBytesA;
+  float* sums = reinterpret_cast<float*>(stage_b + S * Cfg::kBytesB);          // [token][weight row of the tile]
+  __shared__ uint64_t bars[2 * S + 1];
+  __shared__ uint32_t tmem_base_s;
+  __shared__ int failed_s;
+  volatile int* failed = &failed_s;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = blockIdx.x % split, n0 = (blockIdx.x / split) * (GATED ? 64 : 128);
+  const int kb0 = rank * num_kb / split, kb1 = (rank + 1) * num_kb / split;
+
+  if (threadIdx.x == 0) {
+    failed_s = 0;
+    for (int i = 0; i < 2 * S + 1; ++i) mbar_init(smem_u32(&bars[i]), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)), "r"(Cfg::kColsT) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  const uint32_t tmem = tmem_base_s;
+  bool ok = true;
+  if (warp == 0) {
+    if (lane == 0) {
+      int armed = 0;
+      for (int kb = kb0; kb < kb1; ++kb, ++armed) {
+        const int s = armed % S;
+        ok = mbar_wait(smem_u32(&bars[S + s]), ((armed / S) & 1) ^ 1, failed);
+        if (!ok) break;
+        const uint32_t full = smem_u32(&bars[s]), a = smem_u32(smem + s * Cfg::kBytesA);
+        mbar_expect_tx(full, Cfg::kBytesA + Cfg::kBytesB);
+        tma_load_2d(a, &map_lo, full, kb * BK, n0);
+        tma_load_2d(a + Cfg::kBytesA / 2, &map_hi, full, kb * BK, GATED ? n0 : n0 + 64);
+        tma_load_2d(smem_u32(stage_b + s * Cfg::kBytesB), &map_x, full, kb * BK, 0);
+      }
+      if (!ok || *failed) {
+        for (int f = armed > S ? armed - S : 0; f < armed; ++f) {
+          const unsigned long long t0 = now_ns();
+          while (!mbar_try(smem_u32(&bars[f % S]), (f / S) & 1) && now_ns() - t0 < kWaitLimitNs) {}
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(NB >> 3) << 17) | (uint32_t(128 >> 4) << 24);
+    for (int i = 0; i < kb1 - kb0 && ok; ++i) {
+      const int s = i % S;
+      ok = mbar_wait(smem_u32(&bars[s]), (i / S) & 1, failed);
+      if (!ok) break;
+      if (elect_one()) {
+        const uint64_t a = make_desc(smem_u32(smem + s * Cfg::kBytesA)), b = make_desc(smem_u32(stage_b + s * Cfg::kBytesB));
+#pragma unroll
+        for (int k = 0; k < BK / kUmmaK; ++k) umma_f16(tmem, a + uint64_t(2 * k), b + uint64_t(2 * k), idesc, (i | k) != 0 ? 1u : 0u);
+        umma_commit(smem_u32(&bars[S + s]));
+      }
+      __syncwarp();
+    }
+    // also after a failure, so that tensor memory is not freed under a product
+    if (elect_one()) umma_commit(smem_u32(&bars[2 * S]));
+    __syncwarp();
+    if (!ok) {
+      const unsigned long long t0 = now_ns();
+      while (!mbar_try(smem_u32(&bars[2 * S]), 0) && now_ns() - t0 < kWaitLimitNs) {}
+    }
+  } else {
+    const int row = (warp & 3) * 32 + lane;
+    ok = mbar_wait(smem_u32(&bars[2 * S]), 0, failed);
+    fence_after_sync();
+    const uint32_t t = tmem + (uint32_t((warp & 3) * 32) << 16);
+#pragma unroll
+    for (int c = 0; c < NB; c += 16) {
+      uint32_t r[16];
+      tmem_ld16(t + c, r);
+      tmem_wait_ld();
+      tie16(r);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sums[(c + i) * 128 + row] = kb1 > kb0 ? __uint_as_float(r[i]) : 0.f;
+    }
+  }
+  __syncwarp();
+  if (split > 1) {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  } else {
+    __syncthreads();
+  }
+  if (warp >= 2 && ok) {
+    const int e = threadIdx.x - 64;
+    auto total = [&](int at) {
+      float v[8];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        v[c] = 0.f;
+        if (c < split) {
+          const uint32_t addr = mapa_u32(smem_u32(sums + at), c);
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[c]) : "r"(addr) : "memory");
+        }
+      }
+#pragma unroll
+      for (int c = 1; c < 8; ++c) v[0] += v[c];
+      return v[0];
+    };
+    const int first = rank * (NB / split), last = min(first + NB / split, M);
+    if (GATED) {
+      const int f = n0 + (e & 63);
+      for (int t = first + (e >> 6); t < last; t += 2) {
+        const float g = total(t * 128 + (e & 63)), u = total(t * 128 + 64 + (e & 63));
+        if (f < N) {
+          out[size_t(t) * N + f] = __float2bfloat16_rn(gate_fn(g, act, nullptr) * u);
+          if (pre != nullptr) {
+            pre[size_t(t) * (2 * N) + f] = __float2bfloat16_rn(g);
+            pre[size_t(t) * (2 * N) + N + f] = __float2bfloat16_rn(u);
+          }
+        }
+      }
+    } else {
+      const int n = n0 + e;
+      for (int t = first; t < last; ++t) {
+        const float v = total(t * 128 + e);
+        if (n < N) out[size_t(t) * N + n] = __float2bfloat16_rn(v + (residual != nullptr ? __bfloat162float(residual[size_t(t) * N + n]) : 0.f));
+      }
+    }
+  }
+  __syncwarp();
+  if (split > 1) {
+    // nobody leaves while another may still read its shared memory
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
+  fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    fence_after_sync();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Cfg::kColsT) : "memory");
+  }
+  if (threadIdx.x == 0 && failed_s && status != nullptr) atomicExch(status, 1u);
+}
+
 // pitch: elements from row to row (0: the rows follow one another); boxes of 64 columns in the 128-byte swizzle, of 32 in the 64-byte one
 bool MakeMap(CUtensorMap* map, const void* base, int rows, int cols /*K*/, int box_rows, long long pitch = 0, int box_cols = BK) {
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
@@ -1004,7 +1172,70 @@ int SmCount() {
   return sm_count;
 }
 
+template <int NB, bool GATED>
+cudaError_t LaunchSkinny(const CUtensorMap& lo, const CUtensorMap& hi, const CUtensorMap& x, __nv_bfloat16* out, __nv_bfloat16* pre,
+                         const __nv_bfloat16* residual, int M, int N, int K, int act, unsigned int* status, cudaStream_t stream) {
+  using Cfg = SkinnyCfg<NB>;
+  auto kernel = gemm_bf16_skinny_kernel<NB, GATED>;
+  constexpr int kMaxDevices = 64;
+  static bool attr_set[kMaxDevices] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev >= kMaxDevices || !attr_set[dev]) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Cfg::kSmem));
+    if (e != cudaSuccess) return e;
+    if (dev < kMaxDevices) attr_set[dev] = true;
+  }
+  // as many slices of the reduction as give most SMs a CTA, of one 64-column block at least
+  const int width = GATED ? 64 : 128, tiles = (N + width - 1) / width, num_kb = (K + BK - 1) / BK;
+  int split = 1;
+  while (split < 8 && 2 * split <= num_kb && 2 * tiles * split <= 2 * SmCount()) split *= 2;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles) * split);
+  cfg.blockDim = dim3(192);
+  cfg.dynamicSmemBytes = Cfg::kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = split;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, lo, hi, x, out, pre, residual, M, N, num_kb, split, act, status);
+}
+
+// N: output columns (GATED: of the gated product, w holds 2 N rows)
+template <bool GATED>
+cudaError_t Skinny(const void* x, const void* w, void* out, void* pre, const void* residual, int M, int N, int K, int act, unsigned int* status,
+                   cudaStream_t stream) {
+  (void)cudaGetLastError();   // the value returned below must be this launch's own, not an older error of the calling thread
+  const uintptr_t all = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(out) |
+                        reinterpret_cast<uintptr_t>(pre) | reinterpret_cast<uintptr_t>(residual);
+  if (M <= 0 || M > kSkinnyRows || N <= 0 || K <= 0 || (K % 8) != 0 || (N % 8) != 0 || (all & 15) != 0) return cudaErrorInvalidValue;
+  const int nb = M <= 16 ? 16 : M <= 32 ? 32 : 64;
+  CUtensorMap lo, hi, mx;
+  if (!MakeMap(&lo, w, N, K, 64) || !MakeMap(&mx, x, M, K, nb)) return cudaErrorInvalidValue;
+  hi = lo;
+  if (GATED && !MakeMap(&hi, static_cast<const __nv_bfloat16*>(w) + size_t(N) * K, N, K, 64)) return cudaErrorInvalidValue;
+  __nv_bfloat16* o = static_cast<__nv_bfloat16*>(out);
+  __nv_bfloat16* p = static_cast<__nv_bfloat16*>(pre);
+  const __nv_bfloat16* r = static_cast<const __nv_bfloat16*>(residual);
+  const cudaError_t e = nb == 16   ? LaunchSkinny<16, GATED>(lo, hi, mx, o, p, r, M, N, K, act, status, stream)
+                        : nb == 32 ? LaunchSkinny<32, GATED>(lo, hi, mx, o, p, r, M, N, K, act, status, stream)
+                                   : LaunchSkinny<64, GATED>(lo, hi, mx, o, p, r, M, N, K, act, status, stream);
+  if (e != cudaSuccess) return e;
+  CountKernelLaunch();
+  return cudaGetLastError();
+}
+
 }  // namespace
+
+cudaError_t LaunchGemmBf16FewRows(const void* a, const void* b, void* out, int M, int N, int K, unsigned int* status, cudaStream_t stream,
+                                  const void* addend) {
+  return Skinny<false>(a, b, out, nullptr, addend, M, N, K, kActNone, status, stream);
+}
 
 bool GemmSupported() { return GetEncodeFn() != nullptr; }
 
@@ -1155,6 +1386,7 @@ cudaError_t LaunchGemmBf16Gated(const void* a, const void* w, void* h, void* pre
   if ((reinterpret_cast<uintptr_t>(a) & 15) || (reinterpret_cast<uintptr_t>(w) & 15) || (reinterpret_cast<uintptr_t>(h) & 15) ||
       (reinterpret_cast<uintptr_t>(preact) & 15))
     return cudaErrorInvalidValue;
+  if (M <= kSkinnyRows) return Skinny<true>(a, w, h, preact, nullptr, M, F, K, act, status, stream);
   const int sm_count = SmCount();
   const __nv_bfloat16* wu = static_cast<const __nv_bfloat16*>(w) + size_t(F) * K;
   __nv_bfloat16* pre = static_cast<__nv_bfloat16*>(preact);

@@ -39,6 +39,12 @@ cudaError_t LaunchGemmBf16NN(const void* a, const void* b, void* out, int M, int
 cudaError_t LaunchGemmBf16TN(const void* a, const void* b, void* out, int M, int N, int K, unsigned int* status,
                              cudaStream_t stream);
 
+// out[M,N] = a[M,K] * b[N,K]^T (+ addend[M,N]) for at most kSkinnyRows rows, the reduction shared by clusters of CTAs; K % 8 == 0,
+// N % 8 == 0.
+constexpr int kSkinnyRows = 64;
+cudaError_t LaunchGemmBf16FewRows(const void* a, const void* b, void* out, int M, int N, int K, unsigned int* status, cudaStream_t stream,
+                                  const void* addend = nullptr);
+
 // h[M,F] = act(a[M,K] * w[0:F,K]^T) * (a * w[F:2F,K]^T), act kActSilu or kActGeluTanh; K % 8 == 0, F % 8 == 0.  preact
 // (optional, [M,2F]): receives both products before the activation.
 cudaError_t LaunchGemmBf16Gated(const void* a, const void* w, void* h, void* preact, int M, int F, int K, int act,
