@@ -262,32 +262,26 @@ struct DropoutNode : public torch::autograd::Function<DropoutNode> {
 
 unsigned int* GemmStatus(const at::Tensor& like) { return reinterpret_cast<unsigned int*>(GemmStatusWord(like).data_ptr()); }
 
-at::Tensor GatedProduct(const at::Tensor& a, const at::Tensor& w_gate_up, int64_t act, at::Tensor* pre) {
+at::Tensor GatedProduct(const at::Tensor& a, const at::Tensor& w_gate_up, int64_t act, at::Tensor* factors) {
   const int64_t m = a.size(0), f = w_gate_up.size(0) / 2;
   at::Tensor h = at::empty({m, f}, a.options());
-  if (pre != nullptr) *pre = at::empty({m, 2 * f}, a.options());
-  Check(LaunchGemmBf16Gated(a.data_ptr(), w_gate_up.data_ptr(), h.data_ptr(), pre != nullptr ? pre->data_ptr() : nullptr, static_cast<int>(m),
+  if (factors != nullptr) *factors = at::empty({m, 2 * f}, a.options().dtype(at::kShort));
+  Check(LaunchGemmBf16Gated(a.data_ptr(), w_gate_up.data_ptr(), h.data_ptr(), factors != nullptr ? factors->data_ptr() : nullptr, static_cast<int>(m),
                             static_cast<int>(f), static_cast<int>(a.size(1)), static_cast<int>(act), GemmStatus(a), StreamOf(a)),
         "gated_mlp");
   return h;
 }
 at::Tensor DownProduct(const at::Tensor& h, const at::Tensor& w_down, const at::Tensor& residual) {
   at::Tensor y = at::empty({h.size(0), w_down.size(0)}, h.options());
-  if (h.size(0) <= kSkinnyRows) {
-    Check(LaunchGemmBf16FewRows(h.data_ptr(), w_down.data_ptr(), y.data_ptr(), static_cast<int>(h.size(0)), static_cast<int>(w_down.size(0)),
-                                static_cast<int>(h.size(1)), GemmStatus(h), StreamOf(h), residual.defined() ? residual.data_ptr() : nullptr),
-          "gated_mlp");
-    return y;
-  }
-  Check(LaunchGemmBf16NT(h.data_ptr(), w_down.data_ptr(), y.data_ptr(), nullptr, static_cast<int>(h.size(0)), static_cast<int>(w_down.size(0)),
-                         static_cast<int>(h.size(1)), kActNone, GemmStatus(h), StreamOf(h), nullptr, nullptr,
-                         residual.defined() ? residual.data_ptr() : nullptr), "gated_mlp");
+  Check(LaunchGemmGatedDown(h.data_ptr(), w_down.data_ptr(), y.data_ptr(), static_cast<int>(h.size(0)), static_cast<int>(w_down.size(0)),
+                            static_cast<int>(h.size(1)), GemmStatus(h), StreamOf(h), residual.defined() ? residual.data_ptr() : nullptr),
+        "gated_mlp");
   return y;
 }
 // a^T b of two matrices with the same rows: a weight's gradient
 at::Tensor TransposedProduct(const at::Tensor& a, const at::Tensor& b) {
   at::Tensor out = at::empty({a.size(1), b.size(1)}, a.options());
-  Check(LaunchGemmBf16TN(a.data_ptr(), b.data_ptr(), out.data_ptr(), static_cast<int>(a.size(1)), static_cast<int>(b.size(1)),
+  Check(LaunchGemmGatedWeight(a.data_ptr(), b.data_ptr(), out.data_ptr(), static_cast<int>(a.size(1)), static_cast<int>(b.size(1)),
                          static_cast<int>(a.size(0)), GemmStatus(a), StreamOf(a)), "gated_mlp backward");
   return out;
 }
@@ -298,35 +292,34 @@ std::vector<int64_t> WithColumns(const at::Tensor& a, int64_t columns) {
   return s;
 }
 
-// Kept for the backward pass: both pre-activations and their gated product, rounded to bf16 like every activation.
+// Kept for the backward pass: the gated product in bf16 like every activation, and the two factors of its gradient in 16 bits each.
 struct GatedMlpNode : public torch::autograd::Function<GatedMlpNode> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& a0, const at::Tensor& wgu0, const at::Tensor& wd0, int64_t act,
                             const c10::optional<at::Tensor>& residual) {
     const at::Tensor a = Rows2d(a0), wgu = Dense(wgu0), wd = Dense(wd0);
-    at::Tensor pre;
-    const at::Tensor h = GatedProduct(a, wgu, act, &pre);
+    at::Tensor factors;
+    const at::Tensor h = GatedProduct(a, wgu, act, &factors);
     at::Tensor y = DownProduct(h, wd, residual.has_value() ? Rows2d(*residual) : at::Tensor());
-    ctx->save_for_backward({a, wgu, wd, pre, h});
+    ctx->save_for_backward({a, wgu, wd, factors, h});
     ctx->saved_data["residual"] = residual.has_value();
-    ctx->saved_data["act"] = act;
     ctx->saved_data["sizes"] = a0.sizes().vec();
     return y.view(WithColumns(a0, wd.size(0)));
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list saved = ctx->get_saved_variables();
-    const at::Tensor &a = saved[0], &wgu = saved[1], &wd = saved[2], &pre = saved[3], &h = saved[4];
+    const at::Tensor &a = saved[0], &wgu = saved[1], &wd = saved[2], &factors = saved[3], &h = saved[4];
     const c10::cuda::CUDAGuard guard(a.get_device());
     const at::Tensor dy = Rows2d(grads[0]);
     const int m = static_cast<int>(a.size(0)), f = static_cast<int>(h.size(1)), k = static_cast<int>(a.size(1));
     at::Tensor da, dwgu, dwd;
     if (ctx->needs_input_grad(0) || ctx->needs_input_grad(1)) {
       // [dG dU] straight from the epilogue of dH = dy Wd
-      at::Tensor dpre = at::empty(pre.sizes(), pre.options());
-      Check(LaunchGemmBf16NNGatedGrad(dy.data_ptr(), wd.data_ptr(), pre.data_ptr(), dpre.data_ptr(), m, f, static_cast<int>(wd.size(0)),
-                                      static_cast<int>(ctx->saved_data["act"].toInt()), GemmStatus(a), StreamOf(a)), "gated_mlp backward");
+      at::Tensor dpre = at::empty(factors.sizes(), a.options());
+      Check(LaunchGemmBf16NNGatedGrad(dy.data_ptr(), wd.data_ptr(), factors.data_ptr(), dpre.data_ptr(), m, f, static_cast<int>(wd.size(0)),
+                                      GemmStatus(a), StreamOf(a)), "gated_mlp backward");
       if (ctx->needs_input_grad(0)) {
         da = at::empty(a.sizes(), a.options());
-        Check(LaunchGemmBf16NN(dpre.data_ptr(), wgu.data_ptr(), da.data_ptr(), m, k, 2 * f, GemmStatus(a), StreamOf(a)), "gated_mlp backward");
+        Check(LaunchGemmGatedInput(dpre.data_ptr(), wgu.data_ptr(), da.data_ptr(), m, k, 2 * f, GemmStatus(a), StreamOf(a)), "gated_mlp backward");
         da = da.view(ctx->saved_data["sizes"].toIntVector());
       }
       if (ctx->needs_input_grad(1)) dwgu = TransposedProduct(dpre, a);

@@ -30,6 +30,7 @@
 
 #include <cstdlib>
 #include <string>
+#include <type_traits>
 
 #include "gemm_tcgen05.h"
 #include "tcgen05_common.cuh"
@@ -121,6 +122,24 @@ __device__ __forceinline__ float gate_fn(float x, int act, float* grad) {
   if (grad != nullptr) *grad = s + y * (1.f - s) * dw;
   return y;
 }
+// What a gated block keeps for its backward pass, 16 bits each: act(g) and u act'(g), the factors of dH in dU and dG.  Their format
+// has a sign, six bits of exponent (2^-30 to 2^32, smaller values become zero, larger ones the largest) and nine of mantissa:
+// each is off by at most 2^-10 of itself.  Kept in bf16, their rounding, that of dG and dU and that of the gradients
+// themselves made the gradients of the input and of the gate and up weights 1.8 times as far from exact ones as the last
+// rounding alone does; now it is 1.4 times.  Scaled by 2^-96 the exponent of an fp32 number has two leading zeros.
+constexpr float kFactorScale = 1.262177448353618888658765704452e-29f;          // 2^-96
+__device__ __forceinline__ uint32_t pack_factors(float lo, float hi) {
+  const uint32_t a = __float_as_uint(lo * kFactorScale), b = __float_as_uint(hi * kFactorScale);
+  const uint32_t ma = min((a & 0x7fffffffu) + 0x2000u, 0x1fffffffu) >> 14, mb = min((b & 0x7fffffffu) + 0x2000u, 0x1fffffffu) >> 14;
+  return ((a >> 16) & 0x8000u) | ma | (b & 0x80000000u) | (mb << 16);
+}
+// The factors in a word, times 2^-96.
+__device__ __forceinline__ float2 unpack_factors(uint32_t w) {
+  return make_float2(__uint_as_float(((w << 16) & 0x80000000u) | ((w << 14) & 0x1fffc000u)),
+                     __uint_as_float((w & 0x80000000u) | ((w >> 2) & 0x1fffc000u)));
+}
+constexpr float kFactorUnscale = 7.9228162514264337593543950336e28f;           // 2^96
+
 // eight floats as bf16, 16 bytes
 __device__ __forceinline__ uint4 pack8(const float* v) {
   uint4 pk;
@@ -455,7 +474,8 @@ gemm_bf16_nt_persistent_kernel(const __grid_constant__ CUtensorMap map_a, const 
       }
     }
   } else if (warp == 1) {
-    if (lane == 0 && leader) {
+    // the whole warp walks along, one elected lane issues: its descriptors then stay in uniform registers (see elect_one)
+    if (leader) {
       int it = 0, local = 0;
       bool ok = true;
       for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step, ++local) {
@@ -478,33 +498,37 @@ gemm_bf16_nt_persistent_kernel(const __grid_constant__ CUtensorMap map_a, const 
           constexpr uint32_t idesc = Cfg::kIdesc | (AMODE != 0 ? (1u << 15) : 0u) | (BMODE != 0 ? (1u << 16) : 0u);
           constexpr uint64_t a_step = AMODE == 0 ? 2 : (16 * 128) >> 4;
           constexpr uint64_t b_step = BMODE == 0 ? 2 : (16 * 128) >> 4;
+          if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < BK / kUmmaK; ++k) {
-            if (PAIR) {
-              asm volatile(
-                  "{\n\t.reg .pred p;\n\t"
-                  "setp.ne.b32 p, %4, 0;\n\t"
-                  "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5, %5, %5, %5, %5}, p;\n\t}"
-                  ::"r"(tmem_d), "l"(adesc + a_step * uint64_t(k)), "l"(bdesc + b_step * uint64_t(k)), "r"(idesc),
-                    "r"((kb | k) != 0 ? 1u : 0u), "r"(0u)
-                  : "memory");
-            } else {
-              asm volatile(
-                  "{\n\t.reg .pred p;\n\t"
-                  "setp.ne.b32 p, %4, 0;\n\t"
-                  "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                  ::"r"(tmem_d), "l"(adesc + a_step * uint64_t(k)), "l"(bdesc + b_step * uint64_t(k)), "r"(idesc),
-                    "r"((kb | k) != 0 ? 1u : 0u)
-                  : "memory");
+            for (int k = 0; k < BK / kUmmaK; ++k) {
+              if (PAIR) {
+                asm volatile(
+                    "{\n\t.reg .pred p;\n\t"
+                    "setp.ne.b32 p, %4, 0;\n\t"
+                    "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5, %5, %5, %5, %5}, p;\n\t}"
+                    ::"r"(tmem_d), "l"(adesc + a_step * uint64_t(k)), "l"(bdesc + b_step * uint64_t(k)), "r"(idesc),
+                      "r"((kb | k) != 0 ? 1u : 0u), "r"(0u)
+                    : "memory");
+              } else {
+                asm volatile(
+                    "{\n\t.reg .pred p;\n\t"
+                    "setp.ne.b32 p, %4, 0;\n\t"
+                    "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                    ::"r"(tmem_d), "l"(adesc + a_step * uint64_t(k)), "l"(bdesc + b_step * uint64_t(k)), "r"(idesc),
+                      "r"((kb | k) != 0 ? 1u : 0u)
+                    : "memory");
+              }
             }
+            if (PAIR) umma_commit_pair(smem_u32(&bars[S + s]));
+            else umma_commit(smem_u32(&bars[S + s]));
           }
-          if (PAIR) umma_commit_pair(smem_u32(&bars[S + s]));
-          else umma_commit(smem_u32(&bars[S + s]));
+          __syncwarp();
         }
-        if (ok) {
+        if (ok && elect_one()) {
           if (PAIR) umma_commit_pair(smem_u32(&bars[2 * S + acc]));
           else umma_commit(smem_u32(&bars[2 * S + acc]));
         }
+        __syncwarp();
       }
     }
   } else {
@@ -546,8 +570,8 @@ gemm_bf16_nt_persistent_kernel(const __grid_constant__ CUtensorMap map_a, const 
       for (int i = lane; i < 2 * BN_; i += 32) wstat[i] = 0.f;
       __syncwarp();
     }
-    // kEpiGatedGrad: the kept g and u come through TMA boxes of 32 rows x 32 columns, one chunk ahead, into two sets of a g and a u
-    // box per warp; dG and dU replace them there and leave from there.  (Read by the threads row by row, 32 sectors per load,
+    // kEpiGatedGrad: the kept factors come through TMA boxes of 32 rows x 32 columns, one chunk ahead, into two sets of a box for
+    // each per warp; dU and dG replace them there and leave from there.  (Read by the threads row by row, 32 sectors per load,
     // the epilogue took four times as long as the main loop of a reduction of 1024.)
     constexpr int kParts = Cfg::kTileN / 32 / (Cfg::kEpiWarps == 8 ? 2 : 1);
     const int part_first = Cfg::kEpiWarps == 8 ? (ew >> 2) * kParts : 0;
@@ -587,50 +611,60 @@ gemm_bf16_nt_persistent_kernel(const __grid_constant__ CUtensorMap map_a, const 
         }
       }
       if constexpr (EPI == kEpiGated) {
-        // h = act(g) u from the fp32 accumulators; g and u leave too (rounded, for the backward pass) when tma_out is 2.
-        // Their boxes take turns in the warp's two staging buffers.
+        // h = act(g) u from the fp32 accumulators; act(g) and u act'(g) leave too when tma_out is 2.  Boxes of 32 rows x 32 columns,
+        // one for each of the three per warp: they are written when the chunk is computed, so their last stores had that long
+        // to be read (boxes of 64 columns in turn in two buffers: 93 instead of 80 us for 8192 x 1024 x 2752).
 #pragma unroll 1
-        for (int c = c_first; c < c_first + kChunksW; ++c) {
-          const int nbase = n0 + c * 64;
+        for (int c = part_first; c < part_first + kParts; ++c) {
+          const int nbase = n0 + c * 32;
           if (nbase >= N || m0 + q * 32 >= M) break;           // warp-uniform
-          const uint32_t taddr = tmem_base + (uint32_t(q * 32) << 16) + uint32_t(acc * BN_ + c * 64);
-          uint32_t g[64], u[64];
+          const uint32_t taddr = tmem_base + (uint32_t(q * 32) << 16) + uint32_t(acc * BN_ + c * 32);
+          uint32_t g[32], u[32], f[16], d[16];
           tmem_ld32(taddr, g);
-          tmem_ld32(taddr + 32, g + 32);
           tmem_ld32(taddr + BN_ / 2, u);
-          tmem_ld32(taddr + BN_ / 2 + 32, u + 32);
           tmem_wait_ld();
           tie32(g);
-          tie32(g + 32);
           tie32(u);
-          tie32(u + 32);
-          auto leave = [&](const CUtensorMap* map, auto&& value) {
-            if (lane == 0) tma_store_wait_read<1>();           // the box written two stores ago has been read
-            __syncwarp();
-            unsigned char* box = my_out + size_t(boxes & 1) * Cfg::kBytesOutBox;
+          auto put = [&](int box, const uint32_t* v) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              float v[8];
-#pragma unroll
-              for (int i = 0; i < 8; ++i) v[i] = value(j * 8 + i);
-              *reinterpret_cast<uint4*>(box + lane * 128 + ((j ^ (lane & 7)) << 4)) = pack8(v);      // 128-byte swizzle
+            for (int j = 0; j < 4; ++j) {
+              int off = lane * 64 + j * 16;
+              off ^= ((off >> 7) & 3) << 4;                    // 64-byte swizzle
+              *reinterpret_cast<uint4*>(my_out + box * 2048 + off) = make_uint4(v[j * 4], v[j * 4 + 1], v[j * 4 + 2], v[j * 4 + 3]);
             }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) {
-              tma_store_2d(map, smem_u32(box), nbase, m0 + q * 32);
-              tma_store_commit();
-            }
-            ++boxes;
           };
-          if (tma_out == 2) {
-            leave(&map_aux, [&](int i) { return __uint_as_float(g[i]); });
-            leave(&map_aux2, [&](int i) { return __uint_as_float(u[i]); });
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float s0, s1;
+            const float a0 = gate_fn(__uint_as_float(g[2 * i]), act, &s0), a1 = gate_fn(__uint_as_float(g[2 * i + 1]), act, &s1);
+            const float u0 = __uint_as_float(u[2 * i]), u1 = __uint_as_float(u[2 * i + 1]);
+            const __nv_bfloat162 p = __floats2bfloat162_rn(a0 * u0, a1 * u1);
+            if (tma_out == 2) {
+              f[i] = pack_factors(a0, a1);
+              d[i] = pack_factors(u0 * s0, u1 * s1);
+            }
+            g[i] = reinterpret_cast<const uint32_t&>(p);
           }
-          leave(&map_c, [&](int i) { return gate_fn(__uint_as_float(g[i]), act, nullptr) * __uint_as_float(u[i]); });
+          if (lane == 0) tma_store_wait_read<0>();
+          __syncwarp();
+          put(0, g);
+          if (tma_out == 2) {
+            put(1, f);
+            put(2, d);
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&map_c, smem_u32(my_out), nbase, m0 + q * 32);
+            if (tma_out == 2) {
+              tma_store_2d(&map_aux, smem_u32(my_out + 2048), nbase, m0 + q * 32);
+              tma_store_2d(&map_aux2, smem_u32(my_out + 4096), nbase, m0 + q * 32);
+            }
+            tma_store_commit();
+          }
         }
       } else if constexpr (EPI == kEpiGatedGrad) {
-        // accumulator = dH:  dG = dH u act'(g) through map_c, dU = dH act(g) through map_aux
+        // accumulator = dH, times the kept factors:  dG = dH (u act'(g)) through map_c, dU = dH act(g) through map_aux
 #pragma unroll 1
         for (int c = part_first; c < part_first + kParts; ++c) {
           const int nbase = n0 + c * 32;
@@ -649,17 +683,17 @@ gemm_bf16_nt_persistent_kernel(const __grid_constant__ CUtensorMap map_a, const 
           for (int j = 0; j < 4; ++j) {
             int off = lane * 64 + j * 16;
             off ^= ((off >> 7) & 3) << 4;                      // 64-byte swizzle
-            const uint4 gv = *reinterpret_cast<const uint4*>(box + off), uv = *reinterpret_cast<const uint4*>(box + 2048 + off);
-            const __nv_bfloat162* gh = reinterpret_cast<const __nv_bfloat162*>(&gv);
-            const __nv_bfloat162* uh = reinterpret_cast<const __nv_bfloat162*>(&uv);
+            const uint4 fv = *reinterpret_cast<const uint4*>(box + off), dv = *reinterpret_cast<const uint4*>(box + 2048 + off);
+            const uint32_t f[4] = {fv.x, fv.y, fv.z, fv.w}, d[4] = {dv.x, dv.y, dv.z, dv.w};
             float a[8], b[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float2 g2 = __bfloat1622float2(gh[i >> 1]), u2 = __bfloat1622float2(uh[i >> 1]);
-              const float dh = __uint_as_float(r[j * 8 + i]);
-              float slope;
-              b[i] = dh * gate_fn((i & 1) ? g2.y : g2.x, act, &slope);
-              a[i] = dh * ((i & 1) ? u2.y : u2.x) * slope;
+            for (int i = 0; i < 4; ++i) {
+              const float h0 = __uint_as_float(r[j * 8 + 2 * i]) * kFactorUnscale, h1 = __uint_as_float(r[j * 8 + 2 * i + 1]) * kFactorUnscale;
+              const float2 x = unpack_factors(f[i]), y = unpack_factors(d[i]);
+              b[2 * i] = h0 * x.x;
+              b[2 * i + 1] = h1 * x.y;
+              a[2 * i] = h0 * y.x;
+              a[2 * i + 1] = h1 * y.y;
             }
             dg[j] = pack8(a);
             du[j] = pack8(b);
@@ -928,7 +962,7 @@ gemm_bf16_nt_persistent_kernel(const __grid_constant__ CUtensorMap map_a, const 
 // weights only once, and a cluster of `split` CTAs shares a tile's reduction so that all SMs read: with 128 x 256 tiles of
 // the kernel above the two products of that block kept 22 and 4 SMs busy and took 13 and 28 us.  The partial tiles meet in
 // distributed shared memory; every CTA adds up the cluster's sums for its share of the tokens, in the order of the slices.
-// GATED: 64 gate and 64 up rows make a tile, and act(g) u leaves (g and u themselves too when `pre` is given).
+// GATED: 64 gate and 64 up rows make a tile, and act(g) u leaves (the factors for the backward pass too when `pre` is given).
 // ------------------------------------------------------------------------------------------ //
 template <int NB>
 struct SkinnyCfg {
@@ -942,7 +976,7 @@ struct SkinnyCfg {
 template <int NB, bool GATED>
 __global__ void __launch_bounds__(192)
 gemm_bf16_skinny_kernel(const __grid_constant__ CUtensorMap map_lo, const __grid_constant__ CUtensorMap map_hi,
-                        const __grid_constant__ CUtensorMap map_x, __nv_bfloat16* __restrict__ out, __nv_bfloat16* __restrict__ pre,
+                        const __grid_constant__ CUtensorMap map_x, __nv_bfloat16* __restrict__ out, unsigned short* __restrict__ pre,
                         const __nv_bfloat16* __restrict__ residual, const int M, const int N, const int num_kb, const int split, const int act,
                         unsigned int* __restrict__ status) {
   using Cfg = SkinnyCfg<NB>;
@@ -1060,10 +1094,13 @@ gemm_bf16_skinny_kernel(const __grid_constant__ CUtensorMap map_lo, const __grid
       for (int t = first + (e >> 6); t < last; t += 2) {
         const float g = total(t * 128 + (e & 63)), u = total(t * 128 + 64 + (e & 63));
         if (f < N) {
-          out[size_t(t) * N + f] = __float2bfloat16_rn(gate_fn(g, act, nullptr) * u);
+          float slope;
+          const float a = gate_fn(g, act, &slope);
+          out[size_t(t) * N + f] = __float2bfloat16_rn(a * u);
           if (pre != nullptr) {
-            pre[size_t(t) * (2 * N) + f] = __float2bfloat16_rn(g);
-            pre[size_t(t) * (2 * N) + N + f] = __float2bfloat16_rn(u);
+            const uint32_t w = pack_factors(a, u * slope);
+            pre[size_t(t) * (2 * N) + f] = static_cast<unsigned short>(w);
+            pre[size_t(t) * (2 * N) + N + f] = static_cast<unsigned short>(w >> 16);
           }
         }
       }
@@ -1161,6 +1198,21 @@ bool UsePair(int M, int N, int K, int sm_count) {
   return K >= 1024 && tiles >= sm_count / 4;
 }
 
+// Tiles for the products of a gated block, which come in every size: pairs of SMs with 256 columns per tile, or with 128, or single
+// SMs.  A CTA's time for 64 elements of the reduction is that of its loads, 32 KB and 24 KB at about 50 bytes a cycle (the MMAs
+// need 512 and 256 cycles); a tile more costs a whole wave.  1537 x 776 x 2056: 154 us with UsePair's rule, 127 us with
+// 256-column pairs throughout, 124 us with this one.
+enum GemmTiles { kTilesSingle, kTilesPair256, kTilesPair128 };
+GemmTiles PlanTiles(int M, int N, int K, int sm_count) {
+  if (M <= 128 || N <= 128 || sm_count < 2) return kTilesSingle;
+  const long long kb = (K + BK - 1) / BK, pairs = sm_count / 2, rows = (M + 255) / 256;
+  auto cost = [&](long long columns, long long cycles) {
+    const long long tiles = rows * ((N + columns - 1) / columns);
+    return (tiles + pairs - 1) / pairs * (kb * cycles + 2000);
+  };
+  return cost(128, 490) < cost(256, 655) ? kTilesPair128 : kTilesPair256;
+}
+
 int SmCount() {
   static int sm_count = 0;
   if (sm_count == 0) {
@@ -1173,7 +1225,7 @@ int SmCount() {
 }
 
 template <int NB, bool GATED>
-cudaError_t LaunchSkinny(const CUtensorMap& lo, const CUtensorMap& hi, const CUtensorMap& x, __nv_bfloat16* out, __nv_bfloat16* pre,
+cudaError_t LaunchSkinny(const CUtensorMap& lo, const CUtensorMap& hi, const CUtensorMap& x, __nv_bfloat16* out, unsigned short* pre,
                          const __nv_bfloat16* residual, int M, int N, int K, int act, unsigned int* status, cudaStream_t stream) {
   using Cfg = SkinnyCfg<NB>;
   auto kernel = gemm_bf16_skinny_kernel<NB, GATED>;
@@ -1220,7 +1272,7 @@ cudaError_t Skinny(const void* x, const void* w, void* out, void* pre, const voi
   hi = lo;
   if (GATED && !MakeMap(&hi, static_cast<const __nv_bfloat16*>(w) + size_t(N) * K, N, K, 64)) return cudaErrorInvalidValue;
   __nv_bfloat16* o = static_cast<__nv_bfloat16*>(out);
-  __nv_bfloat16* p = static_cast<__nv_bfloat16*>(pre);
+  unsigned short* p = static_cast<unsigned short*>(pre);
   const __nv_bfloat16* r = static_cast<const __nv_bfloat16*>(residual);
   const cudaError_t e = nb == 16   ? LaunchSkinny<16, GATED>(lo, hi, mx, o, p, r, M, N, K, act, status, stream)
                         : nb == 32 ? LaunchSkinny<32, GATED>(lo, hi, mx, o, p, r, M, N, K, act, status, stream)
@@ -1232,12 +1284,52 @@ cudaError_t Skinny(const void* x, const void* w, void* out, void* pre, const voi
 
 }  // namespace
 
-cudaError_t LaunchGemmBf16FewRows(const void* a, const void* b, void* out, int M, int N, int K, unsigned int* status, cudaStream_t stream,
-                                  const void* addend) {
-  return Skinny<false>(a, b, out, nullptr, addend, M, N, K, kActNone, status, stream);
+bool GemmSupported() { return GetEncodeFn() != nullptr; }
+
+// The three plain products of a gated block (kEpiNone or kEpiAddAux) on the tiles that PlanTiles chooses: b is [N, K] for NT, else
+// [K, N]; a is [M, K], for TN [K, M].
+template <int BMODE, int AMODE>
+cudaError_t LaunchPlanned(const void* a, const void* b, void* out, const void* addend, int M, int N, int K, unsigned int* status, cudaStream_t stream) {
+  (void)cudaGetLastError();   // the value returned below must be this launch's own, not an older error of the calling thread
+  const uintptr_t all = reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(addend);
+  if (M <= 0 || N <= 0 || K <= 0 || (N % 8) != 0 || (AMODE == 0 ? K % 8 != 0 : M % 8 != 0) || (all & 15) != 0) return cudaErrorInvalidValue;
+  const int sm_count = SmCount();
+  const GemmTiles tiles = PlanTiles(M, N, K, sm_count);
+  const int bn = tiles == kTilesPair128 || (tiles == kTilesSingle && N <= 128) ? 128 : 256;
+  CUtensorMap map_a, map_b, map_c;
+  if (!(AMODE == 0 ? MakeMap(&map_a, a, M, K, BM) : MakeMap(&map_a, a, K, M, 64)) ||
+      !(BMODE == 0 ? MakeMap(&map_b, b, N, K, tiles == kTilesSingle ? bn : bn / 2) : MakeMap(&map_b, b, K, N, 64)) || !MakeMap(&map_c, out, M, N, 32))
+    return cudaErrorInvalidValue;
+  __nv_bfloat16* o = static_cast<__nv_bfloat16*>(out);
+  const __nv_bfloat16* add = static_cast<const __nv_bfloat16*>(addend);
+  auto go = [&](auto epi) {
+    constexpr int EPI = decltype(epi)::value;
+    if (tiles == kTilesPair256)
+      return LaunchPersistent<256, BMODE, AMODE, EPI, 1>(map_a, map_b, map_c, map_c, o, nullptr, add, M, N, K, 0, 1, sm_count, status, stream);
+    if (tiles == kTilesPair128)
+      return LaunchPersistent<128, BMODE, AMODE, EPI, 1>(map_a, map_b, map_c, map_c, o, nullptr, add, M, N, K, 0, 1, sm_count, status, stream);
+    if (bn == 256) return LaunchPersistent<256, BMODE, AMODE, EPI>(map_a, map_b, map_c, map_c, o, nullptr, add, M, N, K, 0, 1, sm_count, status, stream);
+    return LaunchPersistent<128, BMODE, AMODE, EPI>(map_a, map_b, map_c, map_c, o, nullptr, add, M, N, K, 0, 1, sm_count, status, stream);
+  };
+  cudaError_t e;
+  if constexpr (BMODE == 0) e = add != nullptr ? go(std::integral_constant<int, kEpiAddAux>()) : go(std::integral_constant<int, kEpiNone>());
+  else e = add != nullptr ? cudaErrorInvalidValue : go(std::integral_constant<int, kEpiNone>());
+  if (e != cudaSuccess) return e;
+  CountKernelLaunch();
+  return cudaGetLastError();
 }
 
-bool GemmSupported() { return GetEncodeFn() != nullptr; }
+cudaError_t LaunchGemmGatedDown(const void* a, const void* b, void* out, int M, int N, int K, unsigned int* status, cudaStream_t stream,
+                                const void* addend) {
+  if (M <= kSkinnyRows) return Skinny<false>(a, b, out, nullptr, addend, M, N, K, kActNone, status, stream);
+  return LaunchPlanned<0, 0>(a, b, out, addend, M, N, K, status, stream);
+}
+cudaError_t LaunchGemmGatedInput(const void* a, const void* b, void* out, int M, int N, int K, unsigned int* status, cudaStream_t stream) {
+  return LaunchPlanned<1, 0>(a, b, out, nullptr, M, N, K, status, stream);
+}
+cudaError_t LaunchGemmGatedWeight(const void* a, const void* b, void* out, int M, int N, int K, unsigned int* status, cudaStream_t stream) {
+  return LaunchPlanned<1, 1>(a, b, out, nullptr, M, N, K, status, stream);
+}
 
 cudaError_t LaunchGemmBf16NT(const void* a, const void* b, void* out, const void* bias, int M, int N, int K, int act,
                              unsigned int* status, cudaStream_t stream, void* preact_out, float* col_stats,
@@ -1379,62 +1471,65 @@ cudaError_t LaunchGemmBf16NN(const void* a, const void* b, void* out, int M, int
 
 // h[M,F] = act(a Wg^T) * (a Wu^T) with [Wg; Wu] = w [2F, K]: one tile of the accumulator holds the same columns of both
 // products, so the activation and the product with the gate are part of the epilogue.
-cudaError_t LaunchGemmBf16Gated(const void* a, const void* w, void* h, void* preact, int M, int F, int K, int act,
+cudaError_t LaunchGemmBf16Gated(const void* a, const void* w, void* h, void* factors, int M, int F, int K, int act,
                                 unsigned int* status, cudaStream_t stream) {
   (void)cudaGetLastError();   // the value returned below must be this launch's own, not an older error of the calling thread
   if (M <= 0 || F <= 0 || K <= 0 || (K % 8) != 0 || (F % 8) != 0 || (act != kActSilu && act != kActGeluTanh)) return cudaErrorInvalidValue;
   if ((reinterpret_cast<uintptr_t>(a) & 15) || (reinterpret_cast<uintptr_t>(w) & 15) || (reinterpret_cast<uintptr_t>(h) & 15) ||
-      (reinterpret_cast<uintptr_t>(preact) & 15))
+      (reinterpret_cast<uintptr_t>(factors) & 15))
     return cudaErrorInvalidValue;
-  if (M <= kSkinnyRows) return Skinny<true>(a, w, h, preact, nullptr, M, F, K, act, status, stream);
+  if (M <= kSkinnyRows) return Skinny<true>(a, w, h, factors, nullptr, M, F, K, act, status, stream);
   const int sm_count = SmCount();
   const __nv_bfloat16* wu = static_cast<const __nv_bfloat16*>(w) + size_t(F) * K;
-  __nv_bfloat16* pre = static_cast<__nv_bfloat16*>(preact);
-  CUtensorMap map_a, map_g, map_u, map_h, map_pg, map_pu;
+  unsigned short* kept = static_cast<unsigned short*>(factors);
+  CUtensorMap map_a, map_g, map_u, map_h, map_f, map_d;
   // the weights' boxes: half of the accumulator's columns each
-  const bool pair = UsePair(M, 2 * F, K, sm_count);
+  const bool pair = M > 128 && F > 64 && sm_count >= 2;       // pairs as in PlanTiles; their 256 columns are 128 of the result
   const int box_w = pair || F > 64 ? 128 : 64;
-  if (!MakeMap(&map_a, a, M, K, BM) || !MakeMap(&map_g, w, F, K, box_w) || !MakeMap(&map_u, wu, F, K, box_w) || !MakeMap(&map_h, h, M, F, 32))
+  if (!MakeMap(&map_a, a, M, K, BM) || !MakeMap(&map_g, w, F, K, box_w) || !MakeMap(&map_u, wu, F, K, box_w) || !MakeMap(&map_h, h, M, F, 32, 0, 32))
     return cudaErrorInvalidValue;
-  map_pg = map_pu = map_h;
-  if (pre != nullptr && (!MakeMap(&map_pg, pre, M, F, 32, 2ll * F) || !MakeMap(&map_pu, pre + F, M, F, 32, 2ll * F))) return cudaErrorInvalidValue;
+  map_f = map_d = map_h;
+  if (kept != nullptr && (!MakeMap(&map_f, kept, M, F, 32, 2ll * F, 32) || !MakeMap(&map_d, kept + F, M, F, 32, 2ll * F, 32))) return cudaErrorInvalidValue;
   __nv_bfloat16* o = static_cast<__nv_bfloat16*>(h);
-  const int mode = pre != nullptr ? 2 : 1;
+  const int mode = kept != nullptr ? 2 : 1;
   const cudaError_t e =
-      pair      ? LaunchPersistent<256, 0, 0, kEpiGated, 1>(map_a, map_g, map_h, map_pg, o, nullptr, nullptr, M, F, K, act, mode, sm_count,
-                                                            status, stream, nullptr, &map_u, &map_pu)
-      : F > 64 ? LaunchPersistent<256, 0, 0, kEpiGated>(map_a, map_g, map_h, map_pg, o, nullptr, nullptr, M, F, K, act, mode, sm_count, status,
-                                                        stream, nullptr, &map_u, &map_pu)
-               : LaunchPersistent<128, 0, 0, kEpiGated>(map_a, map_g, map_h, map_pg, o, nullptr, nullptr, M, F, K, act, mode, sm_count, status,
-                                                        stream, nullptr, &map_u, &map_pu);
+      pair      ? LaunchPersistent<256, 0, 0, kEpiGated, 1>(map_a, map_g, map_h, map_f, o, nullptr, nullptr, M, F, K, act, mode, sm_count,
+                                                            status, stream, nullptr, &map_u, &map_d)
+      : F > 64 ? LaunchPersistent<256, 0, 0, kEpiGated>(map_a, map_g, map_h, map_f, o, nullptr, nullptr, M, F, K, act, mode, sm_count, status,
+                                                        stream, nullptr, &map_u, &map_d)
+               : LaunchPersistent<128, 0, 0, kEpiGated>(map_a, map_g, map_h, map_f, o, nullptr, nullptr, M, F, K, act, mode, sm_count, status,
+                                                        stream, nullptr, &map_u, &map_d);
   if (e != cudaSuccess) return e;
   CountKernelLaunch();
   return cudaGetLastError();
 }
 
-// dpre[M,2F] = [dG dU] from dH = a[M,K] * b[K,F] and the kept preact[M,2F] = [G U].
-cudaError_t LaunchGemmBf16NNGatedGrad(const void* a, const void* b, const void* preact, void* dpre, int M, int F, int K, int act,
+// dpre[M,2F] = [dG dU] from dH = a[M,K] * b[K,F] and the kept factors[M,2F] = [act(G), U act'(G)].
+cudaError_t LaunchGemmBf16NNGatedGrad(const void* a, const void* b, const void* factors, void* dpre, int M, int F, int K,
                                       unsigned int* status, cudaStream_t stream) {
   (void)cudaGetLastError();
-  if (M <= 0 || F <= 0 || K <= 0 || (K % 8) != 0 || (F % 8) != 0 || (act != kActSilu && act != kActGeluTanh)) return cudaErrorInvalidValue;
-  if ((reinterpret_cast<uintptr_t>(a) & 15) || (reinterpret_cast<uintptr_t>(b) & 15) || (reinterpret_cast<uintptr_t>(preact) & 15) ||
+  if (M <= 0 || F <= 0 || K <= 0 || (K % 8) != 0 || (F % 8) != 0) return cudaErrorInvalidValue;
+  if ((reinterpret_cast<uintptr_t>(a) & 15) || (reinterpret_cast<uintptr_t>(b) & 15) || (reinterpret_cast<uintptr_t>(factors) & 15) ||
       (reinterpret_cast<uintptr_t>(dpre) & 15))
     return cudaErrorInvalidValue;
   const int sm_count = SmCount();
   __nv_bfloat16* o = static_cast<__nv_bfloat16*>(dpre);
-  const __nv_bfloat16* pre = static_cast<const __nv_bfloat16*>(preact);
-  CUtensorMap map_a, map_b, map_dg, map_du, map_g, map_u;
+  const unsigned short* kept = static_cast<const unsigned short*>(factors);
+  const GemmTiles tiles = PlanTiles(M, F, K, sm_count);
+  CUtensorMap map_a, map_b, map_dg, map_du, map_f, map_d;
   if (!MakeMap(&map_a, a, M, K, BM) || !MakeMap(&map_b, b, K, F, 64) || !MakeMap(&map_dg, o, M, F, 32, 2ll * F, 32) ||
-      !MakeMap(&map_du, o + F, M, F, 32, 2ll * F, 32) || !MakeMap(&map_g, pre, M, F, 32, 2ll * F, 32) ||
-      !MakeMap(&map_u, pre + F, M, F, 32, 2ll * F, 32))
+      !MakeMap(&map_du, o + F, M, F, 32, 2ll * F, 32) || !MakeMap(&map_f, kept, M, F, 32, 2ll * F, 32) ||
+      !MakeMap(&map_d, kept + F, M, F, 32, 2ll * F, 32))
     return cudaErrorInvalidValue;
   const cudaError_t e =
-      UsePair(M, F, K, sm_count) ? LaunchPersistent<256, 1, 0, kEpiGatedGrad, 1>(map_a, map_b, map_dg, map_du, o, nullptr, nullptr, M, F, K, act, 1,
-                                                                                 sm_count, status, stream, nullptr, &map_g, &map_u)
-      : F > 128 ? LaunchPersistent<256, 1, 0, kEpiGatedGrad>(map_a, map_b, map_dg, map_du, o, nullptr, nullptr, M, F, K, act, 1, sm_count, status,
-                                                             stream, nullptr, &map_g, &map_u)
-                : LaunchPersistent<128, 1, 0, kEpiGatedGrad>(map_a, map_b, map_dg, map_du, o, nullptr, nullptr, M, F, K, act, 1, sm_count, status,
-                                                             stream, nullptr, &map_g, &map_u);
+      tiles == kTilesPair256   ? LaunchPersistent<256, 1, 0, kEpiGatedGrad, 1>(map_a, map_b, map_dg, map_du, o, nullptr, nullptr, M, F, K, 0, 1,
+                                                                               sm_count, status, stream, nullptr, &map_f, &map_d)
+      : tiles == kTilesPair128 ? LaunchPersistent<128, 1, 0, kEpiGatedGrad, 1>(map_a, map_b, map_dg, map_du, o, nullptr, nullptr, M, F, K, 0, 1,
+                                                                               sm_count, status, stream, nullptr, &map_f, &map_d)
+      : F > 128 ? LaunchPersistent<256, 1, 0, kEpiGatedGrad>(map_a, map_b, map_dg, map_du, o, nullptr, nullptr, M, F, K, 0, 1, sm_count, status,
+                                                             stream, nullptr, &map_f, &map_d)
+                : LaunchPersistent<128, 1, 0, kEpiGatedGrad>(map_a, map_b, map_dg, map_du, o, nullptr, nullptr, M, F, K, 0, 1, sm_count, status,
+                                                             stream, nullptr, &map_f, &map_d);
   if (e != cudaSuccess) return e;
   CountKernelLaunch();
   return cudaGetLastError();

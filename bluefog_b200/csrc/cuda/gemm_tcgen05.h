@@ -39,18 +39,23 @@ cudaError_t LaunchGemmBf16NN(const void* a, const void* b, void* out, int M, int
 cudaError_t LaunchGemmBf16TN(const void* a, const void* b, void* out, int M, int N, int K, unsigned int* status,
                              cudaStream_t stream);
 
-// out[M,N] = a[M,K] * b[N,K]^T (+ addend[M,N]) for at most kSkinnyRows rows, the reduction shared by clusters of CTAs; K % 8 == 0,
-// N % 8 == 0.
+// The other products of a gated feed-forward block, on tiles chosen for their size.  Up to kSkinnyRows rows the forward products
+// share their reductions between clusters of CTAs.
+//   down    out[M,N] = a[M,K] * b[N,K]^T (+ addend[M,N]);  K % 8 == 0, N % 8 == 0
+//   input   out[M,N] = a[M,K] * b[K,N];                    K % 8 == 0, N % 8 == 0
+//   weight  out[M,N] = a[K,M]^T * b[K,N];                  M % 8 == 0, N % 8 == 0
 constexpr int kSkinnyRows = 64;
-cudaError_t LaunchGemmBf16FewRows(const void* a, const void* b, void* out, int M, int N, int K, unsigned int* status, cudaStream_t stream,
-                                  const void* addend = nullptr);
+cudaError_t LaunchGemmGatedDown(const void* a, const void* b, void* out, int M, int N, int K, unsigned int* status, cudaStream_t stream,
+                                const void* addend = nullptr);
+cudaError_t LaunchGemmGatedInput(const void* a, const void* b, void* out, int M, int N, int K, unsigned int* status, cudaStream_t stream);
+cudaError_t LaunchGemmGatedWeight(const void* a, const void* b, void* out, int M, int N, int K, unsigned int* status, cudaStream_t stream);
 
-// h[M,F] = act(a[M,K] * w[0:F,K]^T) * (a * w[F:2F,K]^T), act kActSilu or kActGeluTanh; K % 8 == 0, F % 8 == 0.  preact
-// (optional, [M,2F]): receives both products before the activation.
-cudaError_t LaunchGemmBf16Gated(const void* a, const void* w, void* h, void* preact, int M, int F, int K, int act,
+// h[M,F] = act(a[M,K] * w[0:F,K]^T) * (a * w[F:2F,K]^T), act kActSilu or kActGeluTanh; K % 8 == 0, F % 8 == 0.  factors
+// (optional, [M,2F] 16-bit words): receives act(G) and U act'(G) in a format of their own, for the gradient.
+cudaError_t LaunchGemmBf16Gated(const void* a, const void* w, void* h, void* factors, int M, int F, int K, int act,
                                 unsigned int* status, cudaStream_t stream);
-// Its gradient: with dH[M,F] = a[M,K] * b[K,F] and preact = [G U], dpre[M,2F] = [dH U act'(G), dH act(G)].
-cudaError_t LaunchGemmBf16NNGatedGrad(const void* a, const void* b, const void* preact, void* dpre, int M, int F, int K, int act,
+// Its gradient: with dH[M,F] = a[M,K] * b[K,F], dpre[M,2F] = [dH U act'(G), dH act(G)].
+cudaError_t LaunchGemmBf16NNGatedGrad(const void* a, const void* b, const void* factors, void* dpre, int M, int F, int K,
                                       unsigned int* status, cudaStream_t stream);
 
 }  // namespace bfb
