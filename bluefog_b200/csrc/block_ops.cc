@@ -278,13 +278,6 @@ at::Tensor DownProduct(const at::Tensor& h, const at::Tensor& w_down, const at::
         "gated_mlp");
   return y;
 }
-// a^T b of two matrices with the same rows: a weight's gradient
-at::Tensor TransposedProduct(const at::Tensor& a, const at::Tensor& b) {
-  at::Tensor out = at::empty({a.size(1), b.size(1)}, a.options());
-  Check(LaunchGemmGatedWeight(a.data_ptr(), b.data_ptr(), out.data_ptr(), static_cast<int>(a.size(1)), static_cast<int>(b.size(1)),
-                         static_cast<int>(a.size(0)), GemmStatus(a), StreamOf(a)), "gated_mlp backward");
-  return out;
-}
 at::Tensor Rows2d(const at::Tensor& t) { return Dense(t.reshape({-1, t.size(-1)})); }
 std::vector<int64_t> WithColumns(const at::Tensor& a, int64_t columns) {
   std::vector<int64_t> s(a.sizes().begin(), a.sizes().end());
@@ -311,20 +304,30 @@ struct GatedMlpNode : public torch::autograd::Function<GatedMlpNode> {
     const c10::cuda::CUDAGuard guard(a.get_device());
     const at::Tensor dy = Rows2d(grads[0]);
     const int m = static_cast<int>(a.size(0)), f = static_cast<int>(h.size(1)), k = static_cast<int>(a.size(1));
-    at::Tensor da, dwgu, dwd;
+    const int n = static_cast<int>(wd.size(0));
+    at::Tensor da, dwgu, dwd, dpre;
+    GemmGroupItem list[3];
+    int count = 0;
     if (ctx->needs_input_grad(0) || ctx->needs_input_grad(1)) {
       // [dG dU] straight from the epilogue of dH = dy Wd
-      at::Tensor dpre = at::empty(factors.sizes(), a.options());
-      Check(LaunchGemmBf16NNGatedGrad(dy.data_ptr(), wd.data_ptr(), factors.data_ptr(), dpre.data_ptr(), m, f, static_cast<int>(wd.size(0)),
-                                      GemmStatus(a), StreamOf(a)), "gated_mlp backward");
+      dpre = at::empty(factors.sizes(), a.options());
+      Check(LaunchGemmBf16NNGatedGrad(dy.data_ptr(), wd.data_ptr(), factors.data_ptr(), dpre.data_ptr(), m, f, n, GemmStatus(a), StreamOf(a)),
+            "gated_mlp backward");
       if (ctx->needs_input_grad(0)) {
         da = at::empty(a.sizes(), a.options());
-        Check(LaunchGemmGatedInput(dpre.data_ptr(), wgu.data_ptr(), da.data_ptr(), m, k, 2 * f, GemmStatus(a), StreamOf(a)), "gated_mlp backward");
-        da = da.view(ctx->saved_data["sizes"].toIntVector());
+        list[count++] = {dpre.data_ptr(), wgu.data_ptr(), da.data_ptr(), m, k, 2 * f, false};
       }
-      if (ctx->needs_input_grad(1)) dwgu = TransposedProduct(dpre, a);
+      if (ctx->needs_input_grad(1)) {
+        dwgu = at::empty(wgu.sizes(), a.options());
+        list[count++] = {dpre.data_ptr(), a.data_ptr(), dwgu.data_ptr(), 2 * f, k, m, true};
+      }
     }
-    if (ctx->needs_input_grad(2)) dwd = TransposedProduct(dy, h);
+    if (ctx->needs_input_grad(2)) {
+      dwd = at::empty(wd.sizes(), a.options());
+      list[count++] = {dy.data_ptr(), h.data_ptr(), dwd.data_ptr(), n, f, m, true};
+    }
+    if (count > 0) Check(LaunchGemmGroup(list, count, GemmStatus(a), StreamOf(a)), "gated_mlp backward");
+    if (da.defined()) da = da.view(ctx->saved_data["sizes"].toIntVector());
     variable_list g = Once("gated_mlp", {da, dwgu, dwd});
     return {g[0], g[1], g[2], at::Tensor(), ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(3) ? grads[0] : at::Tensor()};
   }

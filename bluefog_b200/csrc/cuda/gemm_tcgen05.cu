@@ -28,6 +28,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
+#include <climits>
 #include <cstdlib>
 #include <string>
 #include <type_traits>
@@ -957,6 +959,200 @@ gemm_bf16_nt_persistent_kernel(const __grid_constant__ CUtensorMap map_a, const 
 }
 
 // ------------------------------------------------------------------------------------------ //
+// Up to three products in one launch of the two-SM kernel (256 x 256 tiles): the input gradient and both weight gradients of a
+// gated block do not depend on one another, and as launches of their own each ends in a wave that leaves SM pairs idle (8192 x
+// 1024 x 2752: 128, 88 and 44 tiles on 74 pairs, two, two and one wave, 68 + 91 + 50 us; together REPLACE_GROUP us).  The tiles with the
+// longest reductions come first.  B is [reduction, N] row-major in all of them; A is [M, reduction] or, for a weight
+// gradient, [reduction, M].
+// ------------------------------------------------------------------------------------------ //
+constexpr int kMaxGroup = 3;
+struct GroupProblem {
+  int M, N, num_kb, tiles_m, tiles_n, first_item, a_mn;
+};
+struct GroupArgs {
+  CUtensorMap a[kMaxGroup], b[kMaxGroup], c[kMaxGroup];
+  GroupProblem p[kMaxGroup];
+  int items;
+};
+
+__global__ void __launch_bounds__((PersistentCfg<256, kEpiNone, 1>::kThreadsP), 1)
+gemm_bf16_group_kernel(const __grid_constant__ GroupArgs args, unsigned int* __restrict__ status) {
+  using Cfg = PersistentCfg<256, kEpiNone, 1>;
+  constexpr int S = Cfg::kStagesP;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  unsigned char* stage_a = smem;
+  unsigned char* stage_b = smem + size_t(S) * Cfg::kBytesA;
+  unsigned char* stage_out = smem + size_t(S) * Cfg::kBytesStage;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(stage_out + Cfg::kBytesOut);
+  // bars[0..S): full, [S..2S): empty, [2S..2S+2): acc_full, [2S+2..2S+4): acc_empty
+  __shared__ uint32_t tmem_base_s;
+  __shared__ int failed_s;
+  volatile int* failed = &failed_s;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  const int first = int(blockIdx.x >> 1), step = int(gridDim.x >> 1);
+  // problem of an item and its tile
+  auto locate = [&](int item, int& tm, int& tn) {
+    int i = 0;
+    while (i + 1 < kMaxGroup && item >= args.p[i + 1].first_item) ++i;
+    tile_coords(item - args.p[i].first_item, args.p[i].tiles_m, args.p[i].tiles_n, tm, tn);
+    return i;
+  };
+
+  if (threadIdx.x == 0) {
+    failed_s = 0;
+    for (int s = 0; s < 2 * S + 2; ++s) mbar_init(smem_u32(&bars[s]), 1);
+    for (int a = 0; a < 2; ++a) mbar_init(smem_u32(&bars[2 * S + 2 + a]), 2 * Cfg::kEpiWarps);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)), "r"(Cfg::kCols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  fence_before_sync();
+  __syncthreads();
+  // nobody signals a peer's barrier before the peer has initialised it
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  fence_after_sync();
+  const uint32_t tmem_base = tmem_base_s;
+
+  int armed = 0;
+  if (warp == 0) {
+    if (lane == 0) {
+      bool ok = true;
+      for (int item = first; item < args.items && ok; item += step) {
+        int tm, tn;
+        const int i = locate(item, tm, tn);
+        const int m0 = tm * Cfg::kTileM + int(rank) * BM, n0 = tn * 256 + int(rank) * Cfg::kRowsB;
+        const bool a_mn = args.p[i].a_mn != 0;
+        const int num_kb = args.p[i].num_kb;
+        for (int kb = 0; kb < num_kb; ++kb, ++armed) {
+          const int s = armed % S;
+          ok = mbar_wait(smem_u32(&bars[S + s]), ((armed / S) & 1) ^ 1, failed);
+          if (!ok) break;
+          // the leader's barrier counts the bytes of both CTAs; the leader arms it
+          if (leader) mbar_expect_tx(smem_u32(&bars[s]), 2u * Cfg::kBytesStage);
+          const uint32_t full = mapa_u32(smem_u32(&bars[s]), 0u);
+          const uint32_t a = smem_u32(stage_a + size_t(s) * Cfg::kBytesA), b = smem_u32(stage_b + size_t(s) * Cfg::kBytesB);
+          if (a_mn) {
+#pragma unroll
+            for (int j = 0; j < BM / 64; ++j) tma_load_2d_pair(a + j * 8192, &args.a[i], full, m0 + j * 64, kb * BK);
+          } else {
+            tma_load_2d_pair(a, &args.a[i], full, kb * BK, m0);
+          }
+#pragma unroll
+          for (int j = 0; j < Cfg::kRowsB / 64; ++j) tma_load_2d_pair(b + j * 8192, &args.b[i], full, n0 + j * 64, kb * BK);
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (leader) {
+      int it = 0, local = 0;
+      bool ok = true;
+      for (int item = first; item < args.items && ok; item += step, ++local) {
+        int tm, tn;
+        const int i = locate(item, tm, tn);
+        const int acc = local & 1, num_kb = args.p[i].num_kb;
+        const bool a_mn = args.p[i].a_mn != 0;
+        // the epilogue of both CTAs must have drained this accumulator buffer
+        ok = mbar_wait_cluster(smem_u32(&bars[2 * S + 2 + acc]), ((local >> 1) & 1) ^ 1, failed);
+        if (!ok) break;
+        fence_after_sync();
+        const uint32_t tmem_d = tmem_base + uint32_t(acc * 256);
+        const uint32_t idesc = Cfg::kIdesc | (a_mn ? 1u << 15 : 0u) | (1u << 16);
+        const uint64_t a_step = a_mn ? (16 * 128) >> 4 : 2;
+        for (int kb = 0; kb < num_kb; ++kb, ++it) {
+          const int s = it % S;
+          ok = mbar_wait(smem_u32(&bars[s]), (it / S) & 1, failed);
+          if (!ok) break;
+          const uint32_t a_addr = smem_u32(stage_a + size_t(s) * Cfg::kBytesA);
+          const uint64_t adesc = a_mn ? make_desc_mn(a_addr, 8192, 1024) : make_desc(a_addr);
+          const uint64_t bdesc = make_desc_mn(smem_u32(stage_b + size_t(s) * Cfg::kBytesB), 8192, 1024);
+          if (elect_one()) {
+#pragma unroll
+            for (int k = 0; k < BK / kUmmaK; ++k)
+              asm volatile(
+                  "{\n\t.reg .pred p;\n\t"
+                  "setp.ne.b32 p, %4, 0;\n\t"
+                  "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5, %5, %5, %5, %5}, p;\n\t}"
+                  ::"r"(tmem_d), "l"(adesc + a_step * uint64_t(k)), "l"(bdesc + uint64_t(128 * k)), "r"(idesc),
+                    "r"((kb | k) != 0 ? 1u : 0u), "r"(0u)
+                  : "memory");
+            umma_commit_pair(smem_u32(&bars[S + s]));
+            if (kb == num_kb - 1) umma_commit_pair(smem_u32(&bars[2 * S + acc]));
+          }
+          __syncwarp();
+        }
+      }
+    }
+  } else {
+    const int q = warp & 3, ew = warp - 2;             // quarter of tensor memory; two warps per quarter, half of the columns each
+    unsigned char* my_out = stage_out + size_t(ew) * 2 * Cfg::kBytesOutBox;
+    int local = 0, boxes = 0;
+    for (int item = first; item < args.items; item += step, ++local) {
+      int tm, tn;
+      const int i = locate(item, tm, tn);
+      const int acc = local & 1, M = args.p[i].M, N = args.p[i].N;
+      const int m = tm * Cfg::kTileM + int(rank) * BM + q * 32, n0 = tn * 256 + (ew >> 2) * 128;
+      if (!mbar_wait(smem_u32(&bars[2 * S + acc]), (local >> 1) & 1, failed)) break;
+      fence_after_sync();
+#pragma unroll 1
+      for (int c = 0; c < 2; ++c) {
+        const int n = n0 + c * 64;
+        if (n >= N || m >= M) break;                   // warp-uniform
+        uint32_t r[64];
+        const uint32_t taddr = tmem_base + (uint32_t(q * 32) << 16) + uint32_t(acc * 256 + (ew >> 2) * 128 + c * 64);
+        tmem_ld32(taddr, r);
+        tmem_ld32(taddr + 32, r + 32);
+        if (lane == 0) tma_store_wait_read<1>();       // the box written two stores ago has been read
+        tmem_wait_ld();
+        tie32(r);
+        tie32(r + 32);
+        __syncwarp();
+        unsigned char* box = my_out + size_t(boxes & 1) * Cfg::kBytesOutBox;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          *reinterpret_cast<uint4*>(box + lane * 128 + ((j ^ (lane & 7)) << 4)) = pack8(reinterpret_cast<const float*>(r + j * 8));      // 128-byte swizzle
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_2d(&args.c[i], smem_u32(box), n, m);
+          tma_store_commit();
+        }
+        ++boxes;
+      }
+      fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(mapa_u32(smem_u32(&bars[2 * S + 2 + acc]), 0u));
+    }
+    if (lane == 0) tma_store_wait_all();               // before this shared memory goes away
+    __syncwarp();
+  }
+  if (warp == 0 && lane == 0 && *failed && leader) {
+    for (int it = armed > S ? armed - S : 0; it < armed; ++it) {
+      const unsigned long long t0 = now_ns();
+      while (!mbar_try(smem_u32(&bars[it % S]), (it / S) & 1) && now_ns() - t0 < kWaitLimitNs) {}
+    }
+  }
+  __syncwarp();
+  fence_before_sync();
+  __syncthreads();
+  // neither CTA leaves (or frees tensor memory) while the other may still read its shared memory or signal it
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (warp == 1) {
+    fence_after_sync();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(Cfg::kCols) : "memory");
+  }
+  if (threadIdx.x == 0 && failed_s && status != nullptr) atomicExch(status, 1u);
+}
+
+// ------------------------------------------------------------------------------------------ //
 // Few rows: out[M, N] = x[M, K] w[N, K]^T with M <= 64, where the weights are what is read (8 x 1024 x 2752: 17 MB, 2.6 us from
 // memory).  The roles are swapped - 128 weight rows are the M side of the MMA, NB >= M tokens its N side - so that a CTA reads
 // weights only once, and a cluster of `split` CTAs shares a tile's reduction so that all SMs read: with 128 x 256 tiles of
@@ -1200,8 +1396,8 @@ bool UsePair(int M, int N, int K, int sm_count) {
 
 // Tiles for the products of a gated block, which come in every size: pairs of SMs with 256 columns per tile, or with 128, or single
 // SMs.  A CTA's time for 64 elements of the reduction is that of its loads, 32 KB and 24 KB at about 50 bytes a cycle (the MMAs
-// need 512 and 256 cycles); a tile more costs a whole wave.  1537 x 776 x 2056: 154 us with UsePair's rule, 127 us with
-// 256-column pairs throughout, 124 us with this one.
+// need 512 and 256 cycles); a tile more costs a whole wave.  The block of 1537 x 776 x 2056, three launches for its last three
+// gradients: 154 us with UsePair's rule, 127 us with 256-column pairs throughout, 124 us with this one.
 enum GemmTiles { kTilesSingle, kTilesPair256, kTilesPair128 };
 GemmTiles PlanTiles(int M, int N, int K, int sm_count) {
   if (M <= 128 || N <= 128 || sm_count < 2) return kTilesSingle;
@@ -1286,49 +1482,87 @@ cudaError_t Skinny(const void* x, const void* w, void* out, void* pre, const voi
 
 bool GemmSupported() { return GetEncodeFn() != nullptr; }
 
-// The three plain products of a gated block (kEpiNone or kEpiAddAux) on the tiles that PlanTiles chooses: b is [N, K] for NT, else
-// [K, N]; a is [M, K], for TN [K, M].
-template <int BMODE, int AMODE>
-cudaError_t LaunchPlanned(const void* a, const void* b, void* out, const void* addend, int M, int N, int K, unsigned int* status, cudaStream_t stream) {
+cudaError_t LaunchGemmGatedDown(const void* a, const void* b, void* out, int M, int N, int K, unsigned int* status, cudaStream_t stream,
+                                const void* addend) {
+  if (M <= kSkinnyRows) return Skinny<false>(a, b, out, nullptr, addend, M, N, K, kActNone, status, stream);
   (void)cudaGetLastError();   // the value returned below must be this launch's own, not an older error of the calling thread
   const uintptr_t all = reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(addend);
-  if (M <= 0 || N <= 0 || K <= 0 || (N % 8) != 0 || (AMODE == 0 ? K % 8 != 0 : M % 8 != 0) || (all & 15) != 0) return cudaErrorInvalidValue;
+  if (M <= 0 || N <= 0 || K <= 0 || (N % 8) != 0 || (K % 8) != 0 || (all & 15) != 0) return cudaErrorInvalidValue;
   const int sm_count = SmCount();
   const GemmTiles tiles = PlanTiles(M, N, K, sm_count);
   const int bn = tiles == kTilesPair128 || (tiles == kTilesSingle && N <= 128) ? 128 : 256;
   CUtensorMap map_a, map_b, map_c;
-  if (!(AMODE == 0 ? MakeMap(&map_a, a, M, K, BM) : MakeMap(&map_a, a, K, M, 64)) ||
-      !(BMODE == 0 ? MakeMap(&map_b, b, N, K, tiles == kTilesSingle ? bn : bn / 2) : MakeMap(&map_b, b, K, N, 64)) || !MakeMap(&map_c, out, M, N, 32))
+  if (!MakeMap(&map_a, a, M, K, BM) || !MakeMap(&map_b, b, N, K, tiles == kTilesSingle ? bn : bn / 2) || !MakeMap(&map_c, out, M, N, 32))
     return cudaErrorInvalidValue;
   __nv_bfloat16* o = static_cast<__nv_bfloat16*>(out);
   const __nv_bfloat16* add = static_cast<const __nv_bfloat16*>(addend);
   auto go = [&](auto epi) {
     constexpr int EPI = decltype(epi)::value;
     if (tiles == kTilesPair256)
-      return LaunchPersistent<256, BMODE, AMODE, EPI, 1>(map_a, map_b, map_c, map_c, o, nullptr, add, M, N, K, 0, 1, sm_count, status, stream);
+      return LaunchPersistent<256, 0, 0, EPI, 1>(map_a, map_b, map_c, map_c, o, nullptr, add, M, N, K, 0, 1, sm_count, status, stream);
     if (tiles == kTilesPair128)
-      return LaunchPersistent<128, BMODE, AMODE, EPI, 1>(map_a, map_b, map_c, map_c, o, nullptr, add, M, N, K, 0, 1, sm_count, status, stream);
-    if (bn == 256) return LaunchPersistent<256, BMODE, AMODE, EPI>(map_a, map_b, map_c, map_c, o, nullptr, add, M, N, K, 0, 1, sm_count, status, stream);
-    return LaunchPersistent<128, BMODE, AMODE, EPI>(map_a, map_b, map_c, map_c, o, nullptr, add, M, N, K, 0, 1, sm_count, status, stream);
+      return LaunchPersistent<128, 0, 0, EPI, 1>(map_a, map_b, map_c, map_c, o, nullptr, add, M, N, K, 0, 1, sm_count, status, stream);
+    if (bn == 256) return LaunchPersistent<256, 0, 0, EPI>(map_a, map_b, map_c, map_c, o, nullptr, add, M, N, K, 0, 1, sm_count, status, stream);
+    return LaunchPersistent<128, 0, 0, EPI>(map_a, map_b, map_c, map_c, o, nullptr, add, M, N, K, 0, 1, sm_count, status, stream);
   };
-  cudaError_t e;
-  if constexpr (BMODE == 0) e = add != nullptr ? go(std::integral_constant<int, kEpiAddAux>()) : go(std::integral_constant<int, kEpiNone>());
-  else e = add != nullptr ? cudaErrorInvalidValue : go(std::integral_constant<int, kEpiNone>());
+  const cudaError_t e = add != nullptr ? go(std::integral_constant<int, kEpiAddAux>()) : go(std::integral_constant<int, kEpiNone>());
   if (e != cudaSuccess) return e;
   CountKernelLaunch();
   return cudaGetLastError();
 }
 
-cudaError_t LaunchGemmGatedDown(const void* a, const void* b, void* out, int M, int N, int K, unsigned int* status, cudaStream_t stream,
-                                const void* addend) {
-  if (M <= kSkinnyRows) return Skinny<false>(a, b, out, nullptr, addend, M, N, K, kActNone, status, stream);
-  return LaunchPlanned<0, 0>(a, b, out, addend, M, N, K, status, stream);
-}
-cudaError_t LaunchGemmGatedInput(const void* a, const void* b, void* out, int M, int N, int K, unsigned int* status, cudaStream_t stream) {
-  return LaunchPlanned<1, 0>(a, b, out, nullptr, M, N, K, status, stream);
-}
-cudaError_t LaunchGemmGatedWeight(const void* a, const void* b, void* out, int M, int N, int K, unsigned int* status, cudaStream_t stream) {
-  return LaunchPlanned<1, 1>(a, b, out, nullptr, M, N, K, status, stream);
+cudaError_t LaunchGemmGroup(const GemmGroupItem* list, int count, unsigned int* status, cudaStream_t stream) {
+  (void)cudaGetLastError();
+  if (count < 1 || count > kMaxGroup) return cudaErrorInvalidValue;
+  // the longest reductions first
+  const GemmGroupItem* by_length[kMaxGroup];
+  for (int i = 0; i < count; ++i) by_length[i] = list + i;
+  std::stable_sort(by_length, by_length + count, [](const GemmGroupItem* x, const GemmGroupItem* y) { return x->K > y->K; });
+  GroupArgs args;
+  args.items = 0;
+  for (int i = 0; i < kMaxGroup; ++i) {
+    if (i >= count) {
+      args.p[i] = {0, 0, 0, 1, 1, INT_MAX, 0};
+      continue;
+    }
+    const GemmGroupItem& g = *by_length[i];
+    const uintptr_t all = reinterpret_cast<uintptr_t>(g.a) | reinterpret_cast<uintptr_t>(g.b) | reinterpret_cast<uintptr_t>(g.out);
+    if (g.M <= 0 || g.N <= 0 || g.K <= 0 || g.N % 8 != 0 || (g.a_transposed ? g.M : g.K) % 8 != 0 || (all & 15) != 0) return cudaErrorInvalidValue;
+    if (!(g.a_transposed ? MakeMap(&args.a[i], g.a, g.K, g.M, 64) : MakeMap(&args.a[i], g.a, g.M, g.K, BM)) ||
+        !MakeMap(&args.b[i], g.b, g.K, g.N, 64) || !MakeMap(&args.c[i], g.out, g.M, g.N, 32))
+      return cudaErrorInvalidValue;
+    args.p[i] = {g.M, g.N, (g.K + BK - 1) / BK, (g.M + 255) / 256, (g.N + 255) / 256, args.items, g.a_transposed ? 1 : 0};
+    args.items += args.p[i].tiles_m * args.p[i].tiles_n;
+  }
+  for (int i = count; i < kMaxGroup; ++i) args.a[i] = args.b[i] = args.c[i] = args.a[0];
+  using Cfg = PersistentCfg<256, kEpiNone, 1>;
+  constexpr int kMaxDevices = 64;
+  static bool attr_set[kMaxDevices] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev >= kMaxDevices || !attr_set[dev]) {
+    e = cudaFuncSetAttribute(gemm_bf16_group_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Cfg::kSmem));
+    if (e != cudaSuccess) return e;
+    if (dev < kMaxDevices) attr_set[dev] = true;
+  }
+  const int pairs = std::min(args.items, SmCount() / 2);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs));
+  cfg.blockDim = dim3(Cfg::kThreadsP);
+  cfg.dynamicSmemBytes = Cfg::kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, gemm_bf16_group_kernel, args, status);
+  if (e != cudaSuccess) return e;
+  CountKernelLaunch();
+  return cudaGetLastError();
 }
 
 cudaError_t LaunchGemmBf16NT(const void* a, const void* b, void* out, const void* bias, int M, int N, int K, int act,

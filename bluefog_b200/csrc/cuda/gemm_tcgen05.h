@@ -39,16 +39,22 @@ cudaError_t LaunchGemmBf16NN(const void* a, const void* b, void* out, int M, int
 cudaError_t LaunchGemmBf16TN(const void* a, const void* b, void* out, int M, int N, int K, unsigned int* status,
                              cudaStream_t stream);
 
-// The other products of a gated feed-forward block, on tiles chosen for their size.  Up to kSkinnyRows rows the forward products
-// share their reductions between clusters of CTAs.
-//   down    out[M,N] = a[M,K] * b[N,K]^T (+ addend[M,N]);  K % 8 == 0, N % 8 == 0
-//   input   out[M,N] = a[M,K] * b[K,N];                    K % 8 == 0, N % 8 == 0
-//   weight  out[M,N] = a[K,M]^T * b[K,N];                  M % 8 == 0, N % 8 == 0
+// The down projection of a gated feed-forward block, out[M,N] = a[M,K] * b[N,K]^T (+ addend[M,N]), on tiles chosen for its size;
+// up to kSkinnyRows rows its reduction (and that of LaunchGemmBf16Gated) is shared between clusters of CTAs.  K, N % 8 == 0.
 constexpr int kSkinnyRows = 64;
 cudaError_t LaunchGemmGatedDown(const void* a, const void* b, void* out, int M, int N, int K, unsigned int* status, cudaStream_t stream,
                                 const void* addend = nullptr);
-cudaError_t LaunchGemmGatedInput(const void* a, const void* b, void* out, int M, int N, int K, unsigned int* status, cudaStream_t stream);
-cudaError_t LaunchGemmGatedWeight(const void* a, const void* b, void* out, int M, int N, int K, unsigned int* status, cudaStream_t stream);
+
+// One to three independent products in one launch: out[M,N] = A * b[K,N] with A = a[M,K], or a[K,M]^T when a_transposed.  N % 8
+// == 0, and K % 8 == 0 (M % 8 == 0 when a_transposed).
+struct GemmGroupItem {
+  const void* a;
+  const void* b;
+  void* out;
+  int M, N, K;
+  bool a_transposed;
+};
+cudaError_t LaunchGemmGroup(const GemmGroupItem* list, int count, unsigned int* status, cudaStream_t stream);
 
 // h[M,F] = act(a[M,K] * w[0:F,K]^T) * (a * w[F:2F,K]^T), act kActSilu or kActGeluTanh; K % 8 == 0, F % 8 == 0.  factors
 // (optional, [M,2F] 16-bit words): receives act(G) and U act'(G) in a format of their own, for the gradient.
