@@ -961,7 +961,7 @@ gemm_bf16_nt_persistent_kernel(const __grid_constant__ CUtensorMap map_a, const 
 // ------------------------------------------------------------------------------------------ //
 // Up to three products in one launch of the two-SM kernel (256 x 256 tiles): the input gradient and both weight gradients of a
 // gated block do not depend on one another, and as launches of their own each ends in a wave that leaves SM pairs idle (8192 x
-// 1024 x 2752: 128, 88 and 44 tiles on 74 pairs, two, two and one wave, 68 + 91 + 50 us; together REPLACE_GROUP us).  The tiles with the
+// 1024 x 2752: 128, 88 and 44 tiles on 74 pairs, two, two and one wave, 68 + 91 + 50 us; together 161 us).  The tiles with the
 // longest reductions come first.  B is [reduction, N] row-major in all of them; A is [M, reduction] or, for a weight
 // gradient, [reduction, M].
 // ------------------------------------------------------------------------------------------ //
@@ -1064,30 +1064,36 @@ gemm_bf16_group_kernel(const __grid_constant__ GroupArgs args, unsigned int* __r
         if (!ok) break;
         fence_after_sync();
         const uint32_t tmem_d = tmem_base + uint32_t(acc * 256);
-        const uint32_t idesc = Cfg::kIdesc | (a_mn ? 1u << 15 : 0u) | (1u << 16);
-        const uint64_t a_step = a_mn ? (16 * 128) >> 4 : 2;
-        for (int kb = 0; kb < num_kb; ++kb, ++it) {
-          const int s = it % S;
-          ok = mbar_wait(smem_u32(&bars[s]), (it / S) & 1, failed);
-          if (!ok) break;
-          const uint32_t a_addr = smem_u32(stage_a + size_t(s) * Cfg::kBytesA);
-          const uint64_t adesc = a_mn ? make_desc_mn(a_addr, 8192, 1024) : make_desc(a_addr);
-          const uint64_t bdesc = make_desc_mn(smem_u32(stage_b + size_t(s) * Cfg::kBytesB), 8192, 1024);
-          if (elect_one()) {
+        // with the operand's layout known to the compiler: read from a table, it would leave the descriptors out of uniform registers
+        auto reduce = [&](auto layout) {
+          constexpr bool A_MN = decltype(layout)::value;
+          constexpr uint32_t idesc = Cfg::kIdesc | (A_MN ? 1u << 15 : 0u) | (1u << 16);
+          constexpr uint64_t a_step = A_MN ? (16 * 128) >> 4 : 2;
+          for (int kb = 0; kb < num_kb; ++kb, ++it) {
+            const int s = it % S;
+            ok = mbar_wait(smem_u32(&bars[s]), (it / S) & 1, failed);
+            if (!ok) break;
+            const uint32_t a_addr = smem_u32(stage_a + size_t(s) * Cfg::kBytesA);
+            const uint64_t adesc = A_MN ? make_desc_mn(a_addr, 8192, 1024) : make_desc(a_addr);
+            const uint64_t bdesc = make_desc_mn(smem_u32(stage_b + size_t(s) * Cfg::kBytesB), 8192, 1024);
+            if (elect_one()) {
 #pragma unroll
-            for (int k = 0; k < BK / kUmmaK; ++k)
-              asm volatile(
-                  "{\n\t.reg .pred p;\n\t"
-                  "setp.ne.b32 p, %4, 0;\n\t"
-                  "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5, %5, %5, %5, %5}, p;\n\t}"
-                  ::"r"(tmem_d), "l"(adesc + a_step * uint64_t(k)), "l"(bdesc + uint64_t(128 * k)), "r"(idesc),
-                    "r"((kb | k) != 0 ? 1u : 0u), "r"(0u)
-                  : "memory");
-            umma_commit_pair(smem_u32(&bars[S + s]));
-            if (kb == num_kb - 1) umma_commit_pair(smem_u32(&bars[2 * S + acc]));
+              for (int k = 0; k < BK / kUmmaK; ++k)
+                asm volatile(
+                    "{\n\t.reg .pred p;\n\t"
+                    "setp.ne.b32 p, %4, 0;\n\t"
+                    "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5, %5, %5, %5, %5}, p;\n\t}"
+                    ::"r"(tmem_d), "l"(adesc + a_step * uint64_t(k)), "l"(bdesc + uint64_t(128 * k)), "r"(idesc),
+                      "r"((kb | k) != 0 ? 1u : 0u), "r"(0u)
+                    : "memory");
+              umma_commit_pair(smem_u32(&bars[S + s]));
+              if (kb == num_kb - 1) umma_commit_pair(smem_u32(&bars[2 * S + acc]));
+            }
+            __syncwarp();
           }
-          __syncwarp();
-        }
+        };
+        if (a_mn) reduce(std::true_type());
+        else reduce(std::false_type());
       }
     }
   } else {
