@@ -600,6 +600,7 @@ struct BwdCfg {
   static constexpr uint32_t kYBytes = kBoxes * kN * 128;               // each of the two streamed tiles of a stage
   static constexpr int kStages = 4;
   static constexpr int kSets = DP == 64 ? 1 : 2;
+  static constexpr bool kEarly = kSets == 1;                           // see the products
   static constexpr int kWarps = 8 * kSets;                             // those that take exponentials
   static constexpr int kThreads = 32 * (kWarps + 2);
   static constexpr int kCtasPerSm = DP == 64 ? 2 : 1;
@@ -653,7 +654,7 @@ __device__ __forceinline__ void attn_bwd_body(const CUtensorMap* map_q, const CU
   unsigned char* smem_x = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   unsigned char* ring = smem_x + 2 * Cfg::kXBytes;
   float* ring_stats = reinterpret_cast<float*>(ring + size_t(NS) * 2 * Cfg::kYBytes);      // KV: per stage -lse[64], -delta[64]
-  __shared__ uint64_t bars[2 * NS + 3 + 3 * SETS];
+  __shared__ uint64_t bars[2 * NS + 3 + 4 * SETS];
   __shared__ uint32_t tmem_base_s;
   __shared__ int failed_s;
   volatile int* failed = &failed_s;
@@ -661,9 +662,11 @@ __device__ __forceinline__ void attn_bwd_body(const CUtensorMap* map_q, const CU
   const uint32_t bar_x = bar0 + 8u * (2 * NS), bar_xa = bar_x + 8u, bar_end = bar_x + 16u;
   auto full = [&](int s) { return bar0 + 8u * s; };
   auto empty = [&](int s) { return bar0 + 8u * (NS + s); };
-  auto bar_s = [&](int set) { return bar_x + 24u + 24u * set; };
-  auto bar_dp = [&](int set) { return bar_x + 32u + 24u * set; };
-  auto bar_ds = [&](int set) { return bar_x + 40u + 24u * set; };
+  // bar_p: the scores' place may be used, KV: as the operand P that replaced them, otherwise for the next scores
+  auto bar_s = [&](int set) { return bar_x + 24u + 32u * set; };
+  auto bar_dp = [&](int set) { return bar_x + 32u + 32u * set; };
+  auto bar_p = [&](int set) { return bar_x + 40u + 32u * set; };
+  auto bar_ds = [&](int set) { return bar_x + 48u + 32u * set; };
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // KV: `split` CTAs of a cluster (a power of two) share a tile, each with its part of the group's query heads
@@ -723,6 +726,7 @@ __device__ __forceinline__ void attn_bwd_body(const CUtensorMap* map_q, const CU
     for (int k = 0; k < SETS; ++k) {
       mbar_init(bar_s(k), 1);
       mbar_init(bar_dp(k), 1);
+      mbar_init(bar_p(k), 8);
       mbar_init(bar_ds(k), 8);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -785,33 +789,54 @@ __device__ __forceinline__ void attn_bwd_body(const CUtensorMap* map_q, const CU
       }
       return true;
     };
-    // scores and dP of an iteration, over the operands of the set's tile before: products run in the order of issue
-    auto products = [&](int it) {
+    // Scores and dP of an iteration replace the operands of the set's tile before; products run in the order of issue.  With one
+    // set the next scores are issued as soon as their place is free (kEarly), so that the set finds them ready when it has
+    // written dS, and its exponentials cover the way of dS through the products and of the next dP (8192 tokens, heads of 64: 572
+    // -> 519 us).  With two sets, whose products fill that time, the additional hand-over costs (heads of 128: 829 -> 898 us).
+    auto scores = [&](int it) {
       const uint32_t y = smem_u32(stage(it));
       if (KV) mma_scores<DP, N>(s_col(it), x0, y);
       else mma_scores_ts<DP, N>(s_col(it), tmem + Cfg::kColX, y);
       umma_commit(bar_s(it % SETS));
-      if (KV) mma_scores<DP, N>(s_col(it) + N, x1, y + Cfg::kYBytes);
-      else mma_scores_ts<DP, N>(s_col(it) + N, tmem + Cfg::kColX + DP / 2, y + Cfg::kYBytes);
+    };
+    auto grad_scores = [&](int it) {
+      const uint32_t y = smem_u32(stage(it)) + Cfg::kYBytes;
+      if (KV) mma_scores<DP, N>(s_col(it) + N, x1, y);
+      else mma_scores_ts<DP, N>(s_col(it) + N, tmem + Cfg::kColX + DP / 2, y);
       umma_commit(bar_dp(it % SETS));
     };
     for (int it = 0; it < SETS && it < n && ok; ++it) {
       ok = tiles(it);
-      if (ok && elect_one()) products(it);
+      if (ok && elect_one()) {
+        scores(it);
+        grad_scores(it);
+      }
       __syncwarp();
     }
     for (int it = 0; it < n && ok; ++it) {
       const bool more = it + SETS < n;
+      const uint32_t phase = (it / SETS) & 1;
       // the next tiles have arrived long ago; looked at here, their barrier is not between the operands and the products
-      ok = (!more || tiles(it + SETS)) && mbar_wait(bar_ds(it % SETS), (it / SETS) & 1, failed);
+      ok = !more || tiles(it + SETS);
+      if (Cfg::kEarly) {
+        ok = ok && mbar_wait(bar_p(it % SETS), phase, failed);
+        if (!ok) break;
+        fence_after_sync();
+        if (elect_one()) {
+          if (KV) mma_accumulate<DP, N>(tmem + Cfg::kCol0, s_col(it), 32, smem_u32(stage(it)) + Cfg::kYBytes, it == 0);
+          if (more) scores(it + SETS);
+        }
+        __syncwarp();
+      }
+      ok = ok && mbar_wait(bar_ds(it % SETS), phase, failed);
       if (!ok) break;
       fence_after_sync();
       if (elect_one()) {
-        const uint32_t y = smem_u32(stage(it));
-        if (KV) mma_accumulate<DP, N>(tmem + Cfg::kCol0, s_col(it), 32, y + Cfg::kYBytes, it == 0);
-        mma_accumulate<DP, N>(tmem + Cfg::kCol1, s_col(it) + N, 32, y, it == 0);
+        if (KV && !Cfg::kEarly) mma_accumulate<DP, N>(tmem + Cfg::kCol0, s_col(it), 32, smem_u32(stage(it)) + Cfg::kYBytes, it == 0);
+        mma_accumulate<DP, N>(tmem + Cfg::kCol1, s_col(it) + N, 32, smem_u32(stage(it)), it == 0);
         umma_commit(empty(it % NS));
-        if (more) products(it + SETS);
+        if (!Cfg::kEarly && more) scores(it + SETS);
+        if (more) grad_scores(it + SETS);
       }
       __syncwarp();
     }
@@ -890,6 +915,11 @@ __device__ __forceinline__ void attn_bwd_body(const CUtensorMap* map_q, const CU
       tmem_ld_16x256b_x4(tS + kUpper, r + 16);
       tmem_wait_ld();
       tie32(r);
+      if (Cfg::kEarly && !KV) {
+        fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_p(set));
+      }
       float p[32];
 #pragma unroll
       for (int i = 0; i < 32; i += 2)
@@ -911,6 +941,12 @@ __device__ __forceinline__ void attn_bwd_body(const CUtensorMap* map_q, const CU
         for (int i = 0; i < 16; ++i) pk[i] = pack_bf16(p[2 * i], p[2 * i + 1]);
         tmem_st_16x128b_x4(tS, pk);
         tmem_st_16x128b_x4(tS + kUpper, pk + 8);
+        if (Cfg::kEarly) {
+          tmem_wait_st();
+          fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar_p(set));
+        }
       }
       ok = mbar_wait(bar_dp(set), phase, failed);
       if (!ok) break;
