@@ -125,22 +125,24 @@ __device__ __forceinline__ float gate_fn(float x, int act, float* grad) {
   return y;
 }
 // What a gated block keeps for its backward pass, 16 bits each: act(g) and u act'(g), the factors of dH in dU and dG.  Their format
-// has a sign, six bits of exponent (2^-30 to 2^32, smaller values become zero, larger ones the largest) and nine of mantissa:
-// each is off by at most 2^-10 of itself.  Kept in bf16, their rounding, that of dG and dU and that of the gradients
-// themselves made the gradients of the input and of the gate and up weights 1.8 times as far from exact ones as the last
-// rounding alone does; now it is 1.4 times.  Scaled by 2^-96 the exponent of an fp32 number has two leading zeros.
-constexpr float kFactorScale = 1.262177448353618888658765704452e-29f;          // 2^-96
+// has a sign, six bits of exponent (2^-36 to 2^27; smaller values become zero, what is larger, infinite or not a number becomes
+// the largest code, which reads as NaN) and nine of mantissa: each is off by at most 2^-10 of itself.  Kept in bf16, their
+// rounding, that of dG and dU and that of the gradients themselves made the gradients of the input and of the gate and up
+// weights 1.8 times as far from exact ones as the last rounding alone does; now it is 1.4 times.  Scaled by 2^-90 the exponent
+// of an fp32 number in this range has two leading zeros.
+constexpr float kFactorScale = 8.077935669463161e-28f;                         // 2^-90
 __device__ __forceinline__ uint32_t pack_factors(float lo, float hi) {
   const uint32_t a = __float_as_uint(lo * kFactorScale), b = __float_as_uint(hi * kFactorScale);
   const uint32_t ma = min((a & 0x7fffffffu) + 0x2000u, 0x1fffffffu) >> 14, mb = min((b & 0x7fffffffu) + 0x2000u, 0x1fffffffu) >> 14;
   return ((a >> 16) & 0x8000u) | ma | (b & 0x80000000u) | (mb << 16);
 }
-// The factors in a word, times 2^-96.
+// The factors in a word, times 2^-90.
 __device__ __forceinline__ float2 unpack_factors(uint32_t w) {
   return make_float2(__uint_as_float(((w << 16) & 0x80000000u) | ((w << 14) & 0x1fffc000u)),
                      __uint_as_float((w & 0x80000000u) | ((w >> 2) & 0x1fffc000u)));
 }
-constexpr float kFactorUnscale = 7.9228162514264337593543950336e28f;           // 2^96
+constexpr float kFactorUnscale = 1.2379400392853803e27f;                       // 2^90
+constexpr uint32_t kFactorNan = 0x7fffu;
 
 // eight floats as bf16, 16 bytes
 __device__ __forceinline__ uint4 pack8(const float* v) {
@@ -688,14 +690,26 @@ gemm_bf16_nt_persistent_kernel(const __grid_constant__ CUtensorMap map_a, const 
             const uint4 fv = *reinterpret_cast<const uint4*>(box + off), dv = *reinterpret_cast<const uint4*>(box + 2048 + off);
             const uint32_t f[4] = {fv.x, fv.y, fv.z, fv.w}, d[4] = {dv.x, dv.y, dv.z, dv.w};
             float a[8], b[8];
+            uint32_t top = 0u;                                 // largest codes of the upper and lower halves
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
+              top = __vmaxu2(top, __vmaxu2(f[i] & 0x7fff7fffu, d[i] & 0x7fff7fffu));
               const float h0 = __uint_as_float(r[j * 8 + 2 * i]) * kFactorUnscale, h1 = __uint_as_float(r[j * 8 + 2 * i + 1]) * kFactorUnscale;
               const float2 x = unpack_factors(f[i]), y = unpack_factors(d[i]);
               b[2 * i] = h0 * x.x;
               b[2 * i + 1] = h1 * x.y;
               a[2 * i] = h0 * y.x;
               a[2 * i + 1] = h1 * y.y;
+            }
+            if ((top & 0xffffu) == kFactorNan || top >> 16 == kFactorNan) {       // rare
+              const float nan = __uint_as_float(0x7fffffffu);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                if ((f[i] & 0x7fffu) == kFactorNan) b[2 * i] = nan;
+                if ((f[i] >> 16 & 0x7fffu) == kFactorNan) b[2 * i + 1] = nan;
+                if ((d[i] & 0x7fffu) == kFactorNan) a[2 * i] = nan;
+                if ((d[i] >> 16 & 0x7fffu) == kFactorNan) a[2 * i + 1] = nan;
+              }
             }
             dg[j] = pack8(a);
             du[j] = pack8(b);

@@ -261,7 +261,8 @@ def gated_mlp(a: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor, ac
     """``(act(a @ Wg.T) * (a @ Wu.T)) @ w_down.T (+ residual)`` with ``w_gate_up`` = [Wg; Wu] ``[2 F, K]`` and ``w_down``
     ``[N, F]``; ``a`` [.., K], ``residual`` [.., N]; ``act`` "silu" or "gelu" (the tanh approximation).  bf16 CUDA tensors
     with K, F and N multiples of 8 take the tcgen05 kernels, the activation and the product with the gate inside GEMM
-    epilogues in both directions; other inputs take PyTorch's ops."""
+    epilogues in both directions; other inputs take PyTorch's ops.  The kernels keep ``act(g)`` and ``u act'(g)`` for the
+    backward pass in 16 bits each: what is below 2^-36 counts as zero there, and what reaches 2^27 makes gradients NaN."""
     if act not in _GATES:
         raise ValueError("gated_mlp: act has to be one of %s, got %r" % (sorted(_GATES), act))
     if (a.dim() < 1 or w_gate_up.dim() != 2 or w_down.dim() != 2 or w_gate_up.shape[1] != a.shape[-1]

@@ -151,3 +151,34 @@ def test_gradient_against_differences():
         _, tol = _oracle(x, wgu, wd, dy, None, act)
         bound = math.sqrt(sum((t * s).square().sum().item() for t, s in zip(tol[1:], steps)))       # independent roundings
         assert abs(got - want) <= 4 * bound + 1e-6 * abs(want)
+
+
+@pytest.mark.parametrize("m", [40, 200])
+def test_what_the_kept_factors_cannot_hold(m):
+    """Rows with NaN, infinite or huge pre-activations have gradients that are no numbers; the other rows keep theirs."""
+    from bluefog_b200.ops import gemm
+    x, wgu, wd, dy, _ = _inputs(m, 64, 72, 64, False)
+
+    def da(a):
+        a = a.clone().requires_grad_(True)
+        return torch.autograd.grad(gemm.gated_mlp(a, wgu, wd), a, dy)[0]
+
+    want = da(x)
+    bad = x.clone()
+    bad[3, 5], bad[17, 0], bad[38] = math.nan, math.inf, x[38] * 1e12
+    got = da(bad)
+    rows = torch.ones(m, dtype=torch.bool, device="cuda")
+    rows[[3, 17, 38]] = False
+    assert torch.equal(got[rows], want[rows]) and torch.isfinite(want).all()
+    assert got[~rows].isnan().all()
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -26, 2.0 ** 18])
+def test_small_and_large_activations(scale):
+    from bluefog_b200.ops import gemm
+    x, wgu, wd, dy, _ = _inputs(150, 64, 136, 64, False)
+    leaves = [(x * scale).requires_grad_(True), wgu.clone().requires_grad_(True), wd.clone().requires_grad_(True)]
+    got = torch.autograd.grad(gemm.gated_mlp(*leaves), leaves, dy)
+    want, _ = _oracle(leaves[0], wgu, wd, dy, None, "silu")
+    for g, w in zip(got, want[1:]):
+        assert ((g.double() - w).norm() / w.norm()).item() < 4 * U
