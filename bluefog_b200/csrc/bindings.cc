@@ -31,11 +31,10 @@
 namespace py = pybind11;
 using namespace bfb;
 
-// One device word per process that the GEMM kernel sets when a bounded wait expired.
+// The word that the GEMM kernel sets when a bounded wait expired.
 at::Tensor& bfb::GemmStatusWord(const at::Tensor& like) {
-  static at::Tensor status;
-  if (!status.defined()) status = at::zeros({1}, like.options().dtype(at::kInt));
-  return status;
+  static StatusWords words;
+  return StatusTensor(words, like.get_device());
 }
 
 namespace {

@@ -5,11 +5,9 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
-
-#include <map>
-#include <mutex>
 
 #include "cuda/attn_tcgen05.h"
 #include "cuda/dropout_kernels.h"
@@ -335,13 +333,25 @@ struct GatedMlpNode : public torch::autograd::Function<GatedMlpNode> {
 
 }  // namespace
 
+at::Tensor& StatusTensor(StatusWords& words, int device) {
+  std::lock_guard<std::mutex> lock(words.mu);
+  at::Tensor& w = words.of_device[device];
+  if (!w.defined()) {
+    const c10::cuda::CUDAGuard guard(device);
+    // A first call inside a capture: the word must neither lie in the graph's memory nor be cleared by every replay.  Nothing that
+    // is captured runs before the capture ends, so this clearing has no need to be waited for.
+    c10::cuda::CUDAStreamCaptureModeGuard mode(cudaStreamCaptureModeRelaxed);
+    c10::cuda::OptionalCUDAStreamGuard side;
+    if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None)
+      side.reset_stream(c10::cuda::getStreamFromPool(false, device));
+    w = at::zeros({1}, at::TensorOptions().device(at::kCUDA, device).dtype(at::kInt));
+  }
+  return w;
+}
+
 unsigned int* AttnStatusWord(int device) {
-  static std::mutex mu;
-  static std::map<int, at::Tensor> words;
-  std::lock_guard<std::mutex> lock(mu);
-  at::Tensor& w = words[device];
-  if (!w.defined()) w = at::zeros({1}, at::TensorOptions().device(at::kCUDA, device).dtype(at::kInt));
-  return reinterpret_cast<unsigned int*>(w.data_ptr<int>());
+  static StatusWords words;
+  return reinterpret_cast<unsigned int*>(StatusTensor(words, device).data_ptr<int>());
 }
 
 at::Tensor CausalAttention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const c10::optional<at::Tensor>& cu, double scale) {

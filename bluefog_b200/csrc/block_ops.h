@@ -2,6 +2,9 @@
 #pragma once
 #include <ATen/ATen.h>
 
+#include <map>
+#include <mutex>
+
 namespace bfb {
 
 // Arguments are checked by the callers in bluefog_b200/ops; what the kernels rely on is checked again here.  All take CUDA
@@ -18,7 +21,14 @@ at::Tensor DropoutAdd(const at::Tensor& x, const c10::optional<at::Tensor>& resi
 at::Tensor GatedMlp(const at::Tensor& a, const at::Tensor& w_gate_up, const at::Tensor& w_down, int64_t act,
                     const c10::optional<at::Tensor>& residual);
 
-// Device word of the attention kernels on a device (bits: AttnStatus), and the one that the GEMM kernels share.
+// A word of status bits on every device that was asked for, zero at first.
+struct StatusWords {
+  std::mutex mu;
+  std::map<int, at::Tensor> of_device;
+};
+at::Tensor& StatusTensor(StatusWords& words, int device);
+
+// That of the attention kernels (bits: AttnStatus), and the one that the GEMM kernels share.
 unsigned int* AttnStatusWord(int device);
 at::Tensor& GemmStatusWord(const at::Tensor& like);
 

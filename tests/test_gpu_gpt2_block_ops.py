@@ -6,6 +6,8 @@ off by at most 2^-8 of the value and independent of the others, and between the 
 passes about 16 of them per layer; two layers and the classifier give sqrt(2 * 2 * 16 + 8) * 2^-8 = 0.033.  Twice that is
 allowed, since LayerNorm and the residual stream weigh them unevenly."""
 import math
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -81,3 +83,42 @@ def test_captured_training_step_repeats_the_eager_one():
                 torch.testing.assert_close(a.float(), b.float(), rtol=2.0 ** -7, atol=1e-3 * b.float().abs().max().item())
             else:
                 assert torch.equal(a, b), n
+
+
+_FIRST_CALL = """
+import torch
+from bluefog_b200 import _C
+from bluefog_b200.ops import fused_attention as fa, gemm
+torch.manual_seed(0)
+mk = lambda *s: torch.randn(*s, device="cuda").to(torch.bfloat16)
+qkv, wgu, wd, dy = mk(200, 3 * 128), mk(2 * 136, 128), mk(64, 136), mk(200, 64)
+cu = torch.tensor([0, 77, 200], dtype=torch.int32, device="cuda")
+
+def step(leaves):
+    out = fa.causal_self_attention(leaves[0], 2, cu_seqlens=cu)
+    y = gemm.gated_mlp(out.view(200, 128), *leaves[1:])
+    return [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+
+leaves = [t.clone().requires_grad_(True) for t in (qkv, wgu, wd)]
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = step(leaves)
+fa.check_sequences()
+assert _C.gemm_status() == 0
+want = step([t.clone().requires_grad_(True) for t in (qkv, wgu, wd)])
+for _ in range(2):
+    graph.replay()
+assert all(torch.equal(a, b) for a, b in zip(got, want))
+# what one call reports, a replay does not take back
+fa.causal_self_attention(qkv, 2, cu_seqlens=torch.tensor([0, 150, 120], dtype=torch.int32, device="cuda"))
+graph.replay()
+try:
+    fa.check_sequences()
+except IndexError:
+    print("reported")
+"""
+
+
+def test_first_calls_of_a_process_in_a_capture():
+    run = subprocess.run([sys.executable, "-c", _FIRST_CALL], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and "reported" in run.stdout, run.stdout + run.stderr
