@@ -42,6 +42,8 @@ bool NeedsGrad(std::initializer_list<at::Tensor> tensors) {
 // Gradients of these operators are not differentiable; asking for theirs is an error, at the time they are asked for.
 variable_list Once(const char* what, variable_list grads) {
   if (!at::GradMode::is_enabled()) return grads;
+  for (at::Tensor& g : grads)
+    if (g.defined()) g.requires_grad_(true);                           // or they would pass for constants
   auto node = std::make_shared<torch::autograd::DelayedError>(std::string(what) + " can be differentiated only once",
                                                              static_cast<int64_t>(grads.size()));
   return (*node)(std::move(grads));

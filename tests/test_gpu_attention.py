@@ -255,3 +255,14 @@ def test_offsets_past_32_bits():
         out = fa.causal_attention(*(big[:, i * d:(i + 1) * d].unsqueeze(1) for i in range(3)), cu_seqlens=_cu(lengths))
         want = fa.causal_attention(*(small[:, i * d:(i + 1) * d].unsqueeze(1) for i in range(3)), cu_seqlens=_cu(lengths))
     assert torch.equal(out, want)
+
+
+def test_gradients_of_gradients_are_refused():
+    from bluefog_b200.ops import fused_attention as fa
+    q, k, v, dout = _inputs(60, 2, 2, 64)
+    q.requires_grad_(True)
+    qkv = torch.randn(60, 3 * 128, device="cuda").to(torch.bfloat16).requires_grad_(True)
+    for leaf, out in ((q, fa.causal_attention(q, k, v)), (qkv, fa.causal_self_attention(qkv, 2))):
+        (g,) = torch.autograd.grad(out, leaf, dout.view(out.shape), create_graph=True)
+        with pytest.raises(RuntimeError, match="only once"):
+            g.float().sum().backward()

@@ -182,3 +182,13 @@ def test_small_and_large_activations(scale):
     want, _ = _oracle(leaves[0], wgu, wd, dy, None, "silu")
     for g, w in zip(got, want[1:]):
         assert ((g.double() - w).norm() / w.norm()).item() < 4 * U
+
+
+def test_gradients_of_gradients_are_refused():
+    from bluefog_b200.ops import gemm
+    x, wgu, wd, dy, _ = _inputs(40, 64, 72, 64, False)
+    x.requires_grad_(True)
+    wd.requires_grad_(True)                                           # wgu stays frozen: its gradient is not there
+    g, h = torch.autograd.grad(gemm.gated_mlp(x, wgu, wd), [x, wd], dy, create_graph=True)
+    with pytest.raises(RuntimeError, match="only once"):
+        (g.float().sum() + h.float().sum()).backward()
