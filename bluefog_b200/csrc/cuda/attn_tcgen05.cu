@@ -4,14 +4,13 @@
 //   backward  delta = rowsum(dout * out),  dP = dout v^T,  dS = P (dP - delta)
 //             dv = P^T dout (summed over the query heads of a group),  dk = scale dS^T q (ditto),  dq = scale dS k
 //
-// Every kernel works on tiles of 128 queries x 128 keys, one row of the score tile per thread, and never writes a score
-// to memory.  The backward pass has two kinds of CTAs: those that own a key tile (dk, dv) and those that own a query tile (dq),
-// seven products per tile instead of five, but no atomics, so gradients do not depend on the order in which CTAs run, and
-// no fp32 copy of dq.
+// No kernel writes a score to memory: a CTA keeps 128 queries (or keys) and walks over the others 64 or 128 at a time.  The backward
+// pass has two kinds of CTAs: those that own a key tile (dk, dv) and those that own a query tile (dq), seven products per tile
+// instead of five, but no atomics, so gradients do not depend on the order in which CTAs run, and no fp32 copy of dq.
 //
 // Numbers: scores, row maxima, row sums, all accumulators and the statistics kept for the backward pass are fp32.  P and
-// dS are rounded to bf16 because they are operands of the next product (each rounding is off by at most 2^-9 of the
-// value, the size of the rounding of the result itself).  A row's sum is taken over the unrounded values.
+// dS are rounded to bf16 because they are operands of the next product (each rounding is off by at most 2^-8 of the
+// value, as the rounding of the result itself is).  A row's sum is taken over the unrounded values.
 //
 // Sequences: a tile never crosses a sequence boundary.  Tile slot cu[b] / 128 + b + i belongs to rows [128 i, 128 i + 128)
 // of sequence b; slots of different sequences cannot collide because ceil(len / 128) <= cu[b+1]/128 - cu[b]/128 + 1.  So a
@@ -1119,8 +1118,8 @@ cudaError_t Backward(const AttnShape& s, const CUtensorMap& mq, const CUtensorMa
   // The query heads of a group add to the same key tile.  Up to eight CTAs of a cluster (the portable size) share them and add up
   // their sums through distributed shared memory: without it one CTA walked over all of them, and few key heads left SMs idle
   // (packed documents, four query heads to a key head: 380 against 330 us, forward included).  Three times as many blocks as run
-  // together even out what they differ by; more only add sums.  The query kind then has a
-  // launch of its own, since blocks that need no cluster would still be started as one.
+  // together even out what they differ by; more only add sums.  The query kind then has a launch of its own, since blocks that
+  // need no cluster would still be started as one.
   int split = 1;
   while (split < 8 && g.group % (2 * split) == 0 && g.tiles * s.kv_heads * split < 3 * SmCount() * Cfg::kCtasPerSm) split *= 2;
   const int kv_blocks = g.tiles * s.kv_heads * split, q_blocks = g.tiles * s.heads;
