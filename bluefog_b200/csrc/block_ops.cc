@@ -134,16 +134,24 @@ AttnShape QkvShape(const at::Tensor& qkv, int64_t heads, int64_t kv_heads, const
 at::Tensor StatsFor(const AttnShape& s, const at::Tensor& like) {
   return at::empty({s.heads, AttnTiles(s), 128}, like.options().dtype(at::kFloat));
 }
-float* StatsPtr(const at::Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
+// What the forward pass leaves for the backward pass besides the result.
+struct Kept {
+  at::Tensor stats, low;
+  void Make(const AttnShape& s, const at::Tensor& out) {
+    stats = StatsFor(s, out);
+    low = at::empty(out.sizes(), out.options().dtype(at::kByte));
+  }
+};
+float* StatsPtr(const at::Tensor& t) { return t.data_ptr<float>(); }
 
-at::Tensor SeparateForward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cu, double scale, at::Tensor* stats) {
+at::Tensor SeparateForward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cu, double scale, Kept* kept) {
   TORCH_CHECK(v.sizes() == k.sizes() && k.get_device() == q.get_device() && v.get_device() == q.get_device() &&
               k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(), "attention: q, k and v do not match");
   const AttnShape s = ShapeOf(q, k, cu, scale);
   at::Tensor out = at::empty(q.sizes(), q.options());
-  if (stats != nullptr) *stats = StatsFor(s, q);
-  Check(LaunchAttnForward(s, Described(q), Described(k), Described(v), Described(out), stats != nullptr ? StatsPtr(*stats) : nullptr,
-                          AttnStatusWord(q.get_device()), StreamOf(q)), "attention forward");
+  if (kept != nullptr) kept->Make(s, out);
+  Check(LaunchAttnForward(s, Described(q), Described(k), Described(v), Described(out), kept != nullptr ? Described(kept->low) : AttnTensor(),
+                          kept != nullptr ? StatsPtr(kept->stats) : nullptr, AttnStatusWord(q.get_device()), StreamOf(q)), "attention forward");
   return out;
 }
 
@@ -152,9 +160,9 @@ struct AttentionNode : public torch::autograd::Function<AttentionNode> {
                             const c10::optional<at::Tensor>& boundaries, double scale) {
     const at::Tensor cu = OrUndefined(boundaries);
     const at::Tensor q = Rows(q0), k = Rows(k0), v = Rows(v0);
-    at::Tensor stats;
-    at::Tensor out = SeparateForward(q, k, v, cu, scale, &stats);
-    ctx->save_for_backward({q, k, v, cu, out, stats});
+    Kept kept;
+    at::Tensor out = SeparateForward(q, k, v, cu, scale, &kept);
+    ctx->save_for_backward({q, k, v, cu, out, kept.stats, kept.low});
     ctx->saved_data["scale"] = scale;
     return out;
   }
@@ -166,22 +174,22 @@ struct AttentionNode : public torch::autograd::Function<AttentionNode> {
     const at::Tensor dout = Rows(grads[0]);
     at::Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()), dv = at::empty(v.sizes(), v.options());
     at::Tensor delta = at::empty_like(stats);
-    Check(LaunchAttnBackward(s, Described(q), Described(k), Described(v), Described(out), Described(dout), StatsPtr(stats), StatsPtr(delta),
+    Check(LaunchAttnBackward(s, Described(q), Described(k), Described(v), Described(out), Described(saved[6]), Described(dout), StatsPtr(stats), StatsPtr(delta),
                              Described(dq), Described(dk), Described(dv), AttnStatusWord(q.get_device()), StreamOf(q)), "attention backward");
     variable_list g = Once("attention", {dq, dk, dv});
     return {g[0], g[1], g[2], at::Tensor(), at::Tensor()};
   }
 };
 
-at::Tensor QkvForward(const at::Tensor& qkv, int64_t h, int64_t hkv, const at::Tensor& cu, double scale, at::Tensor* stats) {
+at::Tensor QkvForward(const at::Tensor& qkv, int64_t h, int64_t hkv, const at::Tensor& cu, double scale, Kept* kept) {
   const AttnShape s = QkvShape(qkv, h, hkv, cu, scale);
   std::vector<int64_t> sizes(qkv.sizes().begin(), qkv.sizes().end() - 1);
   sizes.push_back(h);
   sizes.push_back(s.dim);
   at::Tensor out = at::empty(sizes, qkv.options());
-  if (stats != nullptr) *stats = StatsFor(s, qkv);
+  if (kept != nullptr) kept->Make(s, out);
   Check(LaunchAttnForward(s, QkvPart(qkv, 0, s.dim), QkvPart(qkv, h, s.dim), QkvPart(qkv, h + hkv, s.dim), Described(out),
-                          stats != nullptr ? StatsPtr(*stats) : nullptr, AttnStatusWord(qkv.get_device()), StreamOf(qkv)),
+                          kept != nullptr ? Described(kept->low) : AttnTensor(), kept != nullptr ? StatsPtr(kept->stats) : nullptr, AttnStatusWord(qkv.get_device()), StreamOf(qkv)),
         "attention forward");
   return out;
 }
@@ -191,9 +199,9 @@ struct SelfAttentionNode : public torch::autograd::Function<SelfAttentionNode> {
                             double scale) {
     const at::Tensor cu = OrUndefined(boundaries);
     const at::Tensor qkv = QkvRows(qkv0);
-    at::Tensor stats;
-    at::Tensor out = QkvForward(qkv, h, hkv, cu, scale, &stats);
-    ctx->save_for_backward({qkv, cu, out, stats});
+    Kept kept;
+    at::Tensor out = QkvForward(qkv, h, hkv, cu, scale, &kept);
+    ctx->save_for_backward({qkv, cu, out, kept.stats, kept.low});
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["h"] = h;
     ctx->saved_data["hkv"] = hkv;
@@ -207,7 +215,7 @@ struct SelfAttentionNode : public torch::autograd::Function<SelfAttentionNode> {
     const AttnShape s = QkvShape(qkv, h, hkv, saved[1], ctx->saved_data["scale"].toDouble());
     const at::Tensor dout = Rows(grads[0]);
     at::Tensor dqkv = at::empty(qkv.sizes(), qkv.options()), delta = at::empty_like(stats);
-    Check(LaunchAttnBackward(s, QkvPart(qkv, 0, s.dim), QkvPart(qkv, h, s.dim), QkvPart(qkv, h + hkv, s.dim), Described(out), Described(dout),
+    Check(LaunchAttnBackward(s, QkvPart(qkv, 0, s.dim), QkvPart(qkv, h, s.dim), QkvPart(qkv, h + hkv, s.dim), Described(out), Described(saved[4]), Described(dout),
                              StatsPtr(stats), StatsPtr(delta), QkvPart(dqkv, 0, s.dim), QkvPart(dqkv, h, s.dim), QkvPart(dqkv, h + hkv, s.dim),
                              AttnStatusWord(qkv.get_device()), StreamOf(qkv)), "attention backward");
     return {Once("attention", {dqkv})[0], at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};

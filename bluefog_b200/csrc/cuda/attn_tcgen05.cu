@@ -10,7 +10,11 @@
 //
 // Numbers: scores, row maxima, row sums, all accumulators and the statistics kept for the backward pass are fp32.  P and
 // dS are rounded to bf16 because they are operands of the next product (each rounding is off by at most 2^-8 of the
-// value, as the rounding of the result itself is).  A row's sum is taken over the unrounded values.
+// value, as the rounding of the result itself is).  So that delta does not suffer from the rounding of out - it is small against
+// the dP that it is subtracted from only where many keys share the weight -, a forward pass with a backward pass to come
+// also keeps the next eight bits of out (see low_bytes): without them dq and dk of 136 tokens are 1.6 times as far off as their
+// own rounding alone, of 8 tokens 2.2 times, with them 1.45 and 1.5, for 4 of the 154 us of a GPT-2 medium layer.  A row's sum
+// is taken over the unrounded values.
 //
 // Sequences: a tile never crosses a sequence boundary.  Tile slot cu[b] / 128 + b + i belongs to rows [128 i, 128 i + 128)
 // of sequence b; slots of different sequences cannot collide because ceil(len / 128) <= cu[b+1]/128 - cu[b]/128 + 1.  So a
@@ -127,6 +131,22 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   return y;
 }
 
+// Of four fp32 values, times factor, the eight bits that follow those of a bf16 number.  As a signed byte they are to be added to the
+// rounded number in that place: rounding up added the carry that their sign takes back (with_low).  A tie that was rounded
+// down, one value in 2^17, comes out an ulp too small.
+__device__ __forceinline__ uint32_t low_bytes(const uint32_t* v, float factor) {
+  uint32_t b[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) b[i] = __float_as_uint(__uint_as_float(v[i]) * factor);
+  return __byte_perm(__byte_perm(b[0], b[1], 0x0051), __byte_perm(b[2], b[3], 0x0051), 0x5410);
+}
+// byte i of `low` added to a bf16 number in the upper half of its word
+__device__ __forceinline__ float with_low(uint32_t bf16, uint32_t low, int i) {
+  return __uint_as_float(bf16 + static_cast<uint32_t>(static_cast<int>(low << (24 - 8 * i)) >> 16 & ~0xff));
+}
+// where eight of them lie in a box of [128 rows x 64 bytes]
+__device__ __forceinline__ int low_at(int row, int chunk) { return (chunk >> 3) * (kTile * 64) + row * 64 + (((chunk & 7) ^ (row >> 1 & 7)) << 3); }
+
 // two floats in one 64-bit register, and the packed instructions on them
 typedef unsigned long long float2_t;
 __device__ __forceinline__ float2_t pair(float lo, float hi) {
@@ -219,9 +239,10 @@ __device__ __forceinline__ void zero_result(const AttnTensor& t, int head, int r
 }
 
 // One warp's 32 accumulator rows: columns [col0, col0 + 32 NC) of tensor memory are scaled per row, rounded and written to the
-// warp's rows of a staging box (64 columns per box, starting with 16-byte chunk chunk0).
+// warp's rows of a staging box (64 columns per box, starting with 16-byte chunk chunk0); their next bits go to `low`, boxes of
+// 128 rows of 64 bytes, where that is given.
 template <int NC>
-__device__ __forceinline__ void stage_rows(uint32_t taddr, float factor, unsigned char* box, int row, int chunk0) {
+__device__ __forceinline__ void stage_rows(uint32_t taddr, float factor, unsigned char* box, int row, int chunk0, unsigned char* low = nullptr) {
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
     uint32_t r[32];
@@ -237,6 +258,7 @@ __device__ __forceinline__ void stage_rows(uint32_t taddr, float factor, unsigne
       v.w = pack_bf16(__uint_as_float(r[j * 8 + 6]) * factor, __uint_as_float(r[j * 8 + 7]) * factor);
       const int chunk = chunk0 + c * 4 + j;
       *reinterpret_cast<uint4*>(box + size_t(chunk >> 3) * kBoxBytes + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)) = v;
+      if (low != nullptr) *reinterpret_cast<uint2*>(low + low_at(row, chunk)) = make_uint2(low_bytes(r + j * 8, factor), low_bytes(r + j * 8 + 4, factor));
     }
   }
 }
@@ -254,6 +276,21 @@ __device__ __forceinline__ void store_rows(const AttnTensor& t, int head, int to
     const uint4 v = *reinterpret_cast<const uint4*>(box + size_t(chunk >> 3) * kBoxBytes + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
     __nv_bfloat16* p = static_cast<__nv_bfloat16*>(t.ptr) + (long long)(token0 + r) * t.token_stride + (long long)head * t.head_stride;
     *reinterpret_cast<uint4*>(p + chunk * 8) = v;
+  }
+}
+
+// The same for the bytes of `low`, eight at a time.
+template <int CHUNKS>
+__device__ __forceinline__ void store_low(const AttnTensor& t, int head, int token0, int rows_left, int dim, const unsigned char* box,
+                                          int row0, int chunk0) {
+  const int lane = threadIdx.x & 31;
+  const int last = min(chunk0 + CHUNKS, dim / 8) - chunk0;
+#pragma unroll
+  for (int k = 0; k < CHUNKS; ++k) {
+    const int r = (k * 32 + lane) / CHUNKS, c = (k * 32 + lane) % CHUNKS;
+    if (r >= rows_left || c >= last) continue;
+    *reinterpret_cast<uint2*>(static_cast<unsigned char*>(t.ptr) + (long long)(token0 + r) * t.token_stride + (long long)head * t.head_stride + (chunk0 + c) * 8) =
+        *reinterpret_cast<const uint2*>(box + low_at(row0 + r, chunk0 + c));
   }
 }
 
@@ -285,8 +322,8 @@ struct FwdCfg {
 template <int DP>
 __global__ void __launch_bounds__(FwdCfg<DP>::kThreads, FwdCfg<DP>::kCtasPerSm)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                const __grid_constant__ CUtensorMap map_v, const Geo g, const AttnTensor out, float* __restrict__ stats,
-                const float scale_log2, unsigned int* __restrict__ status) {
+                const __grid_constant__ CUtensorMap map_v, const Geo g, const AttnTensor out, const AttnTensor low,
+                float* __restrict__ stats, const float scale_log2, unsigned int* __restrict__ status) {
   using Cfg = FwdCfg<DP>;
   constexpr int NS = Cfg::kSlots, N = Cfg::kN, H = Cfg::kHalves;
   extern __shared__ unsigned char smem_raw[];
@@ -522,10 +559,12 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     }
     if (ok && mbar_wait(bar_pv, (n - 1) & 1, failed)) {
       fence_after_sync();
-      stage_rows<DP / H / 32>(tO, 1.f / l, smem_q, row, half * (DP / H / 8));
+      // all tiles have been used: the ring has room for the low bits
+      stage_rows<DP / H / 32>(tO, 1.f / l, smem_q, row, half * (DP / H / 8), low.ptr != nullptr ? ring : nullptr);
       __syncwarp();
       const int left = t.len - row0 - (row & ~31);
       store_rows<DP / H / 8>(out, head, t.start + row0 + (row & ~31), left, g.dim, smem_q, row & ~31, half * (DP / H / 8));
+      if (low.ptr != nullptr) store_low<DP / H / 8>(low, head, t.start + row0 + (row & ~31), left, g.dim, ring, row & ~31, half * (DP / H / 8));
       if (stats != nullptr && half == 0)
         stats[((long long)head * g.tiles + t.slot) * kTile + row] = lane < left ? -fmaf(m, scale_log2, log2f(l)) : -INFINITY;
     }
@@ -540,41 +579,47 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
 }
 
 // ---------------------------------------------------------------------------------------------------------------- //
-// delta[head, row] = - sum_d dout * out, one tile and head per block; rows that belong to no token get 0.  LANES threads per row,
+// delta[head, row] = - sum_d dout * out, out with its low bits, one tile and head per block; rows that belong to no token get 0.  LANES threads per row,
 // eight values each.
 // ---------------------------------------------------------------------------------------------------------------- //
 template <int LANES>
-__global__ void __launch_bounds__(256) attn_delta_kernel(const Geo g, const AttnTensor out, const AttnTensor dout, float* __restrict__ delta) {
+__global__ void __launch_bounds__(256) attn_delta_kernel(const Geo g, const AttnTensor out, const AttnTensor low, const AttnTensor dout, float* __restrict__ delta) {
   const int order = divide(blockIdx.x, g.by_heads);
   const int head = blockIdx.x - order * g.heads;
   Tile t;
   if (!find_tile(g, order, true, t) || (g.cu != nullptr && t.batch == g.batch)) return;
-  constexpr int kRows = 256 / LANES, kSteps = kTile / kRows;
+  constexpr int kRows = 256 / LANES, kFlight = 4;      // rows of a pass, and passes whose loads are in flight together
   const int sub = threadIdx.x % LANES, r0 = threadIdx.x / LANES;
-  uint4 a[kSteps], b[kSteps];
+  auto place = [&](const AttnTensor& x, int row) { return (long long)(t.start + row) * x.token_stride + (long long)head * x.head_stride + sub * 8; };
+#pragma unroll 1
+  for (int first = 0; first < kTile; first += kFlight * kRows) {
+    uint4 a[kFlight], c[kFlight];
+    uint2 b[kFlight];
 #pragma unroll
-  for (int k = 0; k < kSteps; ++k) {
-    const int row = t.index * kTile + r0 + k * kRows;
-    a[k] = b[k] = make_uint4(0u, 0u, 0u, 0u);
-    if (row < t.len && sub * 8 < g.dim) {
-      const long long tok = t.start + row;
-      a[k] = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(out.ptr) + tok * out.token_stride + (long long)head * out.head_stride + sub * 8);
-      b[k] = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(dout.ptr) + tok * dout.token_stride + (long long)head * dout.head_stride + sub * 8);
-    }
-  }
-#pragma unroll
-  for (int k = 0; k < kSteps; ++k) {
-    const __nv_bfloat162* x = reinterpret_cast<const __nv_bfloat162*>(&a[k]);
-    const __nv_bfloat162* y = reinterpret_cast<const __nv_bfloat162*>(&b[k]);
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 u = __bfloat1622float2(x[i]), v = __bfloat1622float2(y[i]);
-      s = fmaf(u.x, v.x, fmaf(u.y, v.y, s));
+    for (int k = 0; k < kFlight; ++k) {
+      const int row = t.index * kTile + first + r0 + k * kRows;
+      a[k] = c[k] = make_uint4(0u, 0u, 0u, 0u);
+      b[k] = make_uint2(0u, 0u);
+      if (row < t.len && sub * 8 < g.dim) {
+        a[k] = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(out.ptr) + place(out, row));
+        b[k] = *reinterpret_cast<const uint2*>(static_cast<const unsigned char*>(low.ptr) + place(low, row));
+        c[k] = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(dout.ptr) + place(dout, row));
+      }
     }
 #pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (sub == 0) delta[((long long)head * g.tiles + t.slot) * kTile + r0 + k * kRows] = -s;
+    for (int k = 0; k < kFlight; ++k) {
+      const uint32_t x[4] = {a[k].x, a[k].y, a[k].z, a[k].w}, z[4] = {c[k].x, c[k].y, c[k].z, c[k].w};
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t y = i < 2 ? b[k].x : b[k].y;
+        s = fmaf(with_low(x[i] << 16, y, 2 * (i & 1)), __uint_as_float(z[i] << 16),
+                 fmaf(with_low(x[i] & 0xffff0000u, y, 2 * (i & 1) + 1), __uint_as_float(z[i] & 0xffff0000u), s));
+      }
+#pragma unroll
+      for (int o = LANES / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      if (sub == 0) delta[((long long)head * g.tiles + t.slot) * kTile + first + r0 + k * kRows] = -s;
+    }
   }
 }
 
@@ -1095,13 +1140,13 @@ cudaError_t AllowSmem(size_t bytes) {
 
 template <int DP>
 cudaError_t Forward(const AttnShape& s, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const AttnTensor& out,
-                    float* stats, unsigned int* status, cudaStream_t stream) {
+                    const AttnTensor& low, float* stats, unsigned int* status, cudaStream_t stream) {
   constexpr auto kernel = attn_fwd_kernel<DP>;
   using Cfg = FwdCfg<DP>;
   const cudaError_t e = AllowSmem<kernel>(Cfg::kSmem);
   if (e != cudaSuccess) return e;
   const Geo g = MakeGeo(s);
-  kernel<<<static_cast<unsigned>(g.tiles) * g.heads, Cfg::kThreads, Cfg::kSmem, stream>>>(mq, mk, mv, g, out, stats, s.scale * kLog2e, status);
+  kernel<<<static_cast<unsigned>(g.tiles) * g.heads, Cfg::kThreads, Cfg::kSmem, stream>>>(mq, mk, mv, g, out, low, stats, s.scale * kLog2e, status);
   CountKernelLaunch();
   return cudaGetLastError();
 }
@@ -1163,9 +1208,10 @@ bool AttnSupported(const AttnShape& s) {
 }
 
 cudaError_t LaunchAttnForward(const AttnShape& s, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v,
-                              const AttnTensor& out, float* stats, unsigned int* status, cudaStream_t stream) {
+                              const AttnTensor& out, const AttnTensor& low, float* stats, unsigned int* status, cudaStream_t stream) {
   (void)cudaGetLastError();   // the value returned below must be this launch's own, not an older error of the calling thread
-  if (!AttnSupported(s) || !Addressable(q) || !Addressable(k) || !Addressable(v) || !Addressable(out) || status == nullptr)
+  if (!AttnSupported(s) || !Addressable(q) || !Addressable(k) || !Addressable(v) || !Addressable(out) || status == nullptr ||
+      (low.ptr != nullptr && !Addressable(low)))
     return cudaErrorInvalidValue;
   const long long tokens = s.cu == nullptr ? s.batch * s.seq : s.seq;
   const int keys = s.dim <= 64 ? FwdCfg<64>::kN : FwdCfg<128>::kN;
@@ -1173,15 +1219,15 @@ cudaError_t LaunchAttnForward(const AttnShape& s, const AttnTensor& q, const Att
   if (!MakeMap(&mq, q, s.heads, s.dim, tokens, kTile) || !MakeMap(&mk, k, s.kv_heads, s.dim, tokens, keys) ||
       !MakeMap(&mv, v, s.kv_heads, s.dim, tokens, keys))
     return cudaErrorInvalidValue;
-  return s.dim <= 64 ? Forward<64>(s, mq, mk, mv, out, stats, status, stream) : Forward<128>(s, mq, mk, mv, out, stats, status, stream);
+  return s.dim <= 64 ? Forward<64>(s, mq, mk, mv, out, low, stats, status, stream) : Forward<128>(s, mq, mk, mv, out, low, stats, status, stream);
 }
 
 cudaError_t LaunchAttnBackward(const AttnShape& s, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v,
-                               const AttnTensor& out, const AttnTensor& dout, const float* stats, float* delta,
+                               const AttnTensor& out, const AttnTensor& low, const AttnTensor& dout, const float* stats, float* delta,
                                const AttnTensor& dq, const AttnTensor& dk, const AttnTensor& dv, unsigned int* status,
                                cudaStream_t stream) {
   (void)cudaGetLastError();
-  const AttnTensor* all[8] = {&q, &k, &v, &out, &dout, &dq, &dk, &dv};
+  const AttnTensor* all[9] = {&q, &k, &v, &out, &low, &dout, &dq, &dk, &dv};
   for (const AttnTensor* t : all)
     if (!Addressable(*t)) return cudaErrorInvalidValue;
   if (!AttnSupported(s) || stats == nullptr || delta == nullptr || status == nullptr) return cudaErrorInvalidValue;
@@ -1192,8 +1238,8 @@ cudaError_t LaunchAttnBackward(const AttnShape& s, const AttnTensor& q, const At
     return cudaErrorInvalidValue;
   const Geo g = MakeGeo(s);
   const unsigned blocks = static_cast<unsigned>(g.tiles) * g.heads;
-  if (s.dim <= 64) attn_delta_kernel<8><<<blocks, 256, 0, stream>>>(g, out, dout, delta);
-  else attn_delta_kernel<16><<<blocks, 256, 0, stream>>>(g, out, dout, delta);
+  if (s.dim <= 64) attn_delta_kernel<8><<<blocks, 256, 0, stream>>>(g, out, low, dout, delta);
+  else attn_delta_kernel<16><<<blocks, 256, 0, stream>>>(g, out, low, dout, delta);
   CountKernelLaunch();
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;

@@ -34,13 +34,14 @@ long long AttnTiles(const AttnShape& s);
 bool AttnSupported(const AttnShape& s);
 
 // out = softmax(scale q k^T, causal within each sequence) v.  stats (optional, heads * AttnTiles * 128 floats): minus
-// the base-2 logarithm of the row sums of exp, for the backward pass; -inf in rows that belong to no token.
+// the base-2 logarithm of the row sums of exp, for the backward pass; -inf in rows that belong to no token.  low (optional, no
+// pointer without): a byte per element of out, its next bits, for the backward pass.
 cudaError_t LaunchAttnForward(const AttnShape& s, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v,
-                              const AttnTensor& out, float* stats, unsigned int* status, cudaStream_t stream);
+                              const AttnTensor& out, const AttnTensor& low, float* stats, unsigned int* status, cudaStream_t stream);
 
 // dq, dk, dv from dout; delta: workspace of the same size as stats.
 cudaError_t LaunchAttnBackward(const AttnShape& s, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v,
-                               const AttnTensor& out, const AttnTensor& dout, const float* stats, float* delta,
+                               const AttnTensor& out, const AttnTensor& low, const AttnTensor& dout, const float* stats, float* delta,
                                const AttnTensor& dq, const AttnTensor& dk, const AttnTensor& dv, unsigned int* status,
                                cudaStream_t stream);
 

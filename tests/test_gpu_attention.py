@@ -266,3 +266,16 @@ def test_gradients_of_gradients_are_refused():
         (g,) = torch.autograd.grad(out, leaf, dout.view(out.shape), create_graph=True)
         with pytest.raises(RuntimeError, match="only once"):
             g.float().sum().backward()
+
+
+def test_gradients_where_few_keys_share_the_weight():
+    """In sequences of eight tokens delta is as large as the dP that it is subtracted from, so a delta from the rounded result
+    would show.  A rounding to bf16 is off by 2^-8 sqrt((1 - 1/4) / (2 ln 2) / 3) = 0.00166 of the value in the quadratic mean over
+    mantissas; dq and dk may have three of them (dS, P through delta, their own).  A delta from the rounded result adds two."""
+    q, k, v, dout = _inputs(8 * 64, 8, 8, 64, seed=3)
+    cu = _cu([8] * 64)
+    got = _run(q, k, v, dout, cu_seqlens=cu)
+    want, _ = _oracle(q, k, v, dout, [8] * 64, 1 / 8.0)
+    for name, a, b in zip(("dq", "dk"), got[1:3], want[1:3]):
+        off = ((a.double() - b).norm() / b.norm()).item()
+        assert off <= math.sqrt(3) * 0.00166, (name, off)
