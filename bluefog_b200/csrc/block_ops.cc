@@ -298,9 +298,10 @@ struct GatedMlpNode : public torch::autograd::Function<GatedMlpNode> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& a0, const at::Tensor& wgu0, const at::Tensor& wd0, int64_t act,
                             const c10::optional<at::Tensor>& residual) {
     const at::Tensor a = Rows2d(a0), wgu = Dense(wgu0), wd = Dense(wd0);
+    const at::Tensor res = residual.has_value() ? Rows2d(*residual) : at::Tensor();
     at::Tensor factors;
     const at::Tensor h = GatedProduct(a, wgu, act, &factors);
-    at::Tensor y = DownProduct(h, wd, residual.has_value() ? Rows2d(*residual) : at::Tensor());
+    at::Tensor y = DownProduct(h, wd, res);
     ctx->save_for_backward({a, wgu, wd, factors, h});
     ctx->saved_data["residual"] = residual.has_value();
     ctx->saved_data["sizes"] = a0.sizes().vec();
@@ -399,8 +400,9 @@ at::Tensor GatedMlp(const at::Tensor& a, const at::Tensor& w_gate_up, const at::
   if (r.defined()) TORCH_CHECK(r.sizes() == at::IntArrayRef(WithColumns(a, w_down.size(0))), "gated_mlp: residual does not match");
   const c10::cuda::CUDAGuard guard(a.get_device());
   if (NeedsGrad({a, w_gate_up, w_down, r})) return GatedMlpNode::apply(a, w_gate_up, w_down, act, residual);
-  const at::Tensor h = GatedProduct(Rows2d(a), Dense(w_gate_up), act, nullptr);
-  return DownProduct(h, Dense(w_down), r.defined() ? Rows2d(r) : r).view(WithColumns(a, w_down.size(0)));
+  // nothing is launched between the two products: the second one reads its other operands before the kernel in front of it ends
+  const at::Tensor x = Rows2d(a), wgu = Dense(w_gate_up), wd = Dense(w_down), res = r.defined() ? Rows2d(r) : r;
+  return DownProduct(GatedProduct(x, wgu, act, nullptr), wd, res).view(WithColumns(a, w_down.size(0)));
 }
 
 }  // namespace bfb

@@ -1224,18 +1224,28 @@ gemm_bf16_skinny_kernel(const __grid_constant__ CUtensorMap map_lo, const __grid
   fence_after_sync();
   const uint32_t tmem = tmem_base_s;
   bool ok = true;
+  if (GATED) let_next_kernel_start();
   if (warp == 0) {
     if (lane == 0) {
       int armed = 0;
-      for (int kb = kb0; kb < kb1; ++kb, ++armed) {
-        const int s = armed % S;
-        ok = mbar_wait(smem_u32(&bars[S + s]), ((armed / S) & 1) ^ 1, failed);
-        if (!ok) break;
+      auto weights = [&](int i) {
+        const int s = i % S, kb = kb0 + i;
         const uint32_t full = smem_u32(&bars[s]), a = smem_u32(smem + s * Cfg::kBytesA);
         mbar_expect_tx(full, Cfg::kBytesA + Cfg::kBytesB);
         tma_load_2d(a, &map_lo, full, kb * BK, n0);
         tma_load_2d(a + Cfg::kBytesA / 2, &map_hi, full, kb * BK, GATED ? n0 : n0 + 64);
-        tma_load_2d(smem_u32(stage_b + s * Cfg::kBytesB), &map_x, full, kb * BK, 0);
+      };
+      // The down projection starts beside the product before it: what it reads of the weights at first does not depend on that,
+      // everything else comes after the rows.
+      const int early = GATED ? 0 : min(S, kb1 - kb0);
+      for (int i = 0; i < early; ++i) weights(i);
+      if (!GATED) wait_for_kernel_before();
+      for (; armed < kb1 - kb0; ++armed) {
+        const int s = armed % S;
+        ok = mbar_wait(smem_u32(&bars[S + s]), ((armed / S) & 1) ^ 1, failed);
+        if (!ok) break;
+        if (armed >= early) weights(armed);
+        tma_load_2d(smem_u32(stage_b + s * Cfg::kBytesB), &map_x, smem_u32(&bars[s]), (kb0 + armed) * BK, 0);
       }
       if (!ok || *failed) {
         for (int f = armed > S ? armed - S : 0; f < armed; ++f) {
@@ -1464,13 +1474,15 @@ cudaError_t LaunchSkinny(const CUtensorMap& lo, const CUtensorMap& hi, const CUt
   cfg.blockDim = dim3(192);
   cfg.dynamicSmemBytes = Cfg::kSmem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = split;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = GATED ? 1 : 2;
   return cudaLaunchKernelEx(&cfg, kernel, lo, hi, x, out, pre, residual, M, N, num_kb, split, act, status);
 }
 

@@ -40,7 +40,8 @@ cudaError_t LaunchGemmBf16TN(const void* a, const void* b, void* out, int M, int
                              cudaStream_t stream);
 
 // The down projection of a gated feed-forward block, out[M,N] = a[M,K] * b[N,K]^T (+ addend[M,N]), on tiles chosen for its size;
-// up to kSkinnyRows rows its reduction (and that of LaunchGemmBf16Gated) is shared between clusters of CTAs.  K, N % 8 == 0.
+// up to kSkinnyRows rows its reduction (and that of LaunchGemmBf16Gated) is shared between clusters of CTAs, and it may start before the launch in
+// front of it on the stream has ended: that one may write a, nothing else that is read here.  K, N % 8 == 0.
 constexpr int kSkinnyRows = 64;
 cudaError_t LaunchGemmGatedDown(const void* a, const void* b, void* out, int M, int N, int K, unsigned int* status, cudaStream_t stream,
                                 const void* addend = nullptr);

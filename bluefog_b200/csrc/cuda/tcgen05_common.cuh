@@ -195,6 +195,12 @@ __device__ __forceinline__ void tie32(uint32_t* r) {
   asm volatile("" : "+r"(r[30]), "+r"(r[31]));
 }
 
+// Programmatic dependent launch.  The next kernel of the stream, if it was launched for it, may start when every block
+// has said so or ended; it has to wait before it touches what this one writes.
+__device__ __forceinline__ void let_next_kernel_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// Until the kernel before has ended and its results can be read; at once where this one was launched as usual.
+__device__ __forceinline__ void wait_for_kernel_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // One lane of a converged warp, the same one at every call.  The compiler knows that one lane alone runs what this guards, so the
 // descriptors of a tcgen05.mma stay in uniform registers; behind `lane == 0` every MMA first moves them there, which limits
 // the issue to one MMA in 61 cycles (measured: 128 x 64 x 16 out of shared memory 48 cycles with this, 32 with A in tensor memory).

@@ -192,3 +192,33 @@ def test_gradients_of_gradients_are_refused():
     g, h = torch.autograd.grad(gemm.gated_mlp(x, wgu, wd), [x, wd], dy, create_graph=True)
     with pytest.raises(RuntimeError, match="only once"):
         (g.float().sum() + h.float().sum()).backward()
+
+
+def test_few_rows_right_behind_the_kernels_that_write_their_inputs():
+    """The second product starts beside the first: operands written just before, copies of strided ones and captured launches."""
+    from bluefog_b200.ops import gemm
+    sets = [_inputs(8, 1024, 1376, 1024, True, seed=s) for s in range(3)]
+    want = []
+    with torch.no_grad():
+        for x, wgu, wd, _, res in sets:
+            want.append(gemm.gated_mlp(x, wgu, wd, residual=res))
+            torch.cuda.synchronize()
+        x, wgu, wd, _, res = (t.clone() for t in sets[0])
+        across = wd.t().contiguous().t()
+        big = torch.randn(4096, 4096, device="cuda")
+
+        def call():
+            return gemm.gated_mlp(x, wgu, wd, residual=res), gemm.gated_mlp(x, wgu, across, residual=res)
+
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = [call() for _ in range(4)]
+        for i in (1, 2, 0, 2, 1):
+            big = (big @ big).clamp(-1, 1)                            # the host runs ahead of the device
+            for t, s in zip((x, wgu, wd, res), (sets[i][0], sets[i][1], sets[i][2], sets[i][4])):
+                t.copy_(s)
+            across.copy_(sets[i][2])
+            eager = [call() for _ in range(4)]
+            graph.replay()
+            for a, b in zip(eager, y):
+                assert all(torch.equal(t, want[i]) for t in (*a, *b))
