@@ -388,16 +388,16 @@ at::Tensor DropoutAdd(const at::Tensor& x, const c10::optional<at::Tensor>& resi
   return DropoutLaunch(x, r, threshold, factor, key, site);
 }
 
-at::Tensor GatedMlp(const at::Tensor& a, const at::Tensor& w_gate_up, const at::Tensor& w_down, int64_t act,
-                    const c10::optional<at::Tensor>& residual) {
+c10::optional<at::Tensor> GatedMlp(const at::Tensor& a, const at::Tensor& w_gate_up, const at::Tensor& w_down, int64_t act,
+                                   const c10::optional<at::Tensor>& residual) {
   const at::Tensor r = OrUndefined(residual);
-  for (const at::Tensor& t : {a, w_gate_up, w_down, r})
-    TORCH_CHECK(!t.defined() || (t.is_cuda() && t.get_device() == a.get_device() && t.scalar_type() == at::kBFloat16),
-                "gated_mlp expects bf16 tensors on one CUDA device");
-  TORCH_CHECK(a.dim() >= 1 && w_gate_up.dim() == 2 && w_down.dim() == 2 && a.numel() > 0 && w_gate_up.numel() > 0 && w_down.numel() > 0 &&
-              w_gate_up.size(1) == a.size(-1) && w_gate_up.size(0) == 2 * w_down.size(1) && a.size(-1) % 8 == 0 && w_down.size(0) % 8 == 0 &&
-              w_down.size(1) % 8 == 0 && a.numel() / a.size(-1) < (1ll << 31) - 256, "gated_mlp: sizes do not match");
-  if (r.defined()) TORCH_CHECK(r.sizes() == at::IntArrayRef(WithColumns(a, w_down.size(0))), "gated_mlp: residual does not match");
+  auto usable = [&](const at::Tensor& t) { return t.is_cuda() && t.get_device() == a.get_device() && t.scalar_type() == at::kBFloat16; };
+  if (!usable(a) || !usable(w_gate_up) || !usable(w_down) || (r.defined() && !usable(r)) || !GemmSupported()) return c10::nullopt;
+  if (a.dim() < 1 || w_gate_up.dim() != 2 || w_down.dim() != 2 || a.numel() == 0 || w_gate_up.numel() == 0 || w_down.numel() == 0 ||
+      w_gate_up.size(1) != a.size(-1) || w_gate_up.size(0) != 2 * w_down.size(1) || a.size(-1) % 8 != 0 || w_down.size(0) % 8 != 0 ||
+      w_down.size(1) % 8 != 0 || a.numel() / a.size(-1) >= (1ll << 31) - 256)
+    return c10::nullopt;
+  if (r.defined() && r.sizes() != at::IntArrayRef(WithColumns(a, w_down.size(0)))) return c10::nullopt;
   const c10::cuda::CUDAGuard guard(a.get_device());
   if (NeedsGrad({a, w_gate_up, w_down, r})) return GatedMlpNode::apply(a, w_gate_up, w_down, act, residual);
   // nothing is launched between the two products: the second one reads its other operands before the kernel in front of it ends

@@ -18,8 +18,9 @@ at::Tensor CausalSelfAttention(const at::Tensor& qkv, int64_t heads, int64_t kv_
 at::Tensor DropoutAdd(const at::Tensor& x, const c10::optional<at::Tensor>& residual, int64_t threshold, double factor,
                       const at::Tensor& key, int64_t site);
 // (act(a Wg^T) * (a Wu^T)) Wd^T + residual, a [.., K], w_gate_up = [Wg; Wu] [2F, K], w_down [N, F], bf16; act: GemmAct.
-at::Tensor GatedMlp(const at::Tensor& a, const at::Tensor& w_gate_up, const at::Tensor& w_down, int64_t act,
-                    const c10::optional<at::Tensor>& residual);
+// Nothing where the kernels do not take the arguments, whatever the reason: the caller finds out.
+c10::optional<at::Tensor> GatedMlp(const at::Tensor& a, const at::Tensor& w_gate_up, const at::Tensor& w_down, int64_t act,
+                                   const c10::optional<at::Tensor>& residual);
 
 // A word of status bits on every device that was asked for, zero at first.
 struct StatusWords {

@@ -263,6 +263,11 @@ def gated_mlp(a: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor, ac
     with K, F and N multiples of 8 take the tcgen05 kernels, the activation and the product with the gate inside GEMM
     epilogues in both directions; other inputs take PyTorch's ops.  The kernels keep ``act(g)`` and ``u act'(g)`` for the
     backward pass in 16 bits each: what is below 2^-36 counts as zero there, and what reaches 2^27 makes gradients NaN."""
+    if a.is_cuda and act in _GATES:
+        # the arguments are looked at in C++ first: in Python that takes 6 us, as long as the device takes for few rows
+        y = _b.native.gated_mlp(a, w_gate_up, w_down, _GATES[act], residual)
+        if y is not None:
+            return y
     if act not in _GATES:
         raise ValueError("gated_mlp: act has to be one of %s, got %r" % (sorted(_GATES), act))
     if (a.dim() < 1 or w_gate_up.dim() != 2 or w_down.dim() != 2 or w_gate_up.shape[1] != a.shape[-1]
@@ -275,11 +280,7 @@ def gated_mlp(a: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor, ac
         raise ValueError("gated_mlp: residual has to be %s, got %s" % (shape, tuple(residual.shape)))
     if any(t.device != a.device or t.dtype != a.dtype for t in tensors):
         raise ValueError("gated_mlp: all tensors have to share a device and a type")
-    ok = (a.is_cuda and a.dtype == torch.bfloat16 and a.numel() > 0 and w_down.numel() > 0
-          and all(n % 8 == 0 for n in (a.shape[-1], *w_down.shape)) and _b.native.gemm_supported())
-    if not ok:
-        gate, up = torch.nn.functional.linear(a, w_gate_up).chunk(2, -1)
-        gate = torch.nn.functional.silu(gate) if act == "silu" else torch.nn.functional.gelu(gate, approximate="tanh")
-        y = torch.nn.functional.linear(gate * up, w_down)
-        return y if residual is None else y + residual
-    return _b.native.gated_mlp(a, w_gate_up, w_down, _GATES[act], residual)
+    gate, up = torch.nn.functional.linear(a, w_gate_up).chunk(2, -1)
+    gate = torch.nn.functional.silu(gate) if act == "silu" else torch.nn.functional.gelu(gate, approximate="tanh")
+    y = torch.nn.functional.linear(gate * up, w_down)
+    return y if residual is None else y + residual
