@@ -588,6 +588,7 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const Geo g, const Attn
   const int head = blockIdx.x - order * g.heads;
   Tile t;
   if (!find_tile(g, order, true, t) || (g.cu != nullptr && t.batch == g.batch)) return;
+  let_next_kernel_start();
   constexpr int kRows = 256 / LANES, kFlight = 4;      // rows of a pass, and passes whose loads are in flight together
   const int sub = threadIdx.x % LANES, r0 = threadIdx.x / LANES;
   auto place = [&](const AttnTensor& x, int row) { return (long long)(t.start + row) * x.token_stride + (long long)head * x.head_stride + sub * 8; };
@@ -689,7 +690,7 @@ __device__ __forceinline__ void add_up(const uint32_t sums, const int rank, cons
 
 template <int DP, bool KV>
 __device__ __forceinline__ void attn_bwd_body(const CUtensorMap* map_q, const CUtensorMap* map_k, const CUtensorMap* map_v, const CUtensorMap* map_do,
-                                              const Geo& g, const int block, const int split, const float* __restrict__ stats, const float* __restrict__ delta,
+                                              const Geo& g, const int block, const int split, const bool beside, const float* __restrict__ stats, const float* __restrict__ delta,
                                               const AttnTensor& d0, const AttnTensor& d1, const float scale, const float scale_log2,
                                               unsigned int* __restrict__ status) {
   using Cfg = BwdCfg<DP>;
@@ -785,6 +786,10 @@ __device__ __forceinline__ void attn_bwd_body(const CUtensorMap* map_q, const CU
         tma_load_3d(dst, m0, bar_x, b * 64, own_head, t.start + row0 + h * 64);
         tma_load_3d(dst + Cfg::kXBytes, m1, bar_x, b * 64, own_head, t.start + row0 + h * 64);
       }
+    if (KV) {
+      wait_for_kernel_before();                        // delta
+      let_next_kernel_start();
+    }
     load();
   }
   if (warp == Cfg::kWarps + 1) {
@@ -903,6 +908,7 @@ __device__ __forceinline__ void attn_bwd_body(const CUtensorMap* map_q, const CU
     const int sub_row = (warp & 3) * 32 + (lane >> 2), sub_col = half * 32 + (lane & 3) * 2;
     float2_t lse2[4], dlt2[4];                         // KV: column pairs 8 g + sub_col; otherwise rows sub_row + 8 k, twice
     if (!KV) {
+      if (!beside) wait_for_kernel_before();           // delta
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const long long at = ((long long)own_head * g.tiles + t.slot) * kTile + sub_row + 8 * k;
@@ -1073,7 +1079,9 @@ __device__ __forceinline__ void attn_bwd_body(const CUtensorMap* map_q, const CU
   if (threadIdx.x == 0 && failed_s) atomicOr(status, kAttnTimeout);
 }
 
-// The first kv_blocks blocks own key tiles (`split` of a cluster share one), the others query tiles.
+// The first kv_blocks blocks own key tiles (`split` of a cluster share one), the others query tiles.  The kernel starts while the one
+// that computes delta still runs, and waits for it where it reads that.  Query tiles alone (no kv_blocks) start beside the launch of the
+// key tiles, whose blocks let them in only after they have waited for delta.
 template <int DP>
 __global__ void __launch_bounds__(BwdCfg<DP>::kThreads, BwdCfg<DP>::kCtasPerSm)
 attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
@@ -1081,9 +1089,10 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                 const float* __restrict__ stats, const float* __restrict__ delta, const AttnTensor dq, const AttnTensor dk,
                 const AttnTensor dv, const float scale, const float scale_log2, unsigned int* __restrict__ status) {
   if (int(blockIdx.x) < kv_blocks)
-    attn_bwd_body<DP, true>(&map_q, &map_k, &map_v, &map_do, g, blockIdx.x, split, stats, delta, dv, dk, scale, scale_log2, status);
+    attn_bwd_body<DP, true>(&map_q, &map_k, &map_v, &map_do, g, blockIdx.x, split, false, stats, delta, dv, dk, scale, scale_log2, status);
   else
-    attn_bwd_body<DP, false>(&map_q, &map_k, &map_v, &map_do, g, blockIdx.x - kv_blocks, 1, stats, delta, dq, dq, scale, scale_log2, status);
+    attn_bwd_body<DP, false>(&map_q, &map_k, &map_v, &map_do, g, blockIdx.x - kv_blocks, 1, kv_blocks == 0, stats, delta, dq, dq, scale, scale_log2, status);
+  wait_for_kernel_before();                            // the end of this launch is the end of those before it
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------
@@ -1173,20 +1182,22 @@ cudaError_t Backward(const AttnShape& s, const CUtensorMap& mq, const CUtensorMa
   cfg.blockDim = dim3(Cfg::kThreads);
   cfg.dynamicSmemBytes = Cfg::kSmem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = split;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = split;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = split > 1 ? 1 : 0;
+  cfg.numAttrs = split > 1 ? 2 : 1;
   const float scale_log2 = s.scale * kLog2e;
   cudaError_t r = cudaLaunchKernelEx(&cfg, kernel, mq, mk, mv, md, g, kv_blocks, split, stats, delta, dq, dk, dv, s.scale, scale_log2, status);
   if (r != cudaSuccess) return r;
   CountKernelLaunch();
   if (split > 1) {
     cfg.gridDim = dim3(static_cast<unsigned>(q_blocks));
-    cfg.numAttrs = 0;
+    cfg.numAttrs = 1;
     r = cudaLaunchKernelEx(&cfg, kernel, mq, mk, mv, md, g, 0, 1, stats, delta, dq, dk, dv, s.scale, scale_log2, status);
     if (r != cudaSuccess) return r;
     CountKernelLaunch();

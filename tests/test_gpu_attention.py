@@ -279,3 +279,21 @@ def test_gradients_where_few_keys_share_the_weight():
     for name, a, b in zip(("dq", "dk"), got[1:3], want[1:3]):
         off = ((a.double() - b).norm() / b.norm()).item()
         assert off <= math.sqrt(3) * 0.00166, (name, off)
+
+
+def test_calls_one_right_behind_the_other():
+    """The backward launches start beside the ones in front of them: calls in a row, whose memory is used again at once."""
+    cases = [(_inputs(900, 8, 2, 64), _cu([500, 1, 300])), (_inputs(300, 4, 4, 64), None), (_inputs(513, 8, 1, 128), _cu([13, 500])),
+             (_inputs(130, 2, 1, 32), _cu([0, 130]))]
+    want = []
+    for x, cu in cases:
+        want.append(_run(*x, cu_seqlens=cu))
+        torch.cuda.synchronize()
+    got = [_run(*cases[i][0], cu_seqlens=cases[i][1]) for _ in range(10) for i in range(4)]
+    for i, g in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(g, want[i % 4])), i
+    for _ in range(5):                                                # results dropped at once
+        for x, cu in cases:
+            _run(*x, cu_seqlens=cu)
+    for i, (x, cu) in enumerate(cases):
+        assert all(torch.equal(a, b) for a, b in zip(_run(*x, cu_seqlens=cu), want[i]))
