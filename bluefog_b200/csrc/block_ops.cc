@@ -324,16 +324,16 @@ struct GatedMlpNode : public torch::autograd::Function<GatedMlpNode> {
             "gated_mlp backward");
       if (ctx->needs_input_grad(0)) {
         da = at::empty(a.sizes(), a.options());
-        list[count++] = {dpre.data_ptr(), wgu.data_ptr(), da.data_ptr(), m, k, 2 * f, false};
+        list[count++] = {dpre.data_ptr(), wgu.data_ptr(), da.data_ptr(), m, k, 2 * f, false, false};
       }
       if (ctx->needs_input_grad(1)) {
         dwgu = at::empty(wgu.sizes(), a.options());
-        list[count++] = {dpre.data_ptr(), a.data_ptr(), dwgu.data_ptr(), 2 * f, k, m, true};
+        list[count++] = {dpre.data_ptr(), a.data_ptr(), dwgu.data_ptr(), 2 * f, k, m, true, false};
       }
     }
     if (ctx->needs_input_grad(2)) {
       dwd = at::empty(wd.sizes(), a.options());
-      list[count++] = {dy.data_ptr(), h.data_ptr(), dwd.data_ptr(), n, f, m, true};
+      list[count++] = {dy.data_ptr(), h.data_ptr(), dwd.data_ptr(), n, f, m, true, dpre.defined()};             // beside the last wave of dH
     }
     if (count > 0) Check(LaunchGemmGroup(list, count, GemmStatus(a), StreamOf(a)), "gated_mlp backward");
     if (da.defined()) da = da.view(ctx->saved_data["sizes"].toIntVector());

@@ -428,6 +428,7 @@ gemm_bf16_nt_persistent_kernel(const __grid_constant__ CUtensorMap map_a, const 
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   }
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  if (EPI == kEpiGatedGrad) let_next_kernel_start();
   const uint32_t tmem_base = tmem_base_s;
 
   int armed = 0;
@@ -976,12 +977,14 @@ gemm_bf16_nt_persistent_kernel(const __grid_constant__ CUtensorMap map_a, const 
 // Up to three products in one launch of the two-SM kernel (256 x 256 tiles): the input gradient and both weight gradients of a
 // gated block do not depend on one another, and as launches of their own each ends in a wave that leaves SM pairs idle (8192 x
 // 1024 x 2752: 128, 88 and 44 tiles on 74 pairs, two, two and one wave, 68 + 91 + 50 us; together 161 us).  The tiles with the
-// longest reductions come first.  B is [reduction, N] row-major in all of them; A is [M, reduction] or, for a weight
+// longest reductions come first, but for those that need nothing of the kernel before (the down projection's weight gradient
+// does not need the gradient of the gate): they fill the SMs that its last wave leaves idle (1537 x 776 x
+// 2056, whose dH has 63 tiles: 101 -> 99 us for the block).  B is [reduction, N] row-major in all of them; A is [M, reduction] or, for a weight
 // gradient, [reduction, M].
 // ------------------------------------------------------------------------------------------ //
 constexpr int kMaxGroup = 3;
 struct GroupProblem {
-  int M, N, num_kb, tiles_m, tiles_n, first_item, a_mn;
+  int M, N, num_kb, tiles_m, tiles_n, first_item, a_mn, early;
 };
 struct GroupArgs {
   CUtensorMap a[kMaxGroup], b[kMaxGroup], c[kMaxGroup];
@@ -1037,10 +1040,14 @@ gemm_bf16_group_kernel(const __grid_constant__ GroupArgs args, unsigned int* __r
   int armed = 0;
   if (warp == 0) {
     if (lane == 0) {
-      bool ok = true;
+      bool ok = true, waited = false;
       for (int item = first; item < args.items && ok; item += step) {
         int tm, tn;
         const int i = locate(item, tm, tn);
+        if (!waited && args.p[i].early == 0) {
+          wait_for_kernel_before();
+          waited = true;
+        }
         const int m0 = tm * Cfg::kTileM + int(rank) * BM, n0 = tn * 256 + int(rank) * Cfg::kRowsB;
         const bool a_mn = args.p[i].a_mn != 0;
         const int num_kb = args.p[i].num_kb;
@@ -1062,6 +1069,7 @@ gemm_bf16_group_kernel(const __grid_constant__ GroupArgs args, unsigned int* __r
           for (int j = 0; j < Cfg::kRowsB / 64; ++j) tma_load_2d_pair(b + j * 8192, &args.b[i], full, n0 + j * 64, kb * BK);
         }
       }
+      if (!waited) wait_for_kernel_before();           // the end of this launch is the end of those before it
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -1546,15 +1554,17 @@ cudaError_t LaunchGemmGatedDown(const void* a, const void* b, void* out, int M, 
 cudaError_t LaunchGemmGroup(const GemmGroupItem* list, int count, unsigned int* status, cudaStream_t stream) {
   (void)cudaGetLastError();
   if (count < 1 || count > kMaxGroup) return cudaErrorInvalidValue;
-  // the longest reductions first
+  // what can start early, then the longest reductions
   const GemmGroupItem* by_length[kMaxGroup];
   for (int i = 0; i < count; ++i) by_length[i] = list + i;
-  std::stable_sort(by_length, by_length + count, [](const GemmGroupItem* x, const GemmGroupItem* y) { return x->K > y->K; });
+  std::stable_sort(by_length, by_length + count, [](const GemmGroupItem* x, const GemmGroupItem* y) {
+    return x->early != y->early ? x->early : x->K > y->K;
+  });
   GroupArgs args;
   args.items = 0;
   for (int i = 0; i < kMaxGroup; ++i) {
     if (i >= count) {
-      args.p[i] = {0, 0, 0, 1, 1, INT_MAX, 0};
+      args.p[i] = {0, 0, 0, 1, 1, INT_MAX, 0, 0};
       continue;
     }
     const GemmGroupItem& g = *by_length[i];
@@ -1563,7 +1573,7 @@ cudaError_t LaunchGemmGroup(const GemmGroupItem* list, int count, unsigned int* 
     if (!(g.a_transposed ? MakeMap(&args.a[i], g.a, g.K, g.M, 64) : MakeMap(&args.a[i], g.a, g.M, g.K, BM)) ||
         !MakeMap(&args.b[i], g.b, g.K, g.N, 64) || !MakeMap(&args.c[i], g.out, g.M, g.N, 32))
       return cudaErrorInvalidValue;
-    args.p[i] = {g.M, g.N, (g.K + BK - 1) / BK, (g.M + 255) / 256, (g.N + 255) / 256, args.items, g.a_transposed ? 1 : 0};
+    args.p[i] = {g.M, g.N, (g.K + BK - 1) / BK, (g.M + 255) / 256, (g.N + 255) / 256, args.items, g.a_transposed ? 1 : 0, g.early ? 1 : 0};
     args.items += args.p[i].tiles_m * args.p[i].tiles_n;
   }
   for (int i = count; i < kMaxGroup; ++i) args.a[i] = args.b[i] = args.c[i] = args.a[0];
@@ -1584,13 +1594,15 @@ cudaError_t LaunchGemmGroup(const GemmGroupItem* list, int count, unsigned int* 
   cfg.blockDim = dim3(Cfg::kThreadsP);
   cfg.dynamicSmemBytes = Cfg::kSmem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = by_length[0]->early ? 2 : 1;
   e = cudaLaunchKernelEx(&cfg, gemm_bf16_group_kernel, args, status);
   if (e != cudaSuccess) return e;
   CountKernelLaunch();

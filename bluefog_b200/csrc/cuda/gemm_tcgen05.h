@@ -54,6 +54,7 @@ struct GemmGroupItem {
   void* out;
   int M, N, K;
   bool a_transposed;
+  bool early;            // neither operand comes from the launch in front of this one on the stream, nor anything that it reads goes to out
 };
 cudaError_t LaunchGemmGroup(const GemmGroupItem* list, int count, unsigned int* status, cudaStream_t stream);
 
