@@ -13,7 +13,7 @@
 // value, as the rounding of the result itself is).  So that delta does not suffer from the rounding of out - it is small against
 // the dP that it is subtracted from only where many keys share the weight -, a forward pass with a backward pass to come
 // also keeps the next eight bits of out (see low_bytes): without them dq and dk of 136 tokens are 1.6 times as far off as their
-// own rounding alone, of 8 tokens 2.2 times, with them 1.45 and 1.5, for 4 of the 154 us of a GPT-2 medium layer.  A row's sum
+// own rounding alone, of 8 tokens 2.2 times, with them 1.45 and 1.5, for 4 of the 152 us of a GPT-2 medium layer.  A row's sum
 // is taken over the unrounded values.
 //
 // Sequences: a tile never crosses a sequence boundary.  Tile slot cu[b] / 128 + b + i belongs to rows [128 i, 128 i + 128)

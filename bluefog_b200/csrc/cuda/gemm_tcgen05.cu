@@ -978,9 +978,9 @@ gemm_bf16_nt_persistent_kernel(const __grid_constant__ CUtensorMap map_a, const 
 // gated block do not depend on one another, and as launches of their own each ends in a wave that leaves SM pairs idle (8192 x
 // 1024 x 2752: 128, 88 and 44 tiles on 74 pairs, two, two and one wave, 68 + 91 + 50 us; together 161 us).  The tiles with the
 // longest reductions come first, but for those that need nothing of the kernel before (the down projection's weight gradient
-// does not need the gradient of the gate): they fill the SMs that its last wave leaves idle (1537 x 776 x
-// 2056, whose dH has 63 tiles: 101 -> 99 us for the block).  B is [reduction, N] row-major in all of them; A is [M, reduction] or, for a weight
-// gradient, [reduction, M].
+// does not need the gradient of the gate): they fill the SMs that its last wave leaves idle (1537 x 776 x 2056,
+// whose dH has 63 tiles: 101 -> 99 us for the block).  B is [reduction, N] row-major in all of them; A is [M, reduction] or, for a
+// weight gradient, [reduction, M].
 // ------------------------------------------------------------------------------------------ //
 constexpr int kMaxGroup = 3;
 struct GroupProblem {
