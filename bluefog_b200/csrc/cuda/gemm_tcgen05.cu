@@ -334,7 +334,12 @@ struct PersistentCfg {
   // that on the GELU epilogues.  Their staging boxes cost one of the six ring stages.
   static constexpr int kEpiWarps = PAIR ? 8 : 4;
   static constexpr int kThreadsP = 64 + 32 * kEpiWarps;
-  static constexpr int kStagesP = (PAIR ? 5 : ((BN_ == 256) ? 4 : 6)) - (EPI == kEpiColumnStats ? 1 : 0);
+  // the gate's gradient gives one up for a third pair of boxes per epilogue warp, so that two chunks of kept factors are on their
+  // way (dH of 8192 x 1024 x 2752 61 -> 55 us; with a reduction of 2048, which would rather have the stage, 16384 rows and 5504
+  // columns 308 -> 317 us); tiles of 128 columns on pairs have room for both
+  static constexpr int kStagesP =
+      (PAIR ? 5 : ((BN_ == 256) ? 4 : 6)) - (EPI == kEpiColumnStats || (EPI == kEpiGatedGrad && !(PAIR && BN_ == 128)) ? 1 : 0);
+  static constexpr int kPre = EPI == kEpiGatedGrad ? 3 : 2;    // pairs of boxes
   // per epilogue warp: BN_ column sums and BN_ sums of squares
   static constexpr uint32_t kStatBytes = EPI == kEpiColumnStats ? kEpiWarps * 2 * BN_ * 4 : 0;
   static constexpr int kRowsB = PAIR ? BN_ / 2 : BN_;          // rows (output columns) of B one CTA loads
@@ -348,8 +353,10 @@ struct PersistentCfg {
   static constexpr uint32_t kCols = 2 * BN_;
   // output staging: per epilogue warp two [32 rows x 64 columns] bf16 boxes (4 KiB each, 1024-byte aligned)
   static constexpr uint32_t kBytesOutBox = 32 * 64 * 2;
-  static constexpr uint32_t kBytesOut = kEpiWarps * 2 * kBytesOutBox;
-  static constexpr size_t kSmem = 1024 + size_t(kStagesP) * kBytesStage + kBytesOut + 256 + kStatBytes;
+  static constexpr uint32_t kBytesOutWarp = kPre * kBytesOutBox;
+  static constexpr uint32_t kBytesOut = kEpiWarps * kBytesOutWarp;
+  static constexpr uint32_t kBytesBars = EPI == kEpiGatedGrad ? 512 : 256;
+  static constexpr size_t kSmem = 1024 + size_t(kStagesP) * kBytesStage + kBytesOut + kBytesBars + kStatBytes;
   static constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(BN_ >> 3) << 17) | (uint32_t(kTileM >> 4) << 24);
 };
 
@@ -407,7 +414,7 @@ gemm_bf16_nt_persistent_kernel(const __grid_constant__ CUtensorMap map_a, const 
       mbar_init(smem_u32(&bars[2 * S + 2 + a]), (PAIR ? 2 : 1) * Cfg::kEpiWarps);    // one arrive per epilogue warp (of both CTAs)
     }
     if (EPI == kEpiGatedGrad)
-      for (int a = 0; a < 2 * Cfg::kEpiWarps; ++a) mbar_init(smem_u32(&bars[2 * S + 4 + a]), 1);
+      for (int a = 0; a < Cfg::kPre * Cfg::kEpiWarps; ++a) mbar_init(smem_u32(&bars[2 * S + 4 + a]), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -544,14 +551,14 @@ gemm_bf16_nt_persistent_kernel(const __grid_constant__ CUtensorMap map_a, const 
     constexpr int kChunksW = Cfg::kEpiWarps == 8 ? kChunks / 2 : kChunks;
     const int c_first = Cfg::kEpiWarps == 8 ? (ew >> 2) * kChunksW : 0;
     const bool vec_ok = (N % 8) == 0;
-    unsigned char* my_out = stage_out + size_t(ew) * 2 * Cfg::kBytesOutBox;
+    unsigned char* my_out = stage_out + size_t(ew) * Cfg::kBytesOutWarp;
     int local = 0;
     int boxes = 0;                       // TMA stores issued by this warp
     // kEpiColumnStats: this warp's partial column sums [BN_] and sums of squares [BN_] of the current column
     // block live in shared memory (lanes 0-7 each own eight columns of every 64-column chunk, so no atomics)
     // and go to col_stats with vector reductions when the column block changes and at the end: adding every
     // box to global memory directly serialises thousands of reductions per address.
-    float* wstat = reinterpret_cast<float*>(stage_out + Cfg::kBytesOut + 256) + (EPI == kEpiColumnStats ? ew * 2 * BN_ : 0);
+    float* wstat = reinterpret_cast<float*>(stage_out + Cfg::kBytesOut + Cfg::kBytesBars) + (EPI == kEpiColumnStats ? ew * 2 * BN_ : 0);
     int stat_n0 = -1;
     auto flush_stats = [&]() {
       if (stat_n0 >= 0 && lane < 8) {
@@ -575,13 +582,13 @@ gemm_bf16_nt_persistent_kernel(const __grid_constant__ CUtensorMap map_a, const 
       for (int i = lane; i < 2 * BN_; i += 32) wstat[i] = 0.f;
       __syncwarp();
     }
-    // kEpiGatedGrad: the kept factors come through TMA boxes of 32 rows x 32 columns, one chunk ahead, into two sets of a box for
+    // kEpiGatedGrad: the kept factors come through TMA boxes of 32 rows x 32 columns, two chunks ahead, into three sets of a box for
     // each per warp; dU and dG replace them there and leave from there.  (Read by the threads row by row, 32 sectors per load,
     // the epilogue took four times as long as the main loop of a reduction of 1024.)
     constexpr int kParts = Cfg::kTileN / 32 / (Cfg::kEpiWarps == 8 ? 2 : 1);
     const int part_first = Cfg::kEpiWarps == 8 ? (ew >> 2) * kParts : 0;
     int pre_tile = first_tile, pre_part = part_first, loaded = 0, used = 0;
-    auto pre_bar = [&](int set) { return smem_u32(&bars[2 * S + 4 + ew * 2 + set]); };
+    auto pre_bar = [&](int set) { return smem_u32(&bars[2 * S + 4 + ew * Cfg::kPre + set]); };
     auto prefetch = [&]() {
       for (; pre_tile < num_tiles; pre_tile += tile_step, pre_part = part_first) {
         int tm, tn;
@@ -589,7 +596,7 @@ gemm_bf16_nt_persistent_kernel(const __grid_constant__ CUtensorMap map_a, const 
         const int row = tm * Cfg::kTileM + int(rank) * BM + q * 32, col = tn * Cfg::kTileN + pre_part * 32;
         if (pre_part == part_first + kParts || row >= M || col >= N) continue;
         if (lane == 0) {
-          const uint32_t bar = pre_bar(loaded & 1), dst = smem_u32(my_out) + (loaded & 1) * 4096u;
+          const uint32_t bar = pre_bar(loaded % Cfg::kPre), dst = smem_u32(my_out) + (loaded % Cfg::kPre) * 4096u;
           mbar_expect_tx(bar, 4096);
           tma_load_2d(dst, &map_b2, bar, col, row);
           tma_load_2d(dst + 2048, &map_aux2, bar, col, row);
@@ -599,7 +606,10 @@ gemm_bf16_nt_persistent_kernel(const __grid_constant__ CUtensorMap map_a, const 
         return;
       }
     };
-    if constexpr (EPI == kEpiGatedGrad) prefetch();
+    if constexpr (EPI == kEpiGatedGrad) {
+#pragma unroll 1
+      for (int i = 1; i < Cfg::kPre; ++i) prefetch();
+    }
     for (int tile = first_tile; tile < num_tiles; tile += tile_step, ++local) {
       const int acc = local & 1;
       int tm, tn;
@@ -676,8 +686,8 @@ gemm_bf16_nt_persistent_kernel(const __grid_constant__ CUtensorMap map_a, const 
           if (nbase >= N || m0 + q * 32 >= M) break;           // warp-uniform; prefetch() walks the same chunks
           uint32_t r[32];
           tmem_ld32(tmem_base + (uint32_t(q * 32) << 16) + uint32_t(acc * BN_ + c * 32), r);
-          unsigned char* box = my_out + (used & 1) * 4096;
-          if (!mbar_wait(pre_bar(used & 1), (used >> 1) & 1, failed)) {
+          unsigned char* box = my_out + (used % Cfg::kPre) * 4096;
+          if (!mbar_wait(pre_bar(used % Cfg::kPre), (used / Cfg::kPre) & 1, failed)) {
             tmem_wait_ld();
             break;
           }
@@ -947,7 +957,7 @@ gemm_bf16_nt_persistent_kernel(const __grid_constant__ CUtensorMap map_a, const 
     if constexpr (EPI == kEpiGatedGrad) {
       for (; used < loaded; ++used) {
         const unsigned long long t0 = now_ns();
-        while (!mbar_try(pre_bar(used & 1), (used >> 1) & 1) && now_ns() - t0 < kWaitLimitNs) {}
+        while (!mbar_try(pre_bar(used % Cfg::kPre), (used / Cfg::kPre) & 1) && now_ns() - t0 < kWaitLimitNs) {}
       }
     }
   }
