@@ -1085,6 +1085,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   // ---- transformer-block operators with their backward passes (block_ops.cc) --------------------
   m.def("causal_attention", &CausalAttention);
   m.def("causal_self_attention", &CausalSelfAttention);
+  m.def("attention_spacing", &AttentionSpacing, py::arg("t"), py::arg("side_by_side") = false);
   m.def("dropout_add", &DropoutAdd);
   m.def("gated_mlp", &GatedMlp);
   // reads and clears the status word of the attention kernels (synchronises with the device)

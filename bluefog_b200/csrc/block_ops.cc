@@ -51,18 +51,18 @@ variable_list Once(const char* what, variable_list grads) {
 
 // ---- attention -----------------------------------------------------------------------------------------------------
 
-// Spacing of the rows of t [.., tokens, columns...] (`inner` trailing dimensions belong to a row); 0 when they are not evenly spaced.
-// Extents of one have no spacing of their own.
+// Spacing of the rows of t [.., tokens, columns...] (`inner` trailing dimensions belong to a row); 0 when they are not evenly spaced,
+// as the rows of a broadcast dimension are not: they all lie in one place (the gradient of a sum over the tokens).  Extents of
+// one have no spacing of their own.
 int64_t RowStride(const at::Tensor& t, int64_t inner, int64_t row_size) {
-  const int64_t n = t.dim() - inner;
-  int64_t stride = 0, span = 0;
-  for (int64_t i = n - 1; i >= 0; --i) {
+  int64_t stride = -1, span = 0;                       // none met so far
+  for (int64_t i = t.dim() - inner - 1; i >= 0; --i) {
     if (t.size(i) == 1) continue;
-    if (stride == 0) stride = t.stride(i);
-    else if (t.stride(i) != span) return 0;
+    if (t.stride(i) <= 0 || (stride >= 0 && t.stride(i) != span)) return 0;
+    if (stride < 0) stride = t.stride(i);
     span = t.stride(i) * t.size(i);
   }
-  return stride == 0 ? (row_size + 7) / 8 * 8 : stride;
+  return stride < 0 ? (row_size + 7) / 8 * 8 : stride;
 }
 
 // A [.., tokens, heads, D] operand, or false where the kernels cannot address it.
@@ -83,11 +83,12 @@ AttnTensor Described(const at::Tensor& t) {
   TORCH_CHECK(Describe(t, &a), "attention: rows have to be contiguous, 16-byte aligned and evenly spaced");
   return a;
 }
-// qkv with rows that the kernels can address
-at::Tensor QkvRows(const at::Tensor& t) {
+bool QkvAddressable(const at::Tensor& t) {
   const int64_t cols = t.size(-1), stride = RowStride(t, 1, cols);
-  return t.stride(-1) == 1 && Aligned(t) && stride % 8 == 0 && stride >= cols ? t : t.clone(at::MemoryFormat::Contiguous);
+  return t.stride(-1) == 1 && Aligned(t) && stride % 8 == 0 && stride >= cols;
 }
+// qkv with rows that the kernels can address
+at::Tensor QkvRows(const at::Tensor& t) { return QkvAddressable(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
 // the columns of `heads` heads of width d that start with head `first`
 AttnTensor QkvPart(const at::Tensor& t, int64_t first, int64_t d) {
   AttnTensor a;
@@ -343,6 +344,12 @@ struct GatedMlpNode : public torch::autograd::Function<GatedMlpNode> {
 };
 
 }  // namespace
+
+c10::optional<std::vector<int64_t>> AttentionSpacing(const at::Tensor& t, bool side_by_side) {
+  if (side_by_side) return QkvAddressable(t) ? c10::make_optional(std::vector<int64_t>{RowStride(t, 1, t.size(-1))}) : c10::nullopt;
+  AttnTensor a;
+  return Describe(t, &a) ? c10::make_optional(std::vector<int64_t>{a.token_stride, a.head_stride}) : c10::nullopt;
+}
 
 at::Tensor& StatusTensor(StatusWords& words, int device) {
   std::lock_guard<std::mutex> lock(words.mu);

@@ -4,6 +4,7 @@
 
 #include <map>
 #include <mutex>
+#include <vector>
 
 namespace bfb {
 
@@ -14,6 +15,9 @@ namespace bfb {
 at::Tensor CausalAttention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const c10::optional<at::Tensor>& cu, double scale);
 // The three side by side in the columns of qkv [.., T, (heads + 2 kv_heads) D].
 at::Tensor CausalSelfAttention(const at::Tensor& qkv, int64_t heads, int64_t kv_heads, const c10::optional<at::Tensor>& cu, double scale);
+// How the attention kernels walk over the memory of t [.., T, heads, D], {elements from token to token, from head to head}, or of t
+// [.., T, columns] when side_by_side, {elements from token to token}; nothing where they work on a copy.  On any device.
+c10::optional<std::vector<int64_t>> AttentionSpacing(const at::Tensor& t, bool side_by_side);
 // residual + keep * factor * x; threshold of 65536 is the dropped share, key int64 [seed, step].
 at::Tensor DropoutAdd(const at::Tensor& x, const c10::optional<at::Tensor>& residual, int64_t threshold, double factor,
                       const at::Tensor& key, int64_t site);
