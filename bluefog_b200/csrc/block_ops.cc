@@ -135,6 +135,7 @@ AttnShape QkvShape(const at::Tensor& qkv, int64_t heads, int64_t kv_heads, const
 at::Tensor StatsFor(const AttnShape& s, const at::Tensor& like) {
   return at::empty({s.heads, AttnTiles(s), 128}, like.options().dtype(at::kFloat));
 }
+at::Tensor DeltaFor(const at::Tensor& stats) { return at::empty({stats.numel() + kAttnDeltaExtra}, stats.options()); }
 // What the forward pass leaves for the backward pass besides the result.
 struct Kept {
   at::Tensor stats, low;
@@ -174,7 +175,7 @@ struct AttentionNode : public torch::autograd::Function<AttentionNode> {
     const AttnShape s = ShapeOf(q, k, saved[3], ctx->saved_data["scale"].toDouble());
     const at::Tensor dout = Rows(grads[0]);
     at::Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()), dv = at::empty(v.sizes(), v.options());
-    at::Tensor delta = at::empty_like(stats);
+    at::Tensor delta = DeltaFor(stats);
     Check(LaunchAttnBackward(s, Described(q), Described(k), Described(v), Described(out), Described(saved[6]), Described(dout), StatsPtr(stats), StatsPtr(delta),
                              Described(dq), Described(dk), Described(dv), AttnStatusWord(q.get_device()), StreamOf(q)), "attention backward");
     variable_list g = Once("attention", {dq, dk, dv});
@@ -215,7 +216,7 @@ struct SelfAttentionNode : public torch::autograd::Function<SelfAttentionNode> {
     const int64_t h = ctx->saved_data["h"].toInt(), hkv = ctx->saved_data["hkv"].toInt();
     const AttnShape s = QkvShape(qkv, h, hkv, saved[1], ctx->saved_data["scale"].toDouble());
     const at::Tensor dout = Rows(grads[0]);
-    at::Tensor dqkv = at::empty(qkv.sizes(), qkv.options()), delta = at::empty_like(stats);
+    at::Tensor dqkv = at::empty(qkv.sizes(), qkv.options()), delta = DeltaFor(stats);
     Check(LaunchAttnBackward(s, QkvPart(qkv, 0, s.dim), QkvPart(qkv, h, s.dim), QkvPart(qkv, h + hkv, s.dim), Described(out), Described(saved[4]), Described(dout),
                              StatsPtr(stats), StatsPtr(delta), QkvPart(dqkv, 0, s.dim), QkvPart(dqkv, h, s.dim), QkvPart(dqkv, h + hkv, s.dim),
                              AttnStatusWord(qkv.get_device()), StreamOf(qkv)), "attention backward");

@@ -109,6 +109,21 @@ __device__ __forceinline__ bool find_tile(const Geo& g, int order, bool late_fir
   return t.index >= 0 && t.index * kTile < t.len;
 }
 
+// Values that the kernel before may still be writing when this one starts (programmatic launch): an access in its place of the
+// program, behind the wait, and past the L1 cache.  A const __restrict__ pointer would promise the compiler that they never change.
+__device__ __forceinline__ float load_late(const float* p) {
+  float v;
+  asm volatile("ld.global.cg.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory");
+  return v;
+}
+// Hand-over of what a thread has seen, in whichever kernel it was written, to a kernel that runs beside this one.
+__device__ __forceinline__ void hand_over(unsigned int* word) { asm volatile("st.release.gpu.global.u32 [%0], 1;" ::"l"(word) : "memory"); }
+__device__ __forceinline__ bool handed_over(const unsigned int* word) {
+  unsigned int v;
+  asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(word) : "memory");
+  return v != 0u;
+}
+
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -580,10 +595,12 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
 
 // ---------------------------------------------------------------------------------------------------------------- //
 // delta[head, row] = - sum_d dout * out, out with its low bits, one tile and head per block; rows that belong to no token get 0.  LANES threads per row,
-// eight values each.
+// eight values each.  Clears the word by which the key tiles tell the query tiles that all this has ended.
 // ---------------------------------------------------------------------------------------------------------------- //
 template <int LANES>
-__global__ void __launch_bounds__(256) attn_delta_kernel(const Geo g, const AttnTensor out, const AttnTensor low, const AttnTensor dout, float* __restrict__ delta) {
+__global__ void __launch_bounds__(256) attn_delta_kernel(const Geo g, const AttnTensor out, const AttnTensor low, const AttnTensor dout, float* __restrict__ delta,
+                                                         unsigned int* __restrict__ delta_ready) {
+  if (blockIdx.x == 0 && threadIdx.x == 0) *delta_ready = 0u;
   const int order = divide(blockIdx.x, g.by_heads);
   const int head = blockIdx.x - order * g.heads;
   Tile t;
@@ -690,7 +707,7 @@ __device__ __forceinline__ void add_up(const uint32_t sums, const int rank, cons
 
 template <int DP, bool KV>
 __device__ __forceinline__ void attn_bwd_body(const CUtensorMap* map_q, const CUtensorMap* map_k, const CUtensorMap* map_v, const CUtensorMap* map_do,
-                                              const Geo& g, const int block, const int split, const bool beside, const float* __restrict__ stats, const float* __restrict__ delta,
+                                              const Geo& g, const int block, const int split, unsigned int* const delta_ready, const float* stats, const float* delta,
                                               const AttnTensor& d0, const AttnTensor& d1, const float scale, const float scale_log2,
                                               unsigned int* __restrict__ status) {
   using Cfg = BwdCfg<DP>;
@@ -788,6 +805,7 @@ __device__ __forceinline__ void attn_bwd_body(const CUtensorMap* map_q, const CU
       }
     if (KV) {
       wait_for_kernel_before();                        // delta
+      if (split > 1) hand_over(delta_ready);           // the query tiles are a launch of their own
       let_next_kernel_start();
     }
     load();
@@ -908,12 +926,15 @@ __device__ __forceinline__ void attn_bwd_body(const CUtensorMap* map_q, const CU
     const int sub_row = (warp & 3) * 32 + (lane >> 2), sub_col = half * 32 + (lane & 3) * 2;
     float2_t lse2[4], dlt2[4];                         // KV: column pairs 8 g + sub_col; otherwise rows sub_row + 8 k, twice
     if (!KV) {
-      if (!beside) wait_for_kernel_before();           // delta
+      // delta.  As a launch of their own the query tiles run beside the key tiles, all of which have waited for it and said so before
+      // these blocks can start; to wait for the launch of the key tiles itself is right as well, but lets nothing run beside it.
+      if (delta_ready == nullptr || !handed_over(delta_ready)) wait_for_kernel_before();
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const long long at = ((long long)own_head * g.tiles + t.slot) * kTile + sub_row + 8 * k;
-        lse2[k] = pair(stats[at], stats[at]);
-        dlt2[k] = pair(delta[at], delta[at]);
+        const float lse = load_late(stats + at), dlt = load_late(delta + at);
+        lse2[k] = pair(lse, lse);
+        dlt2[k] = pair(dlt, dlt);
       }
       if (set == 0) {
         // q (first half of the warps) or dout (second) from shared to tensor memory, a row per thread
@@ -1081,17 +1102,19 @@ __device__ __forceinline__ void attn_bwd_body(const CUtensorMap* map_q, const CU
 
 // The first kv_blocks blocks own key tiles (`split` of a cluster share one), the others query tiles.  The kernel starts while the one
 // that computes delta still runs, and waits for it where it reads that.  Query tiles alone (no kv_blocks) start beside the launch of the
-// key tiles, whose blocks let them in only after they have waited for delta.
+// key tiles, whose blocks let them in only after they have waited for delta.  That alone orders no memory accesses, so they also
+// hand over what they have seen (delta_ready).
 template <int DP>
 __global__ void __launch_bounds__(BwdCfg<DP>::kThreads, BwdCfg<DP>::kCtasPerSm)
 attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                 const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do, const Geo g, const int kv_blocks, const int split,
-                const float* __restrict__ stats, const float* __restrict__ delta, const AttnTensor dq, const AttnTensor dk,
+                const float* stats, const float* delta, unsigned int* const delta_ready, const AttnTensor dq, const AttnTensor dk,
                 const AttnTensor dv, const float scale, const float scale_log2, unsigned int* __restrict__ status) {
   if (int(blockIdx.x) < kv_blocks)
-    attn_bwd_body<DP, true>(&map_q, &map_k, &map_v, &map_do, g, blockIdx.x, split, false, stats, delta, dv, dk, scale, scale_log2, status);
+    attn_bwd_body<DP, true>(&map_q, &map_k, &map_v, &map_do, g, blockIdx.x, split, delta_ready, stats, delta, dv, dk, scale, scale_log2, status);
   else
-    attn_bwd_body<DP, false>(&map_q, &map_k, &map_v, &map_do, g, blockIdx.x - kv_blocks, 1, kv_blocks == 0, stats, delta, dq, dq, scale, scale_log2, status);
+    attn_bwd_body<DP, false>(&map_q, &map_k, &map_v, &map_do, g, blockIdx.x - kv_blocks, 1, kv_blocks == 0 ? delta_ready : nullptr, stats, delta, dq, dq, scale,
+                             scale_log2, status);
   wait_for_kernel_before();                            // the end of this launch is the end of those before it
 }
 
@@ -1162,7 +1185,7 @@ cudaError_t Forward(const AttnShape& s, const CUtensorMap& mq, const CUtensorMap
 
 template <int DP>
 cudaError_t Backward(const AttnShape& s, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& md,
-                     const float* stats, const float* delta, const AttnTensor& dq, const AttnTensor& dk, const AttnTensor& dv,
+                     const float* stats, const float* delta, unsigned int* delta_ready, const AttnTensor& dq, const AttnTensor& dk, const AttnTensor& dv,
                      unsigned int* status, cudaStream_t stream) {
   constexpr auto kernel = attn_bwd_kernel<DP>;
   using Cfg = BwdCfg<DP>;
@@ -1192,13 +1215,13 @@ cudaError_t Backward(const AttnShape& s, const CUtensorMap& mq, const CUtensorMa
   cfg.attrs = attr;
   cfg.numAttrs = split > 1 ? 2 : 1;
   const float scale_log2 = s.scale * kLog2e;
-  cudaError_t r = cudaLaunchKernelEx(&cfg, kernel, mq, mk, mv, md, g, kv_blocks, split, stats, delta, dq, dk, dv, s.scale, scale_log2, status);
+  cudaError_t r = cudaLaunchKernelEx(&cfg, kernel, mq, mk, mv, md, g, kv_blocks, split, stats, delta, delta_ready, dq, dk, dv, s.scale, scale_log2, status);
   if (r != cudaSuccess) return r;
   CountKernelLaunch();
   if (split > 1) {
     cfg.gridDim = dim3(static_cast<unsigned>(q_blocks));
     cfg.numAttrs = 1;
-    r = cudaLaunchKernelEx(&cfg, kernel, mq, mk, mv, md, g, 0, 1, stats, delta, dq, dk, dv, s.scale, scale_log2, status);
+    r = cudaLaunchKernelEx(&cfg, kernel, mq, mk, mv, md, g, 0, 1, stats, delta, delta_ready, dq, dk, dv, s.scale, scale_log2, status);
     if (r != cudaSuccess) return r;
     CountKernelLaunch();
   }
@@ -1249,13 +1272,14 @@ cudaError_t LaunchAttnBackward(const AttnShape& s, const AttnTensor& q, const At
     return cudaErrorInvalidValue;
   const Geo g = MakeGeo(s);
   const unsigned blocks = static_cast<unsigned>(g.tiles) * g.heads;
-  if (s.dim <= 64) attn_delta_kernel<8><<<blocks, 256, 0, stream>>>(g, out, low, dout, delta);
-  else attn_delta_kernel<16><<<blocks, 256, 0, stream>>>(g, out, low, dout, delta);
+  unsigned int* ready = reinterpret_cast<unsigned int*>(delta + (long long)g.heads * g.tiles * kTile);
+  if (s.dim <= 64) attn_delta_kernel<8><<<blocks, 256, 0, stream>>>(g, out, low, dout, delta, ready);
+  else attn_delta_kernel<16><<<blocks, 256, 0, stream>>>(g, out, low, dout, delta, ready);
   CountKernelLaunch();
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  return s.dim <= 64 ? Backward<64>(s, mq, mk, mv, md, stats, delta, dq, dk, dv, status, stream)
-                     : Backward<128>(s, mq, mk, mv, md, stats, delta, dq, dk, dv, status, stream);
+  return s.dim <= 64 ? Backward<64>(s, mq, mk, mv, md, stats, delta, ready, dq, dk, dv, status, stream)
+                     : Backward<128>(s, mq, mk, mv, md, stats, delta, ready, dq, dk, dv, status, stream);
 }
 
 }  // namespace bfb

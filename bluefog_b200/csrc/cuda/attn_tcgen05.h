@@ -39,7 +39,8 @@ bool AttnSupported(const AttnShape& s);
 cudaError_t LaunchAttnForward(const AttnShape& s, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v,
                               const AttnTensor& out, const AttnTensor& low, float* stats, unsigned int* status, cudaStream_t stream);
 
-// dq, dk, dv from dout; delta: workspace of the same size as stats.
+// dq, dk, dv from dout; delta: workspace of the same size as stats and kAttnDeltaExtra floats more.
+constexpr int kAttnDeltaExtra = 4;
 cudaError_t LaunchAttnBackward(const AttnShape& s, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v,
                                const AttnTensor& out, const AttnTensor& low, const AttnTensor& dout, const float* stats, float* delta,
                                const AttnTensor& dq, const AttnTensor& dk, const AttnTensor& dv, unsigned int* status,
