@@ -1088,18 +1088,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("attention_spacing", &AttentionSpacing, py::arg("t"), py::arg("side_by_side") = false);
   m.def("dropout_add", &DropoutAdd);
   m.def("gated_mlp", &GatedMlp);
-  // reads and clears the status word of the attention kernels (synchronises with the device)
-  m.def("attn_status", [](int device) {
-    c10::cuda::CUDAGuard g(device);
-    cudaStream_t stream = CurrentStream(device);
-    unsigned int* word = AttnStatusWord(device);
-    unsigned int value = 0;
-    cudaError_t e = cudaMemcpyAsync(&value, word, sizeof(value), cudaMemcpyDeviceToHost, stream);
-    if (e == cudaSuccess) e = cudaMemsetAsync(word, 0, sizeof(value), stream);
-    if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
-    TORCH_CHECK(e == cudaSuccess, "attn_status failed: ", cudaGetErrorString(e));
-    return value;
-  });
+  // reads and clears the status word of the attention kernels (waits for the device)
+  m.def("attn_status", &TakeAttnStatus);
 
   m.def("gemm_status", [] {
     at::Tensor probe = at::empty({0}, at::TensorOptions().device(at::kCUDA));

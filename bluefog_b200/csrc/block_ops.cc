@@ -21,7 +21,7 @@ using torch::autograd::variable_list;
 
 cudaStream_t StreamOf(const at::Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
 
-void Check(cudaError_t e, const char* what) { TORCH_CHECK(e == cudaSuccess, what, " launch failed: ", cudaGetErrorString(e)); }
+void Check(cudaError_t e, const char* what) { TORCH_CHECK(e == cudaSuccess, what, " failed: ", cudaGetErrorString(e)); }
 
 bool Aligned(const at::Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0; }
 
@@ -153,7 +153,7 @@ at::Tensor SeparateForward(const at::Tensor& q, const at::Tensor& k, const at::T
   at::Tensor out = at::empty(q.sizes(), q.options());
   if (kept != nullptr) kept->Make(s, out);
   Check(LaunchAttnForward(s, Described(q), Described(k), Described(v), Described(out), kept != nullptr ? Described(kept->low) : AttnTensor(),
-                          kept != nullptr ? StatsPtr(kept->stats) : nullptr, AttnStatusWord(q.get_device()), StreamOf(q)), "attention forward");
+                          kept != nullptr ? StatsPtr(kept->stats) : nullptr, AttnStatusWord(q.get_device()), StreamOf(q)), "attention forward launch");
   return out;
 }
 
@@ -177,7 +177,7 @@ struct AttentionNode : public torch::autograd::Function<AttentionNode> {
     at::Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()), dv = at::empty(v.sizes(), v.options());
     at::Tensor delta = DeltaFor(stats);
     Check(LaunchAttnBackward(s, Described(q), Described(k), Described(v), Described(out), Described(saved[6]), Described(dout), StatsPtr(stats), StatsPtr(delta),
-                             Described(dq), Described(dk), Described(dv), AttnStatusWord(q.get_device()), StreamOf(q)), "attention backward");
+                             Described(dq), Described(dk), Described(dv), AttnStatusWord(q.get_device()), StreamOf(q)), "attention backward launch");
     variable_list g = Once("attention", {dq, dk, dv});
     return {g[0], g[1], g[2], at::Tensor(), at::Tensor()};
   }
@@ -192,7 +192,7 @@ at::Tensor QkvForward(const at::Tensor& qkv, int64_t h, int64_t hkv, const at::T
   if (kept != nullptr) kept->Make(s, out);
   Check(LaunchAttnForward(s, QkvPart(qkv, 0, s.dim), QkvPart(qkv, h, s.dim), QkvPart(qkv, h + hkv, s.dim), Described(out),
                           kept != nullptr ? Described(kept->low) : AttnTensor(), kept != nullptr ? StatsPtr(kept->stats) : nullptr, AttnStatusWord(qkv.get_device()), StreamOf(qkv)),
-        "attention forward");
+        "attention forward launch");
   return out;
 }
 
@@ -219,7 +219,7 @@ struct SelfAttentionNode : public torch::autograd::Function<SelfAttentionNode> {
     at::Tensor dqkv = at::empty(qkv.sizes(), qkv.options()), delta = DeltaFor(stats);
     Check(LaunchAttnBackward(s, QkvPart(qkv, 0, s.dim), QkvPart(qkv, h, s.dim), QkvPart(qkv, h + hkv, s.dim), Described(out), Described(saved[4]), Described(dout),
                              StatsPtr(stats), StatsPtr(delta), QkvPart(dqkv, 0, s.dim), QkvPart(dqkv, h, s.dim), QkvPart(dqkv, h + hkv, s.dim),
-                             AttnStatusWord(qkv.get_device()), StreamOf(qkv)), "attention backward");
+                             AttnStatusWord(qkv.get_device()), StreamOf(qkv)), "attention backward launch");
     return {Once("attention", {dqkv})[0], at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
   }
 };
@@ -243,7 +243,7 @@ at::Tensor DropoutLaunch(const at::Tensor& x, const at::Tensor& residual, int64_
   at::Tensor out = at::empty(x.sizes(), x.options());
   Check(LaunchDropoutAdd(a.data_ptr(), r.defined() ? r.data_ptr() : nullptr, out.data_ptr(), a.numel(), type, static_cast<unsigned int>(threshold),
                          static_cast<float>(factor), reinterpret_cast<const long long*>(k.data_ptr<int64_t>()),
-                         static_cast<unsigned int>(site), StreamOf(x)), "dropout_add");
+                         static_cast<unsigned int>(site), StreamOf(x)), "dropout_add launch");
   return out;
 }
 
@@ -278,14 +278,14 @@ at::Tensor GatedProduct(const at::Tensor& a, const at::Tensor& w_gate_up, int64_
   if (factors != nullptr) *factors = at::empty({m, 2 * f}, a.options().dtype(at::kShort));
   Check(LaunchGemmBf16Gated(a.data_ptr(), w_gate_up.data_ptr(), h.data_ptr(), factors != nullptr ? factors->data_ptr() : nullptr, static_cast<int>(m),
                             static_cast<int>(f), static_cast<int>(a.size(1)), static_cast<int>(act), GemmStatus(a), StreamOf(a)),
-        "gated_mlp");
+        "gated_mlp launch");
   return h;
 }
 at::Tensor DownProduct(const at::Tensor& h, const at::Tensor& w_down, const at::Tensor& residual) {
   at::Tensor y = at::empty({h.size(0), w_down.size(0)}, h.options());
   Check(LaunchGemmGatedDown(h.data_ptr(), w_down.data_ptr(), y.data_ptr(), static_cast<int>(h.size(0)), static_cast<int>(w_down.size(0)),
                             static_cast<int>(h.size(1)), GemmStatus(h), StreamOf(h), residual.defined() ? residual.data_ptr() : nullptr),
-        "gated_mlp");
+        "gated_mlp launch");
   return y;
 }
 at::Tensor Rows2d(const at::Tensor& t) { return Dense(t.reshape({-1, t.size(-1)})); }
@@ -323,7 +323,7 @@ struct GatedMlpNode : public torch::autograd::Function<GatedMlpNode> {
       // [dG dU] straight from the epilogue of dH = dy Wd
       dpre = at::empty(factors.sizes(), a.options());
       Check(LaunchGemmBf16NNGatedGrad(dy.data_ptr(), wd.data_ptr(), factors.data_ptr(), dpre.data_ptr(), m, f, n, GemmStatus(a), StreamOf(a)),
-            "gated_mlp backward");
+            "gated_mlp backward launch");
       if (ctx->needs_input_grad(0)) {
         da = at::empty(a.sizes(), a.options());
         list[count++] = {dpre.data_ptr(), wgu.data_ptr(), da.data_ptr(), m, k, 2 * f, false, false};
@@ -337,7 +337,7 @@ struct GatedMlpNode : public torch::autograd::Function<GatedMlpNode> {
       dwd = at::empty(wd.sizes(), a.options());
       list[count++] = {dy.data_ptr(), h.data_ptr(), dwd.data_ptr(), n, f, m, true, dpre.defined()};             // beside the last wave of dH
     }
-    if (count > 0) Check(LaunchGemmGroup(list, count, GemmStatus(a), StreamOf(a)), "gated_mlp backward");
+    if (count > 0) Check(LaunchGemmGroup(list, count, GemmStatus(a), StreamOf(a)), "gated_mlp backward launch");
     if (da.defined()) da = da.view(ctx->saved_data["sizes"].toIntVector());
     variable_list g = Once("gated_mlp", {da, dwgu, dwd});
     return {g[0], g[1], g[2], at::Tensor(), ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(3) ? grads[0] : at::Tensor()};
@@ -356,14 +356,20 @@ at::Tensor& StatusTensor(StatusWords& words, int device) {
   std::lock_guard<std::mutex> lock(words.mu);
   at::Tensor& w = words.of_device[device];
   if (!w.defined()) {
-    const c10::cuda::CUDAGuard guard(device);
-    // A first call inside a capture: the word must neither lie in the graph's memory nor be cleared by every replay.  Nothing that
-    // is captured runs before the capture ends, so this clearing has no need to be waited for.
+    // Cleared on a stream of its own and waited for, so that no stream's first kernel is overtaken by it.  In a capture that also
+    // keeps the word out of the graph's memory and its clearing out of the replays.
     c10::cuda::CUDAStreamCaptureModeGuard mode(cudaStreamCaptureModeRelaxed);
-    c10::cuda::OptionalCUDAStreamGuard side;
-    if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None)
-      side.reset_stream(c10::cuda::getStreamFromPool(false, device));
+    c10::cuda::CUDAStream side = c10::cuda::getStreamFromPool(false, device);
+    // streams of the pool are handed out in turn, so this one may be part of the capture itself
+    auto captured = [&] {
+      cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+      Check(cudaStreamIsCapturing(side.stream(), &status), "status word");
+      return status != cudaStreamCaptureStatusNone;
+    };
+    for (int i = 0; i < 64 && captured(); ++i) side = c10::cuda::getStreamFromPool(false, device);
+    const c10::cuda::CUDAStreamGuard on(side);
     w = at::zeros({1}, at::TensorOptions().device(at::kCUDA, device).dtype(at::kInt));
+    side.synchronize();
   }
   return w;
 }
@@ -371,6 +377,16 @@ at::Tensor& StatusTensor(StatusWords& words, int device) {
 unsigned int* AttnStatusWord(int device) {
   static StatusWords words;
   return reinterpret_cast<unsigned int*>(StatusTensor(words, device).data_ptr<int>());
+}
+
+unsigned int TakeAttnStatus(int device) {
+  const c10::cuda::CUDAGuard guard(device);
+  unsigned int* word = AttnStatusWord(device);
+  at::Tensor value = at::empty({1}, at::TensorOptions().device(at::kCUDA, device).dtype(at::kInt));
+  // every stream's calls up to now; one of another thread that ends meanwhile is reported now or next time
+  Check(cudaDeviceSynchronize(), "waiting for the device");
+  Check(LaunchTakeStatus(word, reinterpret_cast<unsigned int*>(value.data_ptr<int>()), StreamOf(value)), "attention status");
+  return static_cast<unsigned int>(value.item<int>());
 }
 
 at::Tensor CausalAttention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const c10::optional<at::Tensor>& cu, double scale) {

@@ -35,6 +35,8 @@ at::Tensor& StatusTensor(StatusWords& words, int device);
 
 // That of the attention kernels (bits: AttnStatus), and the one that the GEMM kernels share.
 unsigned int* AttnStatusWord(int device);
+// The bits of the attention kernels of all streams since they were last taken; waits for the device.
+unsigned int TakeAttnStatus(int device);
 at::Tensor& GemmStatusWord(const at::Tensor& like);
 
 }  // namespace bfb

@@ -1118,6 +1118,8 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   wait_for_kernel_before();                            // the end of this launch is the end of those before it
 }
 
+__global__ void take_status_kernel(unsigned int* status, unsigned int* value) { *value = atomicExch(status, 0u); }
+
 // ---- host side ---------------------------------------------------------------------------------------------------
 
 bool MakeMap(CUtensorMap* map, const AttnTensor& t, int heads, int dim, long long tokens, int rows) {
@@ -1229,6 +1231,13 @@ cudaError_t Backward(const AttnShape& s, const CUtensorMap& mq, const CUtensorMa
 }
 
 }  // namespace
+
+cudaError_t LaunchTakeStatus(unsigned int* status, unsigned int* value, cudaStream_t stream) {
+  (void)cudaGetLastError();
+  take_status_kernel<<<1, 1, 0, stream>>>(status, value);
+  CountKernelLaunch();
+  return cudaGetLastError();
+}
 
 long long AttnTiles(const AttnShape& s) {
   return s.cu == nullptr ? s.batch * ((s.seq + kTile - 1) / kTile) : s.seq / kTile + s.batch + 1;

@@ -29,6 +29,9 @@ struct AttnShape {
 // Bits of the status word.
 enum AttnStatus : unsigned int { kAttnTimeout = 1u, kAttnBadSequences = 2u };
 
+// *value = *status, and *status = 0, in one step.
+cudaError_t LaunchTakeStatus(unsigned int* status, unsigned int* value, cudaStream_t stream);
+
 // 128-row tiles that the launches below cover; the row statistics hold 128 floats per head and tile.
 long long AttnTiles(const AttnShape& s);
 bool AttnSupported(const AttnShape& s);

@@ -105,7 +105,7 @@ def causal_self_attention(qkv, n_head, n_kv_head=None, cu_seqlens=None, scale=No
 
 def check_sequences(device=None):
     """Raises IndexError if a kernel on ``device`` (default: the current one) since the last check was given ``cu_seqlens``
-    that fall or reach past the last token, and RuntimeError if a kernel gave up waiting.  Synchronises with the device."""
+    that fall or reach past the last token, and RuntimeError if a kernel gave up waiting.  Waits for the device, all streams."""
     index = torch.device(device).index if device is not None else None
     status = _b.native.attn_status(torch.cuda.current_device() if index is None else index)
     if status & 1:
