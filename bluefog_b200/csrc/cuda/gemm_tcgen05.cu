@@ -136,12 +136,12 @@ __device__ __forceinline__ uint32_t pack_factors(float lo, float hi) {
   const uint32_t ma = min((a & 0x7fffffffu) + 0x2000u, 0x1fffffffu) >> 14, mb = min((b & 0x7fffffffu) + 0x2000u, 0x1fffffffu) >> 14;
   return ((a >> 16) & 0x8000u) | ma | (b & 0x80000000u) | (mb << 16);
 }
-// The factors in a word, times 2^-90.
-__device__ __forceinline__ float2 unpack_factors(uint32_t w) {
-  return make_float2(__uint_as_float(((w << 16) & 0x80000000u) | ((w << 14) & 0x1fffc000u)),
-                     __uint_as_float((w & 0x80000000u) | ((w >> 2) & 0x1fffc000u)));
-}
+// The factors in a word.  Their scale is taken off here and not with dH, which it would make infinite from 2^38 on.
 constexpr float kFactorUnscale = 1.2379400392853803e27f;                       // 2^90
+__device__ __forceinline__ float2 unpack_factors(uint32_t w) {
+  return make_float2(__uint_as_float(((w << 16) & 0x80000000u) | ((w << 14) & 0x1fffc000u)) * kFactorUnscale,
+                     __uint_as_float((w & 0x80000000u) | ((w >> 2) & 0x1fffc000u)) * kFactorUnscale);
+}
 constexpr uint32_t kFactorNan = 0x7fffu;
 
 // eight floats as bf16, 16 bytes
@@ -705,7 +705,7 @@ gemm_bf16_nt_persistent_kernel(const __grid_constant__ CUtensorMap map_a, const 
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               top = __vmaxu2(top, __vmaxu2(f[i] & 0x7fff7fffu, d[i] & 0x7fff7fffu));
-              const float h0 = __uint_as_float(r[j * 8 + 2 * i]) * kFactorUnscale, h1 = __uint_as_float(r[j * 8 + 2 * i + 1]) * kFactorUnscale;
+              const float h0 = __uint_as_float(r[j * 8 + 2 * i]), h1 = __uint_as_float(r[j * 8 + 2 * i + 1]);
               const float2 x = unpack_factors(f[i]), y = unpack_factors(d[i]);
               b[2 * i] = h0 * x.x;
               b[2 * i + 1] = h1 * x.y;
