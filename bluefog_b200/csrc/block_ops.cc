@@ -281,8 +281,9 @@ at::Tensor GatedProduct(const at::Tensor& a, const at::Tensor& w_gate_up, int64_
         "gated_mlp launch");
   return h;
 }
-at::Tensor DownProduct(const at::Tensor& h, const at::Tensor& w_down, const at::Tensor& residual) {
-  at::Tensor y = at::empty({h.size(0), w_down.size(0)}, h.options());
+// y has the given shape from the start: autograd would refuse to change a view made in a node's forward pass in place.
+at::Tensor DownProduct(const at::Tensor& h, const at::Tensor& w_down, const at::Tensor& residual, at::IntArrayRef shape) {
+  at::Tensor y = at::empty(shape, h.options());
   Check(LaunchGemmGatedDown(h.data_ptr(), w_down.data_ptr(), y.data_ptr(), static_cast<int>(h.size(0)), static_cast<int>(w_down.size(0)),
                             static_cast<int>(h.size(1)), GemmStatus(h), StreamOf(h), residual.defined() ? residual.data_ptr() : nullptr),
         "gated_mlp launch");
@@ -303,11 +304,11 @@ struct GatedMlpNode : public torch::autograd::Function<GatedMlpNode> {
     const at::Tensor res = residual.has_value() ? Rows2d(*residual) : at::Tensor();
     at::Tensor factors;
     const at::Tensor h = GatedProduct(a, wgu, act, &factors);
-    at::Tensor y = DownProduct(h, wd, res);
+    at::Tensor y = DownProduct(h, wd, res, WithColumns(a0, wd.size(0)));
     ctx->save_for_backward({a, wgu, wd, factors, h});
     ctx->saved_data["residual"] = residual.has_value();
     ctx->saved_data["sizes"] = a0.sizes().vec();
-    return y.view(WithColumns(a0, wd.size(0)));
+    return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list saved = ctx->get_saved_variables();
@@ -426,7 +427,7 @@ c10::optional<at::Tensor> GatedMlp(const at::Tensor& a, const at::Tensor& w_gate
   if (NeedsGrad({a, w_gate_up, w_down, r})) return GatedMlpNode::apply(a, w_gate_up, w_down, act, residual);
   // nothing is launched between the two products: the second one reads its other operands before the kernel in front of it ends
   const at::Tensor x = Rows2d(a), wgu = Dense(w_gate_up), wd = Dense(w_down), res = r.defined() ? Rows2d(r) : r;
-  return DownProduct(GatedProduct(x, wgu, act, nullptr), wd, res).view(WithColumns(a, w_down.size(0)));
+  return DownProduct(GatedProduct(x, wgu, act, nullptr), wd, res, WithColumns(a, w_down.size(0)));
 }
 
 }  // namespace bfb
