@@ -5,6 +5,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -37,6 +38,15 @@ bool NeedsGrad(std::initializer_list<at::Tensor> tensors) {
   for (const at::Tensor& t : tensors)
     if (t.defined() && t.requires_grad()) return true;
   return false;
+}
+
+// The kernels know nothing of tangents: an input that carries one (of any of the three operators or of their backward passes) is an
+// error, or the result would pass for a constant.
+template <typename... Tensors>
+void NoTangents(const char* what, const Tensors&... tensors) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  const bool any = ((tensors.defined() && tensors._fw_grad(/*level=*/0).defined()) || ...);
+  TORCH_CHECK_NOT_IMPLEMENTED(!any, what, ": forward-mode differentiation is not supported");
 }
 
 // Gradients of these operators are not differentiable; asking for theirs is an error, at the time they are asked for.
@@ -173,6 +183,7 @@ struct AttentionNode : public torch::autograd::Function<AttentionNode> {
     const at::Tensor &q = saved[0], &k = saved[1], &v = saved[2], &out = saved[4], &stats = saved[5];
     const c10::cuda::CUDAGuard guard(q.get_device());
     const AttnShape s = ShapeOf(q, k, saved[3], ctx->saved_data["scale"].toDouble());
+    NoTangents("attention", grads[0]);
     const at::Tensor dout = Rows(grads[0]);
     at::Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()), dv = at::empty(v.sizes(), v.options());
     at::Tensor delta = DeltaFor(stats);
@@ -215,6 +226,7 @@ struct SelfAttentionNode : public torch::autograd::Function<SelfAttentionNode> {
     const c10::cuda::CUDAGuard guard(qkv.get_device());
     const int64_t h = ctx->saved_data["h"].toInt(), hkv = ctx->saved_data["hkv"].toInt();
     const AttnShape s = QkvShape(qkv, h, hkv, saved[1], ctx->saved_data["scale"].toDouble());
+    NoTangents("attention", grads[0]);
     const at::Tensor dout = Rows(grads[0]);
     at::Tensor dqkv = at::empty(qkv.sizes(), qkv.options()), delta = DeltaFor(stats);
     Check(LaunchAttnBackward(s, QkvPart(qkv, 0, s.dim), QkvPart(qkv, h, s.dim), QkvPart(qkv, h + hkv, s.dim), Described(out), Described(saved[4]), Described(dout),
@@ -314,6 +326,7 @@ struct GatedMlpNode : public torch::autograd::Function<GatedMlpNode> {
     const variable_list saved = ctx->get_saved_variables();
     const at::Tensor &a = saved[0], &wgu = saved[1], &wd = saved[2], &factors = saved[3], &h = saved[4];
     const c10::cuda::CUDAGuard guard(a.get_device());
+    NoTangents("gated_mlp", grads[0]);
     const at::Tensor dy = Rows2d(grads[0]);
     const int m = static_cast<int>(a.size(0)), f = static_cast<int>(h.size(1)), k = static_cast<int>(a.size(1));
     const int n = static_cast<int>(wd.size(0));
@@ -393,6 +406,7 @@ unsigned int TakeAttnStatus(int device) {
 at::Tensor CausalAttention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const c10::optional<at::Tensor>& cu, double scale) {
   TORCH_CHECK(q.is_cuda() && k.is_cuda() && v.is_cuda(), "attention expects CUDA tensors");
   const c10::cuda::CUDAGuard guard(q.get_device());
+  NoTangents("attention", q, k, v);
   if (NeedsGrad({q, k, v})) return AttentionNode::apply(q, k, v, cu, scale);
   return SeparateForward(Rows(q), Rows(k), Rows(v), OrUndefined(cu), scale, nullptr);
 }
@@ -400,6 +414,7 @@ at::Tensor CausalAttention(const at::Tensor& q, const at::Tensor& k, const at::T
 at::Tensor CausalSelfAttention(const at::Tensor& qkv, int64_t heads, int64_t kv_heads, const c10::optional<at::Tensor>& cu, double scale) {
   TORCH_CHECK(qkv.is_cuda(), "attention expects CUDA tensors");
   const c10::cuda::CUDAGuard guard(qkv.get_device());
+  NoTangents("attention", qkv);
   if (NeedsGrad({qkv})) return SelfAttentionNode::apply(qkv, heads, kv_heads, cu, scale);
   return QkvForward(QkvRows(qkv), heads, kv_heads, OrUndefined(cu), scale, nullptr);
 }
@@ -409,6 +424,7 @@ at::Tensor DropoutAdd(const at::Tensor& x, const c10::optional<at::Tensor>& resi
   TORCH_CHECK(x.is_cuda(), "dropout_add expects a CUDA tensor");
   const c10::cuda::CUDAGuard guard(x.get_device());
   const at::Tensor r = OrUndefined(residual);
+  NoTangents("dropout_add", x, r);
   if (NeedsGrad({x, r})) return DropoutNode::apply(x, residual, threshold, factor, key, site);
   return DropoutLaunch(x, r, threshold, factor, key, site);
 }
@@ -424,6 +440,7 @@ c10::optional<at::Tensor> GatedMlp(const at::Tensor& a, const at::Tensor& w_gate
     return c10::nullopt;
   if (r.defined() && r.sizes() != at::IntArrayRef(WithColumns(a, w_down.size(0)))) return c10::nullopt;
   const c10::cuda::CUDAGuard guard(a.get_device());
+  NoTangents("gated_mlp", a, w_gate_up, w_down, r);
   if (NeedsGrad({a, w_gate_up, w_down, r})) return GatedMlpNode::apply(a, w_gate_up, w_down, act, residual);
   // nothing is launched between the two products: the second one reads its other operands before the kernel in front of it ends
   const at::Tensor x = Rows2d(a), wgu = Dense(w_gate_up), wd = Dense(w_down), res = r.defined() ? Rows2d(r) : r;
