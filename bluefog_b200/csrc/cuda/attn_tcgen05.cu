@@ -358,7 +358,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   const int order = divide(blockIdx.x, g.by_heads);
   const int head = blockIdx.x - order * g.heads;
   if (g.cu != nullptr && blockIdx.x == 0) {
-    bool bad = false;
+    bool bad = threadIdx.x == 0 && __ldg(g.cu) != 0;   // taken as 0 all the same
     for (int b = threadIdx.x; b < g.batch; b += blockDim.x) {
       const int c = __ldg(g.cu + b + 1);
       bad |= c < (b == 0 ? 0 : __ldg(g.cu + b)) || c > g.seq;

@@ -8,8 +8,8 @@ shape.  Both return ``[..., T, H, D]``: position i attends to the positions up t
 Without ``cu_seqlens`` every row of T tokens is one sequence.  With it (int32 ``[B + 1]`` on the inputs' device, starting
 at 0 and never falling) all tokens together, in order, hold sequences of different lengths: sequence b is
 ``[cu_seqlens[b], cu_seqlens[b + 1])`` and may be empty; tokens behind the last one belong to none, and their results and
-gradients are zero whatever they hold.  The lengths stay on the device.  The kernels clip boundaries that fall or reach
-past the last token and ``check_sequences`` reports them.
+gradients are zero whatever they hold.  The lengths stay on the device.  The kernels take the first boundary as 0, clip
+boundaries that fall or reach past the last token, and ``check_sequences`` reports them.
 
 bf16 CUDA tensors with D a multiple of 8 up to 128 take the kernels, forward and backward, with any row spacing that is
 a multiple of 16 bytes; everything else (CPU, fp32, fp16, other widths) takes PyTorch's operators, sequence by sequence.
@@ -105,10 +105,10 @@ def causal_self_attention(qkv, n_head, n_kv_head=None, cu_seqlens=None, scale=No
 
 def check_sequences(device=None):
     """Raises IndexError if a kernel on ``device`` (default: the current one) since the last check was given ``cu_seqlens``
-    that fall or reach past the last token, and RuntimeError if a kernel gave up waiting.  Waits for the device, all streams."""
+    that do not start at 0, fall or reach past the last token, and RuntimeError if a kernel gave up waiting.  Waits for the device, all streams."""
     index = torch.device(device).index if device is not None else None
     status = _b.native.attn_status(torch.cuda.current_device() if index is None else index)
     if status & 1:
         raise RuntimeError("an attention kernel ran into its time limit")
     if status & 2:
-        raise IndexError("cu_seqlens fall or reach past the last token")
+        raise IndexError("cu_seqlens do not start at 0, fall or reach past the last token")

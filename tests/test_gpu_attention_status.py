@@ -31,3 +31,15 @@ def test_a_report_from_another_stream():
         fa.check_sequences()
     torch.cuda.synchronize()
     fa.check_sequences()                                              # reported once
+
+
+@pytest.mark.parametrize("first", [128, 1, -3])
+def test_boundaries_that_do_not_start_at_zero(first):
+    """The kernels take the first boundary as 0; that it is another one is reported, as the CPU path does."""
+    from bluefog_b200.ops import fused_attention as fa
+    qkv = torch.zeros(256, 3 * 64, dtype=torch.bfloat16, device="cuda")
+    fa.causal_self_attention(qkv, 1, cu_seqlens=torch.tensor([first, 256], dtype=torch.int32, device="cuda"))
+    with pytest.raises(IndexError, match="start at 0"):
+        fa.check_sequences()
+    fa.causal_self_attention(qkv, 1, cu_seqlens=torch.tensor([0, 256], dtype=torch.int32, device="cuda"))
+    fa.check_sequences()
