@@ -142,8 +142,8 @@ class GPT2(nn.Module):
         self.use_b200_gemm = use_b200_gemm
         self.dropout = dropout
         if dropout > 0.0:
-            # [seed, step]; part of the state, so that a resumed run goes on with the masks it would have drawn.  Ranks that
-            # took it from one another by a broadcast draw the same masks until their seeds are set apart.
+            # [seed, step]; part of the state, so that a resumed run goes on with the masks it would have drawn.  Ranks may
+            # take it from one another by a broadcast: each draws masks of its own from it (rank_key).
             self.register_buffer("dropout_key", fused_dropout.new_key(torch.initial_seed() % 2 ** 62))
         self.apply(self._init)
         for name, p in self.named_parameters():
@@ -166,7 +166,7 @@ class GPT2(nn.Module):
         x = fused_embedding.token_position_embedding(idx, self.wte.weight, self.wpe.weight)   # wte[idx] + wpe[:t]
         key = None
         if self.dropout > 0.0 and self.training:
-            key = self.dropout_key.clone()             # the backward pass reads this step's key, the buffer goes on
+            key = fused_dropout.rank_key(self.dropout_key)      # the backward pass reads this step's key, the buffer goes on
             self.dropout_key[1] += 1
             x = fused_dropout.dropout_add(x, None, self.dropout, key)
         for i, block in enumerate(self.h):

@@ -5,7 +5,8 @@ key (int64 ``[seed, step]`` on the device of x), the ``site`` (a number below 65
 apart) and the element's place in x, so no mask is stored: the backward pass computes it again, and the same call gives
 the same mask on every device, in every type.  The key is read on the device: a captured graph whose key is advanced
 between (or inside) replays draws new masks.  The key must not change between a forward pass and its backward pass
-(autograd reports it); keep one and hand out copies, as ``models/gpt2.py`` does.
+(autograd reports it); keep one and hand out copies, as ``models/gpt2.py`` does.  Ranks that start from one another's state
+(``broadcast_parameters(model.state_dict())``) hold the same key: ``rank_key`` gives each of them a copy of its own.
 
 Element i takes the 16-bit word i % 8 of block i // 8 of Philox4x32-10 (Salmon et al., SC 2011) and is dropped if that is
 below ``round(65536 p)``; p is thereby rounded to a multiple of 2^-16 and the factor uses the rounded value.  Dropped
@@ -22,6 +23,17 @@ _b = get_basics()
 def new_key(seed, device=None):
     """A key for ``dropout_add``: ``[seed, 0]``; add to its second element from step to step."""
     return torch.tensor([seed, 0], dtype=torch.int64, device=device)
+
+
+def rank_key(key):
+    """A copy of ``key`` for this rank's masks: the seed plus a multiple of the rank, so rank 0 (and a process that has not called
+    ``init``) draws those of the key itself.  The multiple is 2^64 over the golden ratio: no two ranks with small seeds of their
+    own can meet."""
+    rank = _b.rank() if _b.is_initialized() else 0
+    own = key.clone()
+    if rank != 0:
+        own[0] += (rank * 0x9E3779B97F4A7C15 + 2 ** 63) % 2 ** 64 - 2 ** 63      # wraps, as the addition does
+    return own
 
 
 def _eligible(x):

@@ -992,6 +992,36 @@ def gpu_wait_timeout():
     bf.barrier()
 
 
+@case
+def dropout_masks():
+    """After the state was broadcast the ranks hold one dropout key, and still drop different elements; the key stays common."""
+    from bluefog_b200.models import gpt2
+    r, n, d = bf.rank(), bf.size(), dev()
+    torch.manual_seed(1 + r)
+    model = gpt2.GPT2(vocab_size=50, n_positions=16, d_model=16, n_layer=1, n_head=2, dropout=0.5).to(d)
+    bf.broadcast_parameters(model.state_dict(), root_rank=0)
+    keys = bf.allgather(model.dropout_key.view(1, 2))
+    assert keys.tolist() == [[1, 0]] * n
+    torch.manual_seed(9)
+    idx = torch.randint(0, 50, (2, 16), device=d)
+
+    def logits():
+        return bf.allgather(model(idx).detach().reshape(1, -1).float())
+
+    for step in range(2):
+        out = logits()
+        for i, j in itertools.combinations(range(n), 2):
+            assert not torch.equal(out[i], out[j]), (step, i, j)
+    keys = bf.allgather(model.dropout_key.view(1, 2))
+    assert keys.tolist() == [[1, 2]] * n
+    # the same step again draws the same masks
+    model.dropout_key[1] = 1
+    assert torch.equal(logits(), out)
+    model.eval()
+    out = logits()
+    assert all(torch.equal(out[0], o) for o in out)
+
+
 def main():
     name = sys.argv[1]
     if name not in ("timeline",):
