@@ -12,7 +12,8 @@ gradients are zero whatever they hold.  The lengths stay on the device.  The ker
 boundaries that fall or reach past the last token, and ``check_sequences`` reports them.
 
 bf16 CUDA tensors with D a multiple of 8 up to 128 take the kernels, forward and backward, with any row spacing that is
-a multiple of 16 bytes; everything else (CPU, fp32, fp16, other widths) takes PyTorch's operators, sequence by sequence.
+a multiple of 16 bytes; everything else (CPU, fp32, fp16, other widths, scales that fp32 cannot hold) takes PyTorch's
+operators, sequence by sequence.
 Results and gradients are the same in every run.  As in a softmax written out, a weight of zero does not hide an infinite
 or NaN value of a later position of the same sequence: earlier positions may become NaN.  Before a forward and backward
 pass is captured into a graph, drop eager results of the same leaves: autograd would join their stream with the captured
@@ -32,6 +33,11 @@ def _eligible(t, d):
     """Whether the kernels take ``t`` (q, or q, k and v side by side) with heads of width ``d``."""
     return (t.is_cuda and t.dtype == torch.bfloat16 and d % 8 == 0 and 8 <= d <= 128 and t.numel() // d < 2 ** 31 - 256
             and _b.native.gemm_supported())
+
+
+def _takes(t, d, scale):
+    """Whether the kernels take the call; scales are fp32 numbers there, and so is their product with log2 e."""
+    return 2.0 ** -126 <= scale <= 2.0 ** 126 and _eligible(t, d)
 
 
 def _split(qkv, h, hkv):
@@ -85,7 +91,7 @@ def causal_attention(q, k, v, cu_seqlens=None, scale=None):
     scale = _check(q.shape[-2], k.shape[-2], q.shape[-1], q.device, cu_seqlens, scale)
     if q.numel() == 0:
         return q + (k.sum() + v.sum()) * 0
-    if not _eligible(q, q.shape[-1]):
+    if not _takes(q, q.shape[-1], scale):
         return _plain(q, k, v, cu_seqlens, scale)
     return _b.native.causal_attention(q, k, v, None if cu_seqlens is None else cu_seqlens.contiguous(), scale)
 
@@ -98,7 +104,7 @@ def causal_self_attention(qkv, n_head, n_kv_head=None, cu_seqlens=None, scale=No
                          % (qkv.shape[-1], n_head, hkv))
     scale = _check(n_head, hkv, qkv.shape[-1] // (n_head + 2 * hkv), qkv.device, cu_seqlens, scale)
     d = qkv.shape[-1] // (n_head + 2 * hkv)
-    if qkv.numel() == 0 or not _eligible(qkv, d):
+    if qkv.numel() == 0 or not _takes(qkv, d, scale):
         return causal_attention(*_split(qkv, n_head, hkv), cu_seqlens, scale)
     return _b.native.causal_self_attention(qkv, n_head, hkv, None if cu_seqlens is None else cu_seqlens.contiguous(), scale)
 
