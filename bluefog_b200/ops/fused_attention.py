@@ -12,9 +12,8 @@ gradients are zero whatever they hold.  The lengths stay on the device.  The ker
 boundaries that fall or reach past the last token, and ``check_sequences`` reports them.
 
 bf16 CUDA tensors with D a multiple of 8 up to 128 take the kernels, forward and backward, with any row spacing that is
-a multiple of 16 bytes; everything else (CPU, fp32, fp16, other widths, scales that fp32 cannot hold) takes PyTorch's
-operators, sequence by sequence.
-Results and gradients are the same in every run.  As in a softmax written out, a weight of zero does not hide an infinite
+a multiple of 16 bytes; everything else (CPU, fp32, fp16, other widths, scales that fp32 cannot hold, 2^30 tiles of 128
+rows and a head) takes PyTorch's operators, sequence by sequence.  Results and gradients are the same in every run.  As in a softmax written out, a weight of zero does not hide an infinite
 or NaN value of a later position of the same sequence: earlier positions may become NaN.  Before a forward and backward
 pass is captured into a graph, drop eager results of the same leaves: autograd would join their stream with the captured
 one, which PyTorch answers with an error or worse.  The reference has no attention code; ``models/gpt2.py`` calls this.
@@ -35,9 +34,22 @@ def _eligible(t, d):
             and _b.native.gemm_supported())
 
 
-def _takes(t, d, scale):
-    """Whether the kernels take the call; scales are fp32 numbers there, and so is their product with log2 e."""
-    return 2.0 ** -126 <= scale <= 2.0 ** 126 and _eligible(t, d)
+def _fits(lead, heads, batch):
+    """Whether tokens [*lead] with this many query heads, in ``batch`` packed sequences or one per row (None), stay within the
+    31 bits that the kernels' grids and row coordinates have: 128-row tiles times heads, twice in the backward pass."""
+    tokens = math.prod(lead)
+    tiles = tokens // lead[-1] * ((lead[-1] + 127) // 128) if batch is None else tokens // 128 + batch + 1
+    return tokens < 2 ** 31 - 256 and tiles * heads < 2 ** 30
+
+
+def _takes(t, d, inner, heads, cu, scale):
+    """Whether the kernels take the call, ``inner`` trailing dimensions of t being a row; scales are fp32 numbers there, and so is
+    their product with log2 e."""
+    if not (2.0 ** -126 <= scale <= 2.0 ** 126 and _eligible(t, d)):
+        return False
+    if t.numel() < 2 ** 30 and (cu is None or cu.numel() * heads < 2 ** 28):
+        return True                                                   # at most a tile per token and boundary, which takes less time to see
+    return _fits(t.shape[:-inner], heads, None if cu is None else cu.numel() - 1)
 
 
 def _split(qkv, h, hkv):
@@ -91,7 +103,7 @@ def causal_attention(q, k, v, cu_seqlens=None, scale=None):
     scale = _check(q.shape[-2], k.shape[-2], q.shape[-1], q.device, cu_seqlens, scale)
     if q.numel() == 0:
         return q + (k.sum() + v.sum()) * 0
-    if not _takes(q, q.shape[-1], scale):
+    if not _takes(q, q.shape[-1], 2, q.shape[-2], cu_seqlens, scale):
         return _plain(q, k, v, cu_seqlens, scale)
     return _b.native.causal_attention(q, k, v, None if cu_seqlens is None else cu_seqlens.contiguous(), scale)
 
@@ -104,7 +116,7 @@ def causal_self_attention(qkv, n_head, n_kv_head=None, cu_seqlens=None, scale=No
                          % (qkv.shape[-1], n_head, hkv))
     scale = _check(n_head, hkv, qkv.shape[-1] // (n_head + 2 * hkv), qkv.device, cu_seqlens, scale)
     d = qkv.shape[-1] // (n_head + 2 * hkv)
-    if qkv.numel() == 0 or not _takes(qkv, d, scale):
+    if qkv.numel() == 0 or not _takes(qkv, d, 1, n_head, cu_seqlens, scale):
         return causal_attention(*_split(qkv, n_head, hkv), cu_seqlens, scale)
     return _b.native.causal_self_attention(qkv, n_head, hkv, None if cu_seqlens is None else cu_seqlens.contiguous(), scale)
 
