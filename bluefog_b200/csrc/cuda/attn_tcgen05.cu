@@ -4,6 +4,10 @@
 //   backward  delta = rowsum(dout * out),  dP = dout v^T,  dS = P (dP - delta)
 //             dv = P^T dout (summed over the query heads of a group),  dk = scale dS^T q (ditto),  dq = scale dS k
 //
+// Head widths are padded to 64 or 128 columns: TMA fills the boxes up with zeros, and all MMA steps run over them (80 columns: eight
+// steps in the scores where five hold data).  Two widths are compiled, not sixteen; for heads up to 64 the products are not what the
+// time goes to (8 x 1024 tokens, 16 heads: 35 of 40 us without any), and what steps by the width would gain has not been measured.
+//
 // No kernel writes a score to memory: a CTA keeps 128 queries (or keys) and walks over the others 64 or 128 at a time.  The backward
 // pass has two kinds of CTAs: those that own a key tile (dk, dv) and those that own a query tile (dq), seven products per tile
 // instead of five, but no atomics, so gradients do not depend on the order in which CTAs run, and no fp32 copy of dq.

@@ -990,7 +990,8 @@ gemm_bf16_nt_persistent_kernel(const __grid_constant__ CUtensorMap map_a, const 
 // longest reductions come first, but for those that need nothing of the kernel before (the down projection's weight gradient
 // does not need the gradient of the gate): they fill the SMs that its last wave leaves idle (1537 x 776 x 2056,
 // whose dH has 63 tiles: 101 -> 99 us for the block).  B is [reduction, N] row-major in all of them; A is [M, reduction] or, for a
-// weight gradient, [reduction, M].
+// weight gradient, [reduction, M].  The tile is the same for all sizes: a width of 776 takes four of 256, and the last one holds
+// eight columns; narrower ones have not been tried in this launch.
 // ------------------------------------------------------------------------------------------ //
 constexpr int kMaxGroup = 3;
 struct GroupProblem {

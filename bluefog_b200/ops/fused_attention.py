@@ -13,10 +13,12 @@ boundaries that fall or reach past the last token, and ``check_sequences`` repor
 
 bf16 CUDA tensors with D a multiple of 8 up to 128 take the kernels, forward and backward, with any row spacing that is
 a multiple of 16 bytes; everything else (CPU, fp32, fp16, other widths, scales that fp32 cannot hold, 2^30 tiles of 128
-rows and a head) takes PyTorch's operators, sequence by sequence.  Results and gradients are the same in every run.  As in a softmax written out, a weight of zero does not hide an infinite
-or NaN value of a later position of the same sequence: earlier positions may become NaN.  Before a forward and backward
-pass is captured into a graph, drop eager results of the same leaves: autograd would join their stream with the captured
-one, which PyTorch answers with an error or worse.  The reference has no attention code; ``models/gpt2.py`` calls this.
+rows and a head) takes PyTorch's operators, sequence by sequence.  Results and gradients are the same in every run.  As in
+a softmax written out, a weight of zero does not hide an infinite or NaN value of a later position of the same sequence:
+earlier positions may become NaN.  Before a forward and backward pass is captured into a graph, drop eager results of the
+same leaves: autograd would join their stream with the captured one, which PyTorch answers with an error or worse.
+Gradients of gradients and forward-mode differentiation of the kernels are errors.  The reference has no attention code;
+``models/gpt2.py`` calls this.
 """
 import math
 

@@ -11,7 +11,8 @@ between (or inside) replays draws new masks.  The key must not change between a 
 Element i takes the 16-bit word i % 8 of block i // 8 of Philox4x32-10 (Salmon et al., SC 2011) and is dropped if that is
 below ``round(65536 p)``; p is thereby rounded to a multiple of 2^-16 and the factor uses the rounded value.  Dropped
 elements are zero whatever x holds.  CUDA tensors in fp32, fp16 or bf16 take the kernel, the arithmetic is fp32; the rest
-takes the same generator in PyTorch's operators.  The reference has no dropout of its own.
+takes the same generator in PyTorch's operators.  Forward-mode differentiation of the kernel is an error.  The reference has
+no dropout of its own.
 """
 import torch
 

@@ -262,7 +262,8 @@ def gated_mlp(a: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor, ac
     ``[N, F]``; ``a`` [.., K], ``residual`` [.., N]; ``act`` "silu" or "gelu" (the tanh approximation).  bf16 CUDA tensors
     with K, F and N multiples of 8 take the tcgen05 kernels, the activation and the product with the gate inside GEMM
     epilogues in both directions; other inputs take PyTorch's ops.  The kernels keep ``act(g)`` and ``u act'(g)`` for the
-    backward pass in 16 bits each: what is below 2^-36 counts as zero there, and what reaches 2^27 makes gradients NaN."""
+    backward pass in 16 bits each: what is below 2^-36 counts as zero there, and what reaches 2^27 makes gradients NaN.
+    Gradients of gradients and forward-mode differentiation of the kernels are errors."""
     if a.is_cuda and act in _GATES:
         # the arguments are looked at in C++ first: in Python that takes 6 us, as long as the device takes for few rows
         y = _b.native.gated_mlp(a, w_gate_up, w_down, _GATES[act], residual)
