@@ -49,6 +49,16 @@ void NoTangents(const char* what, const Tensors&... tensors) {
   TORCH_CHECK_NOT_IMPLEMENTED(!any, what, ": forward-mode differentiation is not supported");
 }
 
+// Tensors that stand for others (fake ones, which have no memory, and other subclasses that catch operators) do not reach a launch.
+template <typename... Tensors>
+bool AnyStandIn(const Tensors&... tensors) {
+  return ((tensors.defined() && tensors.unsafeGetTensorImpl()->is_python_dispatch()) || ...);
+}
+template <typename... Tensors>
+void NoStandIns(const char* what, const Tensors&... tensors) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!AnyStandIn(tensors...), what, ": the kernels take plain tensors, not fake ones or other subclasses");
+}
+
 // Gradients of these operators are not differentiable; asking for theirs is an error, at the time they are asked for.
 variable_list Once(const char* what, variable_list grads) {
   if (!at::GradMode::is_enabled()) return grads;
@@ -370,6 +380,8 @@ at::Tensor& StatusTensor(StatusWords& words, int device) {
   std::lock_guard<std::mutex> lock(words.mu);
   at::Tensor& w = words.of_device[device];
   if (!w.defined()) {
+    // Real memory also where a mode that catches operators is active.
+    const c10::impl::ExcludeDispatchKeyGuard no_modes(c10::python_ks);
     // Cleared on a stream of its own and waited for, so that no stream's first kernel is overtaken by it.  In a capture that also
     // keeps the word out of the graph's memory and its clearing out of the replays.
     c10::cuda::CUDAStreamCaptureModeGuard mode(cudaStreamCaptureModeRelaxed);
@@ -395,6 +407,7 @@ unsigned int* AttnStatusWord(int device) {
 
 unsigned int TakeAttnStatus(int device) {
   const c10::cuda::CUDAGuard guard(device);
+  const c10::impl::ExcludeDispatchKeyGuard no_modes(c10::python_ks);
   unsigned int* word = AttnStatusWord(device);
   at::Tensor value = at::empty({1}, at::TensorOptions().device(at::kCUDA, device).dtype(at::kInt));
   // every stream's calls up to now; one of another thread that ends meanwhile is reported now or next time
@@ -405,6 +418,7 @@ unsigned int TakeAttnStatus(int device) {
 
 at::Tensor CausalAttention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const c10::optional<at::Tensor>& cu, double scale) {
   TORCH_CHECK(q.is_cuda() && k.is_cuda() && v.is_cuda(), "attention expects CUDA tensors");
+  NoStandIns("attention", q, k, v, OrUndefined(cu));
   const c10::cuda::CUDAGuard guard(q.get_device());
   NoTangents("attention", q, k, v);
   if (NeedsGrad({q, k, v})) return AttentionNode::apply(q, k, v, cu, scale);
@@ -413,6 +427,7 @@ at::Tensor CausalAttention(const at::Tensor& q, const at::Tensor& k, const at::T
 
 at::Tensor CausalSelfAttention(const at::Tensor& qkv, int64_t heads, int64_t kv_heads, const c10::optional<at::Tensor>& cu, double scale) {
   TORCH_CHECK(qkv.is_cuda(), "attention expects CUDA tensors");
+  NoStandIns("attention", qkv, OrUndefined(cu));
   const c10::cuda::CUDAGuard guard(qkv.get_device());
   NoTangents("attention", qkv);
   if (NeedsGrad({qkv})) return SelfAttentionNode::apply(qkv, heads, kv_heads, cu, scale);
@@ -422,8 +437,9 @@ at::Tensor CausalSelfAttention(const at::Tensor& qkv, int64_t heads, int64_t kv_
 at::Tensor DropoutAdd(const at::Tensor& x, const c10::optional<at::Tensor>& residual, int64_t threshold, double factor,
                       const at::Tensor& key, int64_t site) {
   TORCH_CHECK(x.is_cuda(), "dropout_add expects a CUDA tensor");
-  const c10::cuda::CUDAGuard guard(x.get_device());
   const at::Tensor r = OrUndefined(residual);
+  NoStandIns("dropout_add", x, r, key);
+  const c10::cuda::CUDAGuard guard(x.get_device());
   NoTangents("dropout_add", x, r);
   if (NeedsGrad({x, r})) return DropoutNode::apply(x, residual, threshold, factor, key, site);
   return DropoutLaunch(x, r, threshold, factor, key, site);
@@ -439,6 +455,7 @@ c10::optional<at::Tensor> GatedMlp(const at::Tensor& a, const at::Tensor& w_gate
       w_down.size(1) % 8 != 0 || a.numel() / a.size(-1) >= (1ll << 31) - 256)
     return c10::nullopt;
   if (r.defined() && r.sizes() != at::IntArrayRef(WithColumns(a, w_down.size(0)))) return c10::nullopt;
+  if (AnyStandIn(a, w_gate_up, w_down, r)) return c10::nullopt;
   const c10::cuda::CUDAGuard guard(a.get_device());
   NoTangents("gated_mlp", a, w_gate_up, w_down, r);
   if (NeedsGrad({a, w_gate_up, w_down, r})) return GatedMlpNode::apply(a, w_gate_up, w_down, act, residual);

@@ -1238,6 +1238,7 @@ cudaError_t Backward(const AttnShape& s, const CUtensorMap& mq, const CUtensorMa
 
 cudaError_t LaunchTakeStatus(unsigned int* status, unsigned int* value, cudaStream_t stream) {
   (void)cudaGetLastError();
+  if (status == nullptr || value == nullptr) return cudaErrorInvalidValue;
   take_status_kernel<<<1, 1, 0, stream>>>(status, value);
   CountKernelLaunch();
   return cudaGetLastError();

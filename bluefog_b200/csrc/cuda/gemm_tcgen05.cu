@@ -1512,7 +1512,8 @@ cudaError_t Skinny(const void* x, const void* w, void* out, void* pre, const voi
   (void)cudaGetLastError();   // the value returned below must be this launch's own, not an older error of the calling thread
   const uintptr_t all = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(out) |
                         reinterpret_cast<uintptr_t>(pre) | reinterpret_cast<uintptr_t>(residual);
-  if (M <= 0 || M > kSkinnyRows || N <= 0 || K <= 0 || (K % 8) != 0 || (N % 8) != 0 || (all & 15) != 0) return cudaErrorInvalidValue;
+  if (M <= 0 || M > kSkinnyRows || N <= 0 || K <= 0 || (K % 8) != 0 || (N % 8) != 0 || (all & 15) != 0 || x == nullptr || w == nullptr || out == nullptr)
+    return cudaErrorInvalidValue;
   const int nb = M <= 16 ? 16 : M <= 32 ? 32 : 64;
   CUtensorMap lo, hi, mx;
   if (!MakeMap(&lo, w, N, K, 64) || !MakeMap(&mx, x, M, K, nb)) return cudaErrorInvalidValue;
@@ -1538,7 +1539,8 @@ cudaError_t LaunchGemmGatedDown(const void* a, const void* b, void* out, int M, 
   if (M <= kSkinnyRows) return Skinny<false>(a, b, out, nullptr, addend, M, N, K, kActNone, status, stream);
   (void)cudaGetLastError();   // the value returned below must be this launch's own, not an older error of the calling thread
   const uintptr_t all = reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(addend);
-  if (M <= 0 || N <= 0 || K <= 0 || (N % 8) != 0 || (K % 8) != 0 || (all & 15) != 0) return cudaErrorInvalidValue;
+  if (M <= 0 || N <= 0 || K <= 0 || (N % 8) != 0 || (K % 8) != 0 || (all & 15) != 0 || a == nullptr || b == nullptr || out == nullptr)
+    return cudaErrorInvalidValue;
   const int sm_count = SmCount();
   const GemmTiles tiles = PlanTiles(M, N, K, sm_count);
   const int bn = tiles == kTilesPair128 || (tiles == kTilesSingle && N <= 128) ? 128 : 256;
@@ -1580,7 +1582,8 @@ cudaError_t LaunchGemmGroup(const GemmGroupItem* list, int count, unsigned int* 
     }
     const GemmGroupItem& g = *by_length[i];
     const uintptr_t all = reinterpret_cast<uintptr_t>(g.a) | reinterpret_cast<uintptr_t>(g.b) | reinterpret_cast<uintptr_t>(g.out);
-    if (g.M <= 0 || g.N <= 0 || g.K <= 0 || g.N % 8 != 0 || (g.a_transposed ? g.M : g.K) % 8 != 0 || (all & 15) != 0) return cudaErrorInvalidValue;
+    if (g.M <= 0 || g.N <= 0 || g.K <= 0 || g.N % 8 != 0 || (g.a_transposed ? g.M : g.K) % 8 != 0 || (all & 15) != 0 || g.a == nullptr || g.b == nullptr || g.out == nullptr)
+      return cudaErrorInvalidValue;
     if (!(g.a_transposed ? MakeMap(&args.a[i], g.a, g.K, g.M, 64) : MakeMap(&args.a[i], g.a, g.M, g.K, BM)) ||
         !MakeMap(&args.b[i], g.b, g.K, g.N, 64) || !MakeMap(&args.c[i], g.out, g.M, g.N, 32))
       return cudaErrorInvalidValue;
@@ -1763,7 +1766,8 @@ cudaError_t LaunchGemmBf16NN(const void* a, const void* b, void* out, int M, int
 cudaError_t LaunchGemmBf16Gated(const void* a, const void* w, void* h, void* factors, int M, int F, int K, int act,
                                 unsigned int* status, cudaStream_t stream) {
   (void)cudaGetLastError();   // the value returned below must be this launch's own, not an older error of the calling thread
-  if (M <= 0 || F <= 0 || K <= 0 || (K % 8) != 0 || (F % 8) != 0 || (act != kActSilu && act != kActGeluTanh)) return cudaErrorInvalidValue;
+  if (M <= 0 || F <= 0 || K <= 0 || (K % 8) != 0 || (F % 8) != 0 || (act != kActSilu && act != kActGeluTanh) || a == nullptr || w == nullptr || h == nullptr)
+    return cudaErrorInvalidValue;
   if ((reinterpret_cast<uintptr_t>(a) & 15) || (reinterpret_cast<uintptr_t>(w) & 15) || (reinterpret_cast<uintptr_t>(h) & 15) ||
       (reinterpret_cast<uintptr_t>(factors) & 15))
     return cudaErrorInvalidValue;
@@ -1797,7 +1801,8 @@ cudaError_t LaunchGemmBf16Gated(const void* a, const void* w, void* h, void* fac
 cudaError_t LaunchGemmBf16NNGatedGrad(const void* a, const void* b, const void* factors, void* dpre, int M, int F, int K,
                                       unsigned int* status, cudaStream_t stream) {
   (void)cudaGetLastError();
-  if (M <= 0 || F <= 0 || K <= 0 || (K % 8) != 0 || (F % 8) != 0) return cudaErrorInvalidValue;
+  if (M <= 0 || F <= 0 || K <= 0 || (K % 8) != 0 || (F % 8) != 0 || a == nullptr || b == nullptr || factors == nullptr || dpre == nullptr)
+    return cudaErrorInvalidValue;
   if ((reinterpret_cast<uintptr_t>(a) & 15) || (reinterpret_cast<uintptr_t>(b) & 15) || (reinterpret_cast<uintptr_t>(factors) & 15) ||
       (reinterpret_cast<uintptr_t>(dpre) & 15))
     return cudaErrorInvalidValue;
